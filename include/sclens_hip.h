@@ -33,6 +33,18 @@ extern "C" {
 #define SCLENS_ERR_NOCONV 5    /* eigensolver did not converge */
 #define SCLENS_ERR_NAN 6       /* NaN eigenvalue (reference: redo in Float64 on CPU, scLENS.jl:379-381) */
 #define SCLENS_ERR_STATE 7     /* session call out of order */
+#define SCLENS_ERR_WORKSPACE 8 /* the caller's device workspace is too small (*ws_bytes says how much is needed) */
+
+/* element types of the dense operators on device tensors */
+#define SCLENS_DTYPE_F32 0
+#define SCLENS_DTYPE_BF16 1
+#define SCLENS_DTYPE_F16 2
+/* their activations; GELU is z Phi(z), GELU_TANH its tanh approximation */
+#define SCLENS_ACT_NONE 0
+#define SCLENS_ACT_RELU 1
+#define SCLENS_ACT_SILU 2
+#define SCLENS_ACT_GELU 3
+#define SCLENS_ACT_GELU_TANH 4
 
 typedef struct sclens_hip_ctx sclens_hip_ctx;
 typedef struct sclens_hip_session sclens_hip_session;
@@ -196,6 +208,41 @@ int sclens_hip_get_eigvec_f32(sclens_hip_ctx* ctx, const float* X, int64_t N, in
 int sclens_hip_get_denoised_f32(sclens_hip_ctx* ctx, const float* pca_n1, int64_t N, int64_t n_sig, const float* gene_basis_sig,
                                 int64_t M, const double* tgc, const double* mat2_mean, const double* mat2_std,
                                 const double* norm_tgc, const double* cent, float* out);
+
+/* ---------------------------------------------------------------- (C) dense operators on device tensors ------------ */
+/* Products with an epilogue, their gradient and the orthogonal factor by products, on tensors that live on the context's device
+ * (Python: sclens_amd.dense on torch tensors). Unlike the host-array calls above they DO NOT BLOCK: every launch goes to `stream`
+ * (a hipStream_t of the context's device; NULL = that device's default stream, sclens_hip_stream(ctx) = the context's own), nothing
+ * synchronises or allocates, and a call can be captured into a graph. Matrices are ROW-MAJOR with the given leading dimension (elements
+ * between rows, at least the row's length), any alignment of whole elements; outputs must not overlap inputs. Inputs are read, outputs
+ * written, in the element type `dtype` (SCLENS_DTYPE_*); sums are held in fp32 and rounded once. fp32 products are formed from three
+ * bf16 pieces per operand (24 bits, exact) on the matrix cores, whatever the option "precision" says.
+ * Workspace: device memory of the caller, 256-byte aligned, *ws_bytes its size. A call that needs more launches nothing, stores what it
+ * needs in *ws_bytes and returns SCLENS_ERR_WORKSPACE; it may be reused or freed (in stream order) when the call's work is done, so two
+ * calls that may overlap -- other streams, graphs replayed side by side -- need one each. NULL with *ws_bytes = 0 is a size query, or
+ * the call itself when it needs none.
+ * Any size may be 0: an empty sum is 0.
+ *
+ * linear: y = act(x w' + bias) + residual. x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]; preact [M][N] or
+ * NULL receives the argument of the activation, which linear_backward reads. */
+int sclens_hip_linear(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                      const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr, int act, void* y, int64_t ldy,
+                      void* preact, int64_t ldz, void* ws, int64_t* ws_bytes);
+/* Its gradients: dz = dy * act'(preact) (preact may be NULL for SCLENS_ACT_NONE; relu'(0) = 0), dx = dz w, dw = dz' x, dbias = column
+ * sums of dz; the residual's gradient is dy. dx / dw / dbias may be NULL: not computed (x is then only read for dw, w for dx). For
+ * 16-bit types dz is rounded to that type before the two products. Every sum runs in a fixed order: equal inputs give equal bits. */
+int sclens_hip_linear_backward(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* dy,
+                               int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* preact, int64_t ldz,
+                               int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias, void* ws, int64_t* ws_bytes);
+/* Orthogonalisation by Newton-Schulz products of `batch` matrices of rows x cols (batch strides in elements): x0 = g / (|g|_F + eps),
+ * then for each of the `steps` triples (a, b, c) of coef (host, 3 * steps): x <- a x + (b A + c A A) x with A = x x' (x with at most as
+ * many rows as columns; a taller matrix is worked on transposed). Each singular value s goes through a s + b s^3 + c s^5.
+ * (3.4445, -4.7750, 2.0315) brings everything above ~1e-2 of the norm near 1 in five steps (an optimiser's update); (15/8, -5/4, 3/8)
+ * then converges cubically to the orthogonal factor. A matrix of zeros gives zeros; a NaN or an infinity spoils its own matrix only.
+ * Coefficients under which the singular values could pass 1e15 are refused. */
+int sclens_hip_orthogonalize(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void* x,
+                             int64_t stride_x, int64_t ldx, void* y, int64_t stride_y, int64_t ldy, int steps, const double* coef,
+                             double eps, void* ws, int64_t* ws_bytes);
 
 /* ---------------------------------------------------------------- host statistics (no GPU) ----- */
 /* _mp_calculation(L, Lr)  (scLENS.jl:424-459). L_mp_mask[n] gets 1 where b_minus < L < b_plus. */

@@ -14,7 +14,7 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsclens_hip.so")
 
-ERR_NAMES = {1: "ARG", 2: "NO_DEVICE", 3: "OOM", 4: "HIP", 5: "NOCONV", 6: "NAN", 7: "STATE"}
+ERR_NAMES = {1: "ARG", 2: "NO_DEVICE", 3: "OOM", 4: "HIP", 5: "NOCONV", 6: "NAN", 7: "STATE", 8: "WORKSPACE"}
 
 c_f32p = C.POINTER(C.c_float)
 c_f64p = C.POINTER(C.c_double)
@@ -101,6 +101,11 @@ SIGNATURES = {
     "sclens_hip_gram_counts_f32": (C.c_int, [vp, i64, i64, c_i64p, c_i32p, c_f32p, C.c_int, C.c_int, C.c_int, C.c_float, c_f32p]),
     "sclens_hip_get_eigvec_f32": (C.c_int, [vp, c_f32p, i64, i64, i64, c_f32p, c_f32p, c_i64p]),
     "sclens_hip_get_denoised_f32": (C.c_int, [vp, c_f32p, i64, i64, c_f32p, i64, c_f64p, c_f64p, c_f64p, c_f64p, c_f64p, c_f32p]),
+    "sclens_hip_linear": (C.c_int, [vp, vp, C.c_int, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, C.c_int, vp, i64, vp, i64, vp, c_i64p]),
+    "sclens_hip_linear_backward": (C.c_int, [vp, vp, C.c_int, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, vp, i64, vp, i64,
+                                             vp, vp, c_i64p]),
+    "sclens_hip_orthogonalize": (C.c_int, [vp, vp, C.c_int, i64, i64, i64, vp, i64, i64, vp, i64, i64, C.c_int, c_f64p, C.c_double, vp,
+                                           c_i64p]),
     "sclens_mp_calculation": (C.c_int, [c_f64p, i64, c_f64p, i64, c_f64p, c_f64p, c_u8p]),
     "sclens_tw": (C.c_int, [i64, c_f64p, i64, c_f64p, c_f64p, c_f64p, c_f64p]),
     "sclens_mp_check": (C.c_int, [c_f64p, i64, C.c_double, c_f64p, C.POINTER(C.c_int)]),
@@ -156,6 +161,9 @@ SIGNATURES = {
 }
 
 _lib = None
+# True if torch was there when the library was loaded: both then use torch's HIP runtime, so torch's streams (and its graph captures) are
+# valid handles for the library's launches. Otherwise the library brought the system's runtime, which knows nothing of them.
+shares_torch_runtime = False
 
 
 class SclensHipError(RuntimeError):
@@ -166,7 +174,7 @@ class SclensHipError(RuntimeError):
 
 def load():
     """Load the shared library (no GPU needed for loading or for the host statistics)."""
-    global _lib
+    global _lib, shares_torch_runtime
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
@@ -174,6 +182,7 @@ def load():
             f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
             "(or `make -C sclens_amd/csrc`). sclens_amd has no CPU fallback."
         )
+    shares_torch_runtime = "torch" in sys.modules
     lib = C.CDLL(LIB_PATH)
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is not exported

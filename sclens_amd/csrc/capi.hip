@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "dense.h"
 #include "pattern.h"
 
 namespace scl {
@@ -304,6 +305,118 @@ int sclens_hip_get_denoised_f32(sclens_hip_ctx* h, const float* pca_n1, int64_t 
                                 const double* norm_tgc, const double* cent, float* out) {
   CTX_GUARD(h);
   return scl::denoise_host(&h->c, pca_n1, N, n_sig, gene_basis_sig, M, tgc, mat2_mean, mat2_std, norm_tgc, cent, out);
+}
+
+// ---------------------------------------------------------------- dense operators on device tensors
+}  // extern "C"
+namespace {
+// the caller's current device comes back when the call returns: these calls run between a host framework's own
+struct DeviceScope {
+  int prev = -1;
+  explicit DeviceScope(int device) {
+    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+    if (prev != device) (void)hipSetDevice(device);
+    else prev = -1;
+    (void)hipGetLastError();  // an error another library left behind is not this call's
+  }
+  ~DeviceScope() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+// rows x cols elements with leading dimension ld at p; empty matrices need no memory
+bool mat_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, int size, bool optional = false) {
+  if (!p && optional) return true;
+  if (rows == 0 || cols == 0) return true;
+  return p && ld >= cols && ld < ((int64_t)1 << 40) && reinterpret_cast<uintptr_t>(p) % size == 0;
+}
+bool size_ok(int64_t n) { return n >= 0 && n <= 0x7fffffff; }
+template <class F>
+int dense_call(sclens_hip_ctx* h, void* ws, int64_t* ws_bytes, F f) {
+  try {
+    DeviceScope scope(h->c.device);
+    int64_t need = 0;
+    const int rc = f(&need);
+    if (rc == SCLENS_ERR_WORKSPACE) *ws_bytes = need;
+    return rc;
+  } catch (const std::exception& e) {
+    return SCLENS_ERR_OOM;
+  } catch (...) {
+    return SCLENS_ERR_HIP;
+  }
+}
+const char* dense_common(int dtype, const void* ws, const int64_t* ws_bytes) {
+  if (dtype < 0 || dtype > 2) return "unknown element type";
+  if (!ws_bytes || *ws_bytes < 0 || (!ws && *ws_bytes > 0)) return "workspace: a pointer and its size, or NULL and 0";
+  if (reinterpret_cast<uintptr_t>(ws) % 256 != 0) return "the workspace has to start on 256 bytes";
+  return nullptr;
+}
+}  // namespace
+extern "C" {
+int sclens_hip_linear(sclens_hip_ctx* h, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
+                      int64_t ldw, const void* bias, const void* residual, int64_t ldr, int act, void* y, int64_t ldy, void* preact,
+                      int64_t ldz, void* ws, int64_t* ws_bytes) {
+  if (!h) return SCLENS_ERR_ARG;
+  if (const char* bad = dense_common(dtype, ws, ws_bytes)) return h->c.fail(SCLENS_ERR_ARG, std::string("linear: ") + bad);
+  const int size = dtype == SCLENS_DTYPE_F32 ? 4 : 2;
+  if (!size_ok(M) || !size_ok(N) || !size_ok(K)) return h->c.fail(SCLENS_ERR_ARG, "linear: sizes have to lie in [0, 2^31)");
+  if (act < 0 || act > 4) return h->c.fail(SCLENS_ERR_ARG, "linear: unknown activation");
+  if (!mat_ok(x, M, K, ldx, size) || !mat_ok(w, N, K, ldw, size) || !mat_ok(bias, 1, N, N, size, true) ||
+      !mat_ok(residual, M, N, ldr, size, true) || !mat_ok(y, M, N, ldy, size) || !mat_ok(preact, M, N, ldz, size, true))
+    return h->c.fail(SCLENS_ERR_ARG, "linear: null or misaligned matrix, or a leading dimension below the row length");
+  return dense_call(h, ws, ws_bytes, [&](int64_t* need) {
+    scl::LinearArgs a;
+    a.dtype = dtype; a.act = act;
+    a.M = M; a.N = N; a.K = K;
+    a.x = x; a.w = w; a.bias = bias; a.res = residual; a.y = y; a.pre = preact;
+    a.ldx = ldx; a.ldw = ldw; a.ldr = ldr; a.ldy = ldy; a.ldz = ldz;
+    return scl::linear_forward(&h->c, static_cast<hipStream_t>(stream), a, ws, *ws_bytes, need);
+  });
+}
+int sclens_hip_linear_backward(sclens_hip_ctx* h, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t lddy,
+                               const void* x, int64_t ldx, const void* w, int64_t ldw, const void* preact, int64_t ldz, int act, void* dx,
+                               int64_t lddx, void* dw, int64_t lddw, void* dbias, void* ws, int64_t* ws_bytes) {
+  if (!h) return SCLENS_ERR_ARG;
+  if (const char* bad = dense_common(dtype, ws, ws_bytes)) return h->c.fail(SCLENS_ERR_ARG, std::string("linear_backward: ") + bad);
+  const int size = dtype == SCLENS_DTYPE_F32 ? 4 : 2;
+  if (!size_ok(M) || !size_ok(N) || !size_ok(K)) return h->c.fail(SCLENS_ERR_ARG, "linear_backward: sizes have to lie in [0, 2^31)");
+  if (act < 0 || act > 4) return h->c.fail(SCLENS_ERR_ARG, "linear_backward: unknown activation");
+  if (act != SCLENS_ACT_NONE && !preact && M > 0 && N > 0)
+    return h->c.fail(SCLENS_ERR_ARG, "linear_backward: an activation's gradient needs the pre-activation");
+  if (!mat_ok(dy, M, N, lddy, size) || !mat_ok(x, M, K, ldx, size, !dw) || !mat_ok(w, N, K, ldw, size, !dx) ||
+      !mat_ok(preact, M, N, ldz, size, true) || !mat_ok(dx, M, K, lddx, size, true) || !mat_ok(dw, N, K, lddw, size, true) ||
+      !mat_ok(dbias, 1, N, N, size, true))
+    return h->c.fail(SCLENS_ERR_ARG, "linear_backward: null or misaligned matrix, or a leading dimension below the row length");
+  return dense_call(h, ws, ws_bytes, [&](int64_t* need) {
+    scl::LinearBwdArgs a;
+    a.dtype = dtype; a.act = act;
+    a.M = M; a.N = N; a.K = K;
+    a.dy = dy; a.x = x; a.w = w; a.pre = preact; a.dx = dx; a.dw = dw; a.db = dbias;
+    a.lddy = lddy; a.ldx = ldx; a.ldw = ldw; a.ldz = ldz; a.lddx = lddx; a.lddw = lddw;
+    return scl::linear_backward(&h->c, static_cast<hipStream_t>(stream), a, ws, *ws_bytes, need);
+  });
+}
+int sclens_hip_orthogonalize(sclens_hip_ctx* h, void* stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void* x,
+                             int64_t stride_x, int64_t ldx, void* y, int64_t stride_y, int64_t ldy, int steps, const double* coef, double eps,
+                             void* ws, int64_t* ws_bytes) {
+  if (!h) return SCLENS_ERR_ARG;
+  if (const char* bad = dense_common(dtype, ws, ws_bytes)) return h->c.fail(SCLENS_ERR_ARG, std::string("orthogonalize: ") + bad);
+  const int size = dtype == SCLENS_DTYPE_F32 ? 4 : 2;
+  if (!size_ok(batch) || !size_ok(rows) || !size_ok(cols)) return h->c.fail(SCLENS_ERR_ARG, "orthogonalize: sizes have to lie in [0, 2^31)");
+  if (steps < 1 || steps > 1000 || !coef) return h->c.fail(SCLENS_ERR_ARG, "orthogonalize: 1 to 1000 steps, three coefficients each");
+  if (!(eps >= 0.0)) return h->c.fail(SCLENS_ERR_ARG, "orthogonalize: eps has to be >= 0");
+  const bool some = batch > 0 && rows > 0 && cols > 0;
+  if (!mat_ok(x, some ? 1 : 0, cols, ldx, size) || !mat_ok(y, some ? 1 : 0, cols, ldy, size) ||
+      (some && batch > 1 && (stride_x < 0 || stride_y < (rows - 1) * ldy + cols)))
+    return h->c.fail(SCLENS_ERR_ARG, "orthogonalize: null or misaligned matrix, a leading dimension below the row length, or outputs that overlap");
+  return dense_call(h, ws, ws_bytes, [&](int64_t* need) {
+    scl::OrthArgs a;
+    a.dtype = dtype;
+    a.batch = batch; a.rows = rows; a.cols = cols;
+    a.x = x; a.y = y;
+    a.sx = stride_x; a.ldx = ldx; a.sy = stride_y; a.ldy = ldy;
+    a.steps = steps; a.coef = coef; a.eps = eps;
+    return scl::orthogonalize(&h->c, static_cast<hipStream_t>(stream), a, ws, *ws_bytes, need);
+  });
 }
 
 int sclens_hip_session_create(sclens_hip_ctx* h, int64_t N, int64_t M, const int64_t* colptr, const int32_t* rowval,

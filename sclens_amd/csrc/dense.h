@@ -1,0 +1,89 @@
+// Dense operators on device tensors: the product family behind sclens_hip_linear, sclens_hip_linear_backward and
+// sclens_hip_orthogonalize (dense_gemm.hip: the products; dense_ops.hip: the operators).
+#pragma once
+#include "common.h"
+
+namespace scl {
+
+// element types of the C ABI (SCLENS_DTYPE_*); D_PL3 is internal: an fp32 value held as three bf16 pieces in three planes
+enum { D_F32 = 0, D_BF16 = 1, D_F16 = 2, D_PL3 = 3 };
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
+
+// A matrix on the device: element (r, c) of batch b at p + b * batch + r * ld + c; plane: distance of the planes of D_PL3.
+struct Mat {
+  void* p = nullptr;
+  int64_t ld = 0, batch = 0, plane = 0;
+  int vec = 0;  // 16-byte loads / stores of 8 columns are aligned
+  int pad = 0;  // rows / columns up to the next multiple of 8 exist and are written as zeros (images of the library)
+};
+
+// C[b] = epilogue(alpha * A[b] B[b]'), A [M][K], B [N][K], K contiguous.
+struct Product {
+  int type = D_BF16;  // D_BF16 / D_F16: what the 16-bit images hold; D_PL3: three bf16 planes each, six products per term
+  Mat A, B;
+  int64_t M = 0, N = 0, K = 0;
+  int batch = 1;
+  int symmetric = 0;  // M == N and C is symmetric: tiles on / below the diagonal, mirrored
+  // epilogue: v = alpha acc + bias[col]; pre = v; v = act(v) + beta res; out = v; outT (transposed) = v
+  float alpha = 1.f, beta = 0.f;
+  int act = ACT_NONE;
+  const void* bias = nullptr;
+  Mat res, pre, out, outT;
+  int out_type = D_BF16, res_type = D_BF16;  // pre and bias have out_type
+  // fp32 slabs of split contractions (see product_slab_bytes); nullptr: the contraction is never split
+  float* slabs = nullptr;
+  int64_t slab_bytes = 0;
+};
+int64_t product_slab_bytes(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric);
+int product(Ctx* ctx, hipStream_t st, const Product& p);
+
+// 16-bit image (D_F32: three bf16 planes) of src (element (r, k) at r * ld + k, transposed: k * ld + r), rows x K, K padded with zeros
+// to image_ld(K)
+static inline int64_t image_ld(int64_t K) { return round_up(K > 0 ? K : 1, 64); }
+static inline int64_t image_elems(int64_t rows, int64_t K) { return round_up(rows, 8) * image_ld(K); }
+static inline int planes_of(int dtype) { return dtype == D_F32 ? 3 : 1; }
+int pack_image(Ctx* ctx, hipStream_t st, int dtype, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img);
+
+struct LinearArgs {
+  int dtype = D_F32, act = ACT_NONE;
+  int64_t M = 0, N = 0, K = 0;
+  const void *x = nullptr, *w = nullptr, *bias = nullptr, *res = nullptr;
+  void *y = nullptr, *pre = nullptr;
+  int64_t ldx = 0, ldw = 0, ldr = 0, ldy = 0, ldz = 0;
+};
+struct LinearBwdArgs {
+  int dtype = D_F32, act = ACT_NONE;
+  int64_t M = 0, N = 0, K = 0;
+  const void *dy = nullptr, *x = nullptr, *w = nullptr, *pre = nullptr;
+  void *dx = nullptr, *dw = nullptr, *db = nullptr;
+  int64_t lddy = 0, ldx = 0, ldw = 0, ldz = 0, lddx = 0, lddw = 0;
+};
+struct OrthArgs {
+  int dtype = D_F32;
+  int64_t batch = 0, rows = 0, cols = 0;
+  const void* x = nullptr;
+  void* y = nullptr;
+  int64_t sx = 0, ldx = 0, sy = 0, ldy = 0;
+  int steps = 0;
+  const double* coef = nullptr;  // steps x (a, b, c), host
+  double eps = 0;
+};
+// *need: bytes of scratch the call wants; launched only if ws_bytes >= *need (SCLENS_ERR_WORKSPACE otherwise)
+int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
+int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
+int orthogonalize(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
+
+// scratch handed out in order, 256-byte aligned; with base == nullptr only the sizes are summed
+struct Carve {
+  char* base;
+  int64_t used = 0;
+  explicit Carve(void* b) : base(static_cast<char*>(b)) {}
+  template <class T>
+  T* take(int64_t count) {
+    const int64_t off = used;
+    used += round_up(count * (int64_t)sizeof(T), 256);
+    return base ? reinterpret_cast<T*>(base + off) : nullptr;
+  }
+};
+
+}  // namespace scl

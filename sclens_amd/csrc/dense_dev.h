@@ -1,0 +1,155 @@
+// Device helpers of the dense operators: element types, the three-plane form of fp32, activations.
+#pragma once
+#include "dense.h"
+
+namespace scl {
+
+__host__ __device__ constexpr int64_t round_up8(int64_t x) { return (x + 7) & ~(int64_t)7; }
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+struct __attribute__((packed, aligned(2))) u16x8_any { unsigned short v[8]; };  // 16 bytes at any element address
+struct __attribute__((packed, aligned(4))) f32x8_any { float v[8]; };
+
+__device__ __forceinline__ float bf16_to_f32(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
+__device__ __forceinline__ unsigned short f32_to_bf16(float v) {  // round to nearest, ties to even; NaN stays NaN
+  return __builtin_bit_cast(unsigned short, (__bf16)v);
+}
+__device__ __forceinline__ float f16_to_f32(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
+__device__ __forceinline__ unsigned short f32_to_f16(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
+
+// v = p0 + p1 + p2 exactly, each piece a bf16: p0 is v rounded to 8 bits, the remainder (exact in fp32, at most 2^-8 |v|) gives p1,
+// the next one (at most 8 bits left) is p2. Infinities and NaN sit in p0 alone. A v that would round up to infinity is cut instead.
+__device__ __forceinline__ void split3(float v, unsigned short& p0, unsigned short& p1, unsigned short& p2) {
+  const unsigned u = __float_as_uint(v);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    p0 = f32_to_bf16(v);
+    p1 = p2 = 0;
+    return;
+  }
+  p0 = f32_to_bf16(v);
+  if ((p0 & 0x7f80u) == 0x7f80u) p0 = (unsigned short)(u >> 16);
+  const float r1 = v - bf16_to_f32(p0);
+  p1 = f32_to_bf16(r1);
+  p2 = f32_to_bf16(r1 - bf16_to_f32(p1));
+}
+
+template <int T> struct Elem;  // 16-bit and fp32 elements
+template <> struct Elem<D_F32> {
+  typedef float type;
+  static __device__ __forceinline__ float ld(const float* p) { return *p; }
+  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
+};
+template <> struct Elem<D_BF16> {
+  typedef unsigned short type;
+  static __device__ __forceinline__ float ld(const unsigned short* p) { return bf16_to_f32(*p); }
+  static __device__ __forceinline__ void st(unsigned short* p, float v) { *p = f32_to_bf16(v); }
+};
+template <> struct Elem<D_F16> {
+  typedef unsigned short type;
+  static __device__ __forceinline__ float ld(const unsigned short* p) { return f16_to_f32(*p); }
+  static __device__ __forceinline__ void st(unsigned short* p, float v) { *p = f32_to_f16(v); }
+};
+
+// eight consecutive elements at off (elements from m.p); `n` of them are inside the matrix (the rest read as 0 / are not written,
+// or, for an image of the library (m.pad), are written as zeros by the caller passing n = 8)
+template <int T>
+__device__ __forceinline__ void load8(const Mat& m, int64_t off, int n, float v[8]) {
+  if constexpr (T == D_PL3) {
+    const unsigned short* p = static_cast<const unsigned short*>(m.p) + off;
+    const u16x8 a = *reinterpret_cast<const u16x8*>(p), b = *reinterpret_cast<const u16x8*>(p + m.plane),
+                c = *reinterpret_cast<const u16x8*>(p + 2 * m.plane);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (bf16_to_f32(a[e]) + bf16_to_f32(b[e])) + bf16_to_f32(c[e]);
+  } else {
+    typedef typename Elem<T>::type E;
+    const E* p = static_cast<const E*>(m.p) + off;
+    if (n >= 8 && m.vec) {
+      if constexpr (T == D_F32) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+      } else {
+        const u16x8 a = *reinterpret_cast<const u16x8*>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned short h = a[e];
+          v[e] = Elem<T>::ld(&h);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? Elem<T>::ld(p + e) : 0.f;
+    }
+  }
+}
+template <int T>
+__device__ __forceinline__ void store8(const Mat& m, int64_t off, int n, const float v[8]) {
+  if constexpr (T == D_PL3) {
+    unsigned short* p = static_cast<unsigned short*>(m.p) + off;
+    u16x8 a, b, c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      unsigned short x, y, z;
+      split3(v[e], x, y, z);
+      a[e] = x; b[e] = y; c[e] = z;
+    }
+    *reinterpret_cast<u16x8*>(p) = a;
+    *reinterpret_cast<u16x8*>(p + m.plane) = b;
+    *reinterpret_cast<u16x8*>(p + 2 * m.plane) = c;
+  } else {
+    typedef typename Elem<T>::type E;
+    E* p = static_cast<E*>(m.p) + off;
+    if (n >= 8 && m.vec) {
+      if constexpr (T == D_F32) {
+        f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+        *reinterpret_cast<f32x4*>(p) = a;
+        *reinterpret_cast<f32x4*>(p + 4) = b;
+      } else {
+        u16x8 a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          unsigned short h;
+          Elem<T>::st(&h, v[e]);
+          a[e] = h;
+        }
+        *reinterpret_cast<u16x8*>(p) = a;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) Elem<T>::st(p + e, v[e]);
+    }
+  }
+}
+
+// activations and their derivatives in fp32 (the value is rounded once, when it is stored)
+__device__ __forceinline__ float act_apply(float z, int act) {
+  switch (act) {
+    case ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+    case ACT_SILU: return z / (1.f + expf(-z));
+    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    case ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_grad(float z, int act) {
+  switch (act) {
+    case ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    case ACT_SILU: {
+      const float s = 1.f / (1.f + expf(-z));
+      return s * (1.f + z * (1.f - s));
+    }
+    case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+    case ACT_GELU_TANH: {
+      const float u = 0.79788456f * (z + 0.044715f * z * z * z), t = tanhf(u);
+      return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * z * z);
+    }
+    default: return 1.f;
+  }
+}
+
+}  // namespace scl

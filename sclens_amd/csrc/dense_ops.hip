@@ -1,0 +1,413 @@
+// Dense operators on device tensors (sclens_amd/dense.py):
+//   linear            y = act(x w' + b) + r
+//   linear_backward   dz = dy act'(z),  dx = dz w,  dw = dz' x,  db = column sums of dz
+//   orthogonalize     x0 = g / (|g|_F + eps);  per step (a, b, c): A = x x',  x <- a x + (b A + c A A) x
+// The products are those of dense_gemm.hip; here are the passes around them and the order of the launches. Every launch goes to the
+// caller's stream, scratch is the caller's, nothing synchronises: a call can be captured into a graph.
+#include <algorithm>
+#include <cmath>
+
+#include "dense_dev.h"
+
+namespace scl {
+
+namespace {
+int no_room(Ctx* ctx, int64_t need) {
+  return ctx->fail(SCLENS_ERR_WORKSPACE, "this call needs " + std::to_string(need) + " bytes of device workspace");
+}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// a 16-bit matrix whose rows start on 16 bytes and whose contraction is whole 8-column chunks feeds the products as it lies
+bool direct(int dtype, const void* p, int64_t ld, int64_t K) { return dtype != D_F32 && ld % 8 == 0 && K % 8 == 0 && aligned16(p); }
+
+Mat user_mat(const void* p, int64_t ld, int64_t batch = 0) {
+  Mat m;
+  m.p = const_cast<void*>(p);
+  m.ld = ld;
+  m.batch = batch;
+  m.vec = ld % 8 == 0 && batch % 8 == 0 && aligned16(p);
+  return m;
+}
+Mat image_of(Carve& c, int dtype, int64_t rows, int64_t K, int64_t batch = 1) {
+  Mat m;
+  m.batch = image_elems(rows, K);
+  m.plane = m.batch * batch;
+  m.ld = image_ld(K);
+  m.vec = m.pad = 1;
+  m.p = c.take<unsigned short>(m.plane * planes_of(dtype));
+  return m;
+}
+int image_type(int dtype) { return dtype == D_F32 ? D_PL3 : dtype; }
+}  // namespace
+
+// ------------------------------------------------------------------ linear
+int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
+  Carve c(ws);
+  const bool dx = direct(a.dtype, a.x, a.ldx, a.K), dw = direct(a.dtype, a.w, a.ldw, a.K);
+  Product p;
+  p.type = image_type(a.dtype);
+  p.out_type = p.res_type = a.dtype;
+  p.M = a.M; p.N = a.N; p.K = a.K;
+  p.A = dx ? user_mat(a.x, a.ldx) : image_of(c, a.dtype, a.M, a.K);
+  p.B = dw ? user_mat(a.w, a.ldw) : image_of(c, a.dtype, a.N, a.K);
+  p.slab_bytes = product_slab_bytes(a.M, a.N, a.K, 1, p.type, 0);
+  if (p.slab_bytes) p.slabs = c.take<float>(p.slab_bytes / 4);
+  *need = c.used;
+  if (c.used > ws_bytes) return no_room(ctx, c.used);
+  if (a.M == 0 || a.N == 0) return SCLENS_OK;
+  if (!dx) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, false, a.M, a.K, &p.A));
+  if (!dw) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, false, a.N, a.K, &p.B));
+  p.bias = a.bias;
+  p.act = a.act;
+  if (a.res) { p.res = user_mat(a.res, a.ldr); p.beta = 1.f; }
+  if (a.pre) p.pre = user_mat(a.pre, a.ldz);
+  p.out = user_mat(a.y, a.ldy);
+  return product(ctx, st, p);
+}
+
+// ------------------------------------------------------------------ linear, backward
+// dz = dy act'(z) for a 64 x 64 block: its image (contraction over the columns), the image of its transpose (contraction over the
+// rows) and the block's column sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the
+// saved pre-activation and the gradient that comes in already are.
+template <int T>
+__global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, Mat imgT, float* __restrict__ part) {
+  constexpr int IT = T == D_F32 ? D_PL3 : T;
+  __shared__ float L[64][65];
+  const int64_t nb = (N + 63) / 64, mb = blockIdx.x / nb;
+  const int64_t m0 = mb * 64, n0 = (blockIdx.x % nb) * 64;
+  const int tid = threadIdx.x, cc = (tid & 7) * 8;
+  const int64_t col = n0 + cc;
+  const int nin = (int)max((int64_t)0, min((int64_t)8, N - col));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int lr = i * 32 + (tid >> 3);
+    const int64_t row = m0 + lr;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (row < M && nin > 0) {
+      load8<T>(dy, row * dy.ld + col, nin, v);
+      if (act != ACT_NONE) {
+        float zz[8];
+        load8<T>(z, row * z.ld + col, nin, zz);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < nin) v[e] *= act_grad(zz[e], act);
+      }
+    }
+    if (img.p && row < M) store8<IT>(img, row * img.ld + col, 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) L[lr][cc + e] = v[e];
+  }
+  __syncthreads();
+  if (imgT.p) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lc = i * 32 + (tid >> 3), lr = (tid & 7) * 8;
+      if (n0 + lc < N) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = L[lr + e][lc];
+        store8<IT>(imgT, (n0 + lc) * imgT.ld + m0 + lr, 8, v);
+      }
+    }
+  }
+  if (part && tid < 64 && n0 + tid < N) {
+    float s = 0.f;
+    for (int r = 0; r < 64; ++r) s += L[r][tid];
+    part[mb * N + n0 + tid] = s;
+  }
+}
+template <int T>
+__global__ __launch_bounds__(256) void k_colsum_join(const float* __restrict__ part, int64_t nmb, int64_t N, typename Elem<T>::type* __restrict__ out) {
+  __shared__ double S[4][64];
+  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  double s = 0.0;
+  if (col < N)
+    for (int64_t b = g; b < nmb; b += 4) s += (double)part[b * N + col];
+  S[g][c] = s;
+  __syncthreads();
+  if (g == 0 && col < N) Elem<T>::st(out + col, (float)((S[0][c] + S[1][c]) + (S[2][c] + S[3][c])));
+}
+
+int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
+  Carve c(ws);
+  const int64_t nmb = (a.M + 63) / 64;
+  const bool as_is = a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
+  Mat dz, dzT, wT, xT;
+  if (a.dx) {
+    dz = as_is ? user_mat(a.dy, a.lddy) : image_of(c, a.dtype, a.M, a.N);
+    wT = image_of(c, a.dtype, a.K, a.N);
+  }
+  if (a.dw) {
+    dzT = image_of(c, a.dtype, a.N, a.M);
+    xT = image_of(c, a.dtype, a.K, a.M);
+  }
+  float* part = a.db ? c.take<float>(std::max<int64_t>(1, nmb * a.N)) : nullptr;
+  const int type = image_type(a.dtype);
+  const int64_t slab_dx = a.dx ? product_slab_bytes(a.M, a.K, a.N, 1, type, 0) : 0;
+  const int64_t slab_dw = a.dw ? product_slab_bytes(a.N, a.K, a.M, 1, type, 0) : 0;
+  const int64_t slab = std::max(slab_dx, slab_dw);
+  float* slabs = slab ? c.take<float>(slab / 4) : nullptr;
+  *need = c.used;
+  if (c.used > ws_bytes) return no_room(ctx, c.used);
+
+  if (a.M > 0 && a.N > 0 && (a.dw || a.db || (a.dx && !as_is))) {
+    const int64_t blocks = nmb * ((a.N + 63) / 64);
+    if (blocks > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
+    const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
+    Mat img = as_is || !a.dx ? Mat() : dz;
+#define SCL_DZ(T) hipLaunchKernelGGL(k_dz<T>, dim3((unsigned)blocks), dim3(256), 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part)
+    if (a.dtype == D_F32) SCL_DZ(D_F32);
+    else if (a.dtype == D_BF16) SCL_DZ(D_BF16);
+    else SCL_DZ(D_F16);
+#undef SCL_DZ
+    SCL_HIP(ctx, hipGetLastError());
+  }
+  if (a.db && a.N > 0) {
+    const dim3 grid((unsigned)((a.N + 63) / 64));
+    if (a.dtype == D_F32) hipLaunchKernelGGL(k_colsum_join<D_F32>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<float*>(a.db));
+    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_colsum_join<D_BF16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
+    else hipLaunchKernelGGL(k_colsum_join<D_F16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
+    SCL_HIP(ctx, hipGetLastError());
+  }
+  Product p;
+  p.type = type;
+  p.out_type = p.res_type = a.dtype;
+  p.slabs = slabs;
+  p.slab_bytes = slab;
+  if (a.dx && a.M > 0 && a.K > 0) {
+    SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, true, a.K, a.N, &wT));
+    p.M = a.M; p.N = a.K; p.K = a.N;
+    p.A = dz; p.B = wT;
+    p.out = user_mat(a.dx, a.lddx);
+    SCL_TRY(product(ctx, st, p));
+  }
+  if (a.dw && a.N > 0 && a.K > 0) {
+    SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, true, a.K, a.M, &xT));
+    p.M = a.N; p.N = a.K; p.K = a.M;
+    p.A = dzT; p.B = xT;
+    p.out = user_mat(a.dw, a.lddw);
+    SCL_TRY(product(ctx, st, p));
+  }
+  return SCLENS_OK;
+}
+
+// ------------------------------------------------------------------ orthogonalize
+// |g|_F^2 of each matrix: partial sums in fp64 (fp32 squares of large entries overflow), added in a fixed order by whoever needs them
+template <int T>
+__global__ __launch_bounds__(256) void k_sumsq(const typename Elem<T>::type* __restrict__ x, int64_t batch, int64_t ld, int64_t rows, int64_t cols,
+                                               int tpr, double* __restrict__ part) {
+  __shared__ double S[256];
+  const int tid = threadIdx.x, tr = tid / tpr, tc = tid % tpr, rpb = 256 / tpr;
+  const auto* p = x + (int64_t)blockIdx.y * batch;
+  double s = 0.0;
+  for (int64_t r = (int64_t)blockIdx.x * rpb + tr; r < rows; r += (int64_t)gridDim.x * rpb)
+    for (int64_t c = tc; c < cols; c += tpr) {
+      const double v = (double)Elem<T>::ld(p + r * ld + c);
+      s += v * v;
+    }
+  S[tid] = s;
+  __syncthreads();
+  for (int w = 128; w > 0; w >>= 1) {
+    if (tid < w) S[tid] += S[tid + w];
+    __syncthreads();
+  }
+  if (tid == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = S[0];
+}
+
+// x0 = scale g / (|g|_F + eps), a 64 x 64 block: its image and the image of its transpose. `img` has the orientation of the source.
+template <int T, int IT>
+__global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64_t cols, const double* __restrict__ part, int nparts, double eps,
+                                                    double scale, Mat img, Mat imgT) {
+  __shared__ float L[64][65];
+  __shared__ double factor;
+  const int64_t nb = (cols + 63) / 64, b = blockIdx.y;
+  const int64_t m0 = (blockIdx.x / nb) * 64, n0 = (blockIdx.x % nb) * 64;
+  const int tid = threadIdx.x, cc = (tid & 7) * 8;
+  if (tid == 0) {
+    double s = 0.0;
+    for (int i = 0; i < nparts; ++i) s += part[b * nparts + i];
+    factor = scale / (sqrt(s) + eps);
+  }
+  __syncthreads();
+  const double f = factor;
+  const int64_t col = n0 + cc;
+  const int nin = (int)max((int64_t)0, min((int64_t)8, cols - col));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int lr = i * 32 + (tid >> 3);
+    const int64_t row = m0 + lr;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (row < rows && nin > 0) {
+      load8<T>(src, b * src.batch + row * src.ld + col, nin, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < nin ? (float)((double)v[e] * f) : 0.f;
+    }
+    if (row < rows) store8<IT>(img, b * img.batch + row * img.ld + col, 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) L[lr][cc + e] = v[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int lc = i * 32 + (tid >> 3), lr = (tid & 7) * 8;
+    if (n0 + lc < cols) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = L[lr + e][lc];
+      store8<IT>(imgT, b * imgT.batch + (n0 + lc) * imgT.ld + m0 + lr, 8, v);
+    }
+  }
+}
+
+namespace {
+// largest |a s + b s^3 + c s^5| over 0 <= s <= B: the singular values' bound after a step
+double step_bound(double a, double b, double c, double B) {
+  auto f = [&](double s) { return std::fabs(((c * s * s + b) * s * s + a) * s); };
+  double best = f(B);
+  // a + 3 b q + 5 c q^2 = 0, q = s^2
+  auto at = [&](double q) {
+    if (q > 0 && q < B * B) best = std::max(best, f(std::sqrt(q)));
+  };
+  if (c != 0.0) {
+    const double d = 9 * b * b - 20 * a * c;
+    if (d >= 0) {
+      at((-3 * b + std::sqrt(d)) / (10 * c));
+      at((-3 * b - std::sqrt(d)) / (10 * c));
+    }
+  } else if (b != 0.0)
+    at(-a / (3 * b));
+  return best;
+}
+// the power of two that brings a bound just under 2^14 (fp16 holds 65504: a factor of four is left for rounding)
+double pow2_scale(double bound) { return std::ldexp(1.0, 13 - std::ilogb(std::max(bound, 1e-30))); }
+}  // namespace
+
+static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
+  // x has m <= n: a matrix with more rows than columns is worked on transposed
+  const bool tall = a.rows > a.cols;
+  const int64_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
+  // 16-bit inputs: x, A and b A + c A A between the products are fp16 under power-of-two scales from the bound of the singular values
+  // (11 bits: eight times finer than bf16, so that what five steps amplify stays below the rounding of a bf16 result). fp32 inputs:
+  // three bf16 planes, exact.
+  const bool f32 = a.dtype == D_F32;
+  const int IT = f32 ? D_PL3 : D_F16, img_dtype = f32 ? D_F32 : D_F16;
+  Carve c(ws);
+  const int64_t elems = m * n;
+  const int nparts = (int)std::min<int64_t>(64, std::max<int64_t>(1, elems / 8192));
+  double* part = c.take<double>(a.batch * nparts);
+  Mat X[2], XT[2];
+  for (int i = 0; i < (a.steps > 1 ? 2 : 1); ++i) {
+    X[i] = image_of(c, img_dtype, m, n, a.batch);
+    XT[i] = image_of(c, img_dtype, n, m, a.batch);
+  }
+  Mat A = image_of(c, img_dtype, m, m, a.batch), P = image_of(c, img_dtype, m, m, a.batch);
+  int64_t slab = std::max(product_slab_bytes(m, m, n, (int)a.batch, IT, 1), product_slab_bytes(m, m, m, (int)a.batch, IT, 1));
+  slab = std::max(slab, product_slab_bytes(m, n, m, (int)a.batch, IT, 0));
+  float* slabs = slab ? c.take<float>(slab / 4) : nullptr;
+  *need = c.used;
+  if (c.used > ws_bytes) return no_room(ctx, c.used);
+
+  const Mat src = user_mat(a.x, a.ldx, a.sx), dst = user_mat(a.y, a.ldy, a.sy);
+  int tpr = 1;
+  while (tpr < 256 && tpr < a.cols) tpr *= 2;
+  const int64_t tiles = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
+  if (tiles > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: too many elements");
+  double bound = 1.0;
+  double s_x = f32 ? 1.0 : pow2_scale(bound);
+  {
+    const dim3 g1((unsigned)nparts, (unsigned)a.batch), g2((unsigned)tiles, (unsigned)a.batch), blk(256);
+    Mat& i0 = tall ? XT[0] : X[0];
+    Mat& i1 = tall ? X[0] : XT[0];
+#define SCL_START(T, I)                                                                                                             \
+  do {                                                                                                                              \
+    hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, static_cast<const Elem<T>::type*>(a.x), a.sx, a.ldx, a.rows, a.cols, tpr, part); \
+    hipLaunchKernelGGL((k_orth_start<T, I>), g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
+  } while (0)
+    if (a.dtype == D_F32) SCL_START(D_F32, D_PL3);
+    else if (a.dtype == D_BF16) SCL_START(D_BF16, D_F16);
+    else SCL_START(D_F16, D_F16);
+#undef SCL_START
+    SCL_HIP(ctx, hipGetLastError());
+  }
+  for (int t = 0; t < a.steps; ++t) {
+    const double ca = a.coef[3 * t], cb = a.coef[3 * t + 1], cc = a.coef[3 * t + 2];
+    const bool last = t + 1 == a.steps;
+    const Mat &x = X[t & 1], &xt = XT[t & 1];
+    const double next = step_bound(ca, cb, cc, bound);
+    const double s_a = f32 ? 1.0 : pow2_scale(bound * bound);
+    const double s_p = f32 ? 1.0 : pow2_scale(std::fabs(cb) * bound * bound + std::fabs(cc) * bound * bound * bound * bound);
+    const double s_n = f32 || last ? 1.0 : pow2_scale(next);
+    Product p;
+    p.type = IT;
+    p.batch = (int)a.batch;
+    p.slabs = slabs;
+    p.slab_bytes = slab;
+    p.out_type = p.res_type = IT;
+    p.symmetric = 1;
+    p.M = p.N = m;
+    // A = x x'
+    p.K = n;
+    p.A = p.B = x;
+    p.out = A;
+    p.alpha = (float)(s_a / (s_x * s_x));
+    SCL_TRY(product(ctx, st, p));
+    // P = b A + c A A
+    p.K = m;
+    p.A = p.B = p.res = A;
+    p.out = P;
+    p.alpha = (float)(cc * s_p / (s_a * s_a));
+    p.beta = (float)(cb * s_p / s_a);
+    SCL_TRY(product(ctx, st, p));
+    // x <- a x + P x
+    p.symmetric = 0;
+    p.N = n;
+    p.A = P;
+    p.B = xt;
+    p.res = x;
+    p.alpha = (float)(s_n / (s_p * s_x));
+    p.beta = (float)(ca * s_n / s_x);
+    if (last) {
+      p.out_type = a.dtype;
+      p.out = tall ? Mat() : dst;
+      p.outT = tall ? dst : Mat();
+    } else {
+      p.out = X[(t + 1) & 1];
+      p.outT = XT[(t + 1) & 1];
+    }
+    SCL_TRY(product(ctx, st, p));
+    bound = next;
+    s_x = s_n;
+  }
+  return SCLENS_OK;
+}
+
+int orthogonalize(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
+  *need = 0;
+  if (a.batch == 0 || a.rows == 0 || a.cols == 0) return SCLENS_OK;
+  double bound = 1.0;
+  for (int t = 0; t < a.steps; ++t) {
+    bound = step_bound(a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2], bound);
+    if (!(bound < 1e15)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: these coefficients let the singular values grow without bound");
+  }
+  const int64_t chunk = 32768;  // matrices per launch (a grid holds 65535 in y)
+  OrthArgs b = a;
+  b.batch = std::min(a.batch, chunk);
+  for (int64_t b0 = 0; b0 < a.batch; b0 += chunk) {
+    b.batch = std::min(chunk, a.batch - b0);
+    const int size = a.dtype == D_F32 ? 4 : 2;
+    b.x = static_cast<const char*>(a.x) + b0 * a.sx * size;
+    b.y = static_cast<char*>(a.y) + b0 * a.sy * size;
+    int64_t n1 = 0;
+    const int rc = orth_chunk(ctx, st, b, ws, ws_bytes, &n1);
+    *need = std::max(*need, n1);
+    if (rc != SCLENS_OK) return rc;
+  }
+  return SCLENS_OK;
+}
+
+}  // namespace scl

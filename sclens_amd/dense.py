@@ -1,0 +1,240 @@
+"""Dense operators on torch tensors of one MI355X: the product with bias, activation and residual, its gradient, and the orthogonal
+factor of a matrix by products. They stand beside the per-call drop-ins of `sclens_amd.api` (`_wishart_matrix`, `corr_mat`, `_get_eigen`):
+scores of cells outside a decomposition (`linear` with the centring as the bias), covariates taken out of a matrix (the residual), heads
+and encoders trained on the signals (`linear`, `linear_backward`, an `orthogonalize`d update), bases of two runs or members turned onto
+each other (`orthogonalize` of `corr_mat(V1, V2)`).
+
+Element types are torch.bfloat16, torch.float16 and torch.float32; sums are held in 32 bits and rounded once. Calls are queued on the
+tensors' device on torch's current stream of that device; they neither block nor synchronise, and can be captured into a graph after one
+eager call of the same thread (which creates the thread's context). They record no autograd graph: gradients are the explicit call.
+
+torch has to be imported before the library is first used (importing this module does it): both then run on one HIP runtime and torch's
+streams are valid for the library.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import threading
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from ._lib import Context
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+#: steep quintic step: five of them bring the singular values above about 1e-2 of the norm into 0.7 .. 1.2
+UPDATE_STEP = (3.4445, -4.7750, 2.0315)
+#: p(1) = 1, p'(1) = p''(1) = 0: converges cubically to the orthogonal factor from there
+POLAR_STEP = (1.875, -1.25, 0.375)
+
+_local = threading.local()
+
+
+def _context(device: torch.device, ctx: Optional[Context]) -> Context:
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if ctx is None:
+        mine = getattr(_local, "contexts", None)
+        if mine is None:
+            mine = _local.contexts = {}
+        ctx = mine.get(index)
+        if ctx is None:
+            ctx = mine[index] = Context(index)  # one host thread per context
+    elif ctx.device != index:
+        raise ValueError(f"the tensors are on device {index}, the context on device {ctx.device}")
+    if not _lib.shares_torch_runtime:
+        raise RuntimeError("libsclens_hip.so was loaded before torch and runs on another HIP runtime: import torch (or sclens_amd.dense) "
+                           "before the first use of sclens_amd")
+    return ctx
+
+
+def _check(name: str, t, like=None, shape=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} has to be a torch tensor")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name}: element type {t.dtype} (bfloat16, float16 or float32 expected)")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} is on {t.device}, expected a GPU")
+    return t
+
+
+def _rows(name: str, t: torch.Tensor) -> Tuple[int, int]:
+    """(rows, leading dimension) of t as a matrix of rows along its last axis"""
+    cols = t.size(-1)
+    if t.dim() == 2:
+        rows, ld = t.size(0), t.stride(0)
+    elif t.dim() == 1:
+        rows, ld = 1, cols
+    else:
+        rows, ld = t.numel() // cols if cols else 0, cols
+        if not t.is_contiguous():
+            try:
+                v = t.view(-1, cols)
+            except RuntimeError:
+                raise ValueError(f"{name}: the leading axes of strides {t.stride()} do not join into one; call .contiguous()") from None
+            rows, ld = v.size(0), v.stride(0)
+    if t.numel() == 0:
+        return rows, max(1, cols)
+    if cols > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: rows have to be contiguous (strides {t.stride()}); call .contiguous()")
+    if rows <= 1:
+        ld = cols
+    if ld < cols:
+        raise ValueError(f"{name}: rows overlap (strides {t.stride()}); call .contiguous()")
+    return rows, ld
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {name!r} (one of {', '.join(ACTIVATIONS)})")
+    return ACTIVATIONS[name]
+
+
+def _p(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def _run(fn, key, ctx: Context, device: torch.device, *args):
+    """the call with its workspace: the size the last call of these sizes needed is tried first, then what the library asks for"""
+    sizes = getattr(_local, "sizes", None)
+    if sizes is None or len(sizes) > 4096:
+        sizes = _local.sizes = {}
+    size = sizes.get(key, 0)
+    n = C.c_int64(size)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    rc = fn(ctx.h, stream, *args, _p(ws), C.byref(n))
+    if rc == 8:  # SCLENS_ERR_WORKSPACE: nothing was launched
+        sizes[key] = size = n.value
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        rc = fn(ctx.h, stream, *args, _p(ws), C.byref(n))
+    if rc != 0:
+        ctx.check(rc)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+           activation: str = "none", save_preact: bool = False,
+           ctx: Optional[Context] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """activation(x @ weight.T + bias) + residual in one pass: x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N].
+
+    `save_preact` also returns the argument of the activation, which `linear_backward` reads. activation: "none", "relu", "silu",
+    "gelu" (z Phi(z)) or "gelu_tanh". One row (or a few) streams the weights once: the form for serving."""
+    act = _activation(activation)
+    _check("x", x)
+    _check("weight", weight, like=x)
+    if x.dim() < 1 or weight.dim() != 2 or weight.size(1) != x.size(-1):
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: expected [..., K] and [N, K]")
+    N, K = weight.shape
+    out_shape = tuple(x.shape[:-1]) + (N,)
+    if bias is not None:
+        _check("bias", bias, like=x, shape=(N,))
+        if N > 1 and bias.stride(0) != 1:
+            raise ValueError("bias has to be contiguous")
+    if residual is not None:
+        _check("residual", residual, like=x, shape=out_shape)
+    M, ldx = _rows("x", x)
+    if K == 0:
+        M = 1
+        for s in out_shape[:-1]:
+            M *= s
+    _, ldw = _rows("weight", weight)
+    _, ldr = _rows("residual", residual) if residual is not None else (0, N)
+    ctx = _context(x.device, ctx)
+    y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(out_shape, dtype=x.dtype, device=x.device) if save_preact else None
+    dt = DTYPES[x.dtype]
+    _run(ctx.lib.sclens_hip_linear, ("f", dt, M, N, K), ctx, x.device, dt, M, N, K, _p(x), ldx, _p(weight), ldw, _p(bias), _p(residual), ldr,
+         act, _p(y), max(1, N), _p(z), max(1, N))
+    return (y, z) if save_preact else y
+
+
+def linear_backward(grad: torch.Tensor, x: Optional[torch.Tensor], weight: Optional[torch.Tensor], preact: Optional[torch.Tensor] = None,
+                    activation: str = "none", need_x: bool = True, need_weight: bool = True, need_bias: bool = True,
+                    ctx: Optional[Context] = None):
+    """Gradients of `linear`: (dx, dweight, dbias), those not needed None. grad [..., N] is the gradient of the result (and already that
+    of the residual), preact what `linear(save_preact=True)` returned (not needed for "none"; relu'(0) = 0). x may be None if
+    need_weight is false, weight if need_x is false. All leading axes are summed over in dweight and dbias, in a fixed order."""
+    act = _activation(activation)
+    _check("grad", grad)
+    if grad.dim() < 1:
+        raise ValueError("grad: expected [..., N]")
+    N = grad.size(-1)
+    lead = tuple(grad.shape[:-1])
+    M = 1
+    for s in lead:
+        M *= s
+    if need_weight and x is None or need_x and weight is None:
+        raise ValueError("dweight needs x, dx needs weight")
+    K = x.size(-1) if x is not None else (weight.size(-1) if weight is not None else 0)
+    if x is not None:
+        _check("x", x, like=grad, shape=lead + (K,))
+    if weight is not None:
+        _check("weight", weight, like=grad, shape=(N, K))
+    if act:
+        if preact is None:
+            raise ValueError(f"the gradient of {activation!r} needs preact (linear(..., save_preact=True))")
+        _check("preact", preact, like=grad, shape=grad.shape)
+    _, lddy = _rows("grad", grad)
+    ldx = _rows("x", x)[1] if need_weight else max(1, K)
+    ldw = _rows("weight", weight)[1] if need_x else max(1, K)
+    ldz = _rows("preact", preact)[1] if act else max(1, N)
+    ctx = _context(grad.device, ctx)
+    new = lambda shape: torch.empty(shape, dtype=grad.dtype, device=grad.device)  # noqa: E731
+    dx = new(lead + (K,)) if need_x else None
+    dw = new((N, K)) if need_weight else None
+    db = new((N,)) if need_bias else None
+    dt = DTYPES[grad.dtype]
+    _run(ctx.lib.sclens_hip_linear_backward, ("b", dt, M, N, K, need_x, need_weight, need_bias), ctx, grad.device, dt, M, N, K, _p(grad), lddy,
+         _p(x) if need_weight else None, ldx, _p(weight) if need_x else None, ldw, _p(preact) if act else None, ldz, act, _p(dx),
+         max(1, K), _p(dw), max(1, K), _p(db))
+    return dx, dw, db
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Union[Sequence[float], Sequence[Sequence[float]]] = UPDATE_STEP,
+                  eps: float = 1e-7, ctx: Optional[Context] = None) -> torch.Tensor:
+    """x [..., rows, cols] with its singular values driven towards 1, by products: x0 = x / (|x|_F + eps), then per step (a, b, c)
+    x <- a x + (b A + c A A) x with A = x x' on the shorter side, so that every singular value s becomes a s + b s^3 + c s^5.
+
+    `coefficients`: one triple, used `steps` times, or a sequence of triples, one per step. [UPDATE_STEP] * 5 is an optimiser's update;
+    [UPDATE_STEP] * 5 + [POLAR_STEP] * 3 converges to the orthogonal factor (singular values well above 1e-2 of the norm). Every matrix
+    of the leading axes is worked on by itself."""
+    _check("x", x)
+    if x.dim() < 2:
+        raise ValueError(f"x {tuple(x.shape)}: expected [..., rows, cols]")
+    coef = [float(v) for v in coefficients] if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else None
+    if coef is not None:
+        if int(steps) < 1:
+            raise ValueError("at least one step")
+        coef = coef * int(steps)
+    else:
+        if len(coefficients) < 1 or any(len(t) != 3 for t in coefficients):
+            raise ValueError("coefficients: one (a, b, c) or a sequence of them, one per step")
+        coef = [float(v) for t in coefficients for v in t]
+    rows, cols = x.shape[-2:]
+    batch = 1
+    for s in x.shape[:-2]:
+        batch *= s
+    v = x
+    if x.dim() > 3:
+        try:
+            v = x.view(batch, rows, cols)
+        except RuntimeError:
+            raise ValueError(f"x: the leading axes of strides {x.stride()} do not join into one; call .contiguous()") from None
+    stride = v.stride(0) if v.dim() == 3 and batch > 1 else rows * cols
+    ld = v.stride(-2) if rows > 1 else cols
+    if x.numel() and (cols > 1 and v.stride(-1) != 1 or ld < cols):
+        raise ValueError(f"x: rows have to be contiguous and apart (strides {x.stride()}); call .contiguous()")
+    ctx = _context(x.device, ctx)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dt = DTYPES[x.dtype]
+    arr = (C.c_double * len(coef))(*coef)
+    _run(ctx.lib.sclens_hip_orthogonalize, ("o", dt, batch, rows, cols, len(coef) > 3), ctx, x.device, dt, batch, rows, cols, _p(x), stride,
+         max(1, ld), _p(y), rows * cols, max(1, cols), len(coef) // 3, arr, float(eps))
+    return y
