@@ -37,6 +37,15 @@ struct Product {
 int64_t product_slab_bytes(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric);
 int product(Ctx* ctx, hipStream_t st, const Product& p);
 
+// the join of slabs [slices][M][round_up8(N)] written by somebody else, through p's epilogue (p.slabs set; operands only for fp32 NaN)
+int product_join(Ctx* ctx, hipStream_t st, const Product& p, int slices);
+
+// dense_stream.hip: products with one short side (linear_forward has the rule)
+constexpr int64_t STREAM_SHORT = 128;
+int stream_slices(int64_t R, int64_t K, int* kchunk);
+int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t ldb, int64_t R, const Mat& small, int64_t S, int64_t K,
+                   float* slabs, int64_t slab, int64_t sr, int64_t ss);
+
 // 16-bit image (D_F32: three bf16 planes) of src (element (r, k) at r * ld + k, transposed: k * ld + r), rows x K, K padded with zeros
 // to image_ld(K)
 static inline int64_t image_ld(int64_t K) { return round_up(K > 0 ? K : 1, 64); }
@@ -68,6 +77,10 @@ struct OrthArgs {
   const double* coef = nullptr;  // steps x (a, b, c), host
   double eps = 0;
 };
+bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: a short side of at most 64
+int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
+int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a);  // M <= 16
+
 // *need: bytes of scratch the call wants; launched only if ws_bytes >= *need (SCLENS_ERR_WORKSPACE otherwise)
 int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
 int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need);

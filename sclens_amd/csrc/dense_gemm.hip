@@ -491,6 +491,18 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   return ctx->fail(SCLENS_ERR_ARG, "product: element types");
 }
 
+int product_join(Ctx* ctx, hipStream_t st, const Product& p, int slices) {
+  ProdArgs g{};
+  g.p = p;
+  g.ksplit = slices;
+  const dim3 grid((unsigned)(((p.M + 31) / 32) * ((p.N + 63) / 64)), (unsigned)p.batch), blk(256);
+  if (p.out_type == D_F32) hipLaunchKernelGGL((k_product_join<D_F32, D_F32, false>), grid, blk, 0, st, g);
+  else if (p.out_type == D_BF16) hipLaunchKernelGGL((k_product_join<D_BF16, D_BF16, false>), grid, blk, 0, st, g);
+  else hipLaunchKernelGGL((k_product_join<D_F16, D_F16, false>), grid, blk, 0, st, g);
+  SCL_HIP(ctx, hipGetLastError());
+  return SCLENS_OK;
+}
+
 // ------------------------------------------------------------------ images
 // 64 rows x 64 columns of the image per workgroup. Straight: 8 columns per lane. Transposed: through LDS, reads along the source's rows.
 template <int T, bool TRANS>

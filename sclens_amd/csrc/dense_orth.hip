@@ -1,0 +1,375 @@
+// Orthogonalisation with a short side m of at most 64. All steps of x <- (a + b A + c A A) x, A = x x', act on x from the short side, so
+//   x_T = Q x_0,   P = a I + b A + c A A,   Q <- P Q,   A <- P A P
+// needs the m x n matrix twice (for A_0 = x_0 x_0' and for the last product) whatever the number of steps; |g|_F^2 is the trace of g g'.
+// In exact arithmetic that is the definition. In floating point an error of A_0 grows with the square of a small singular value's growth
+// (five steps of a = 3.4445: a^8 = 2e4 relative to the largest), which fp32 cannot pay and fp64 can: the m x m side and both products run
+// on v_mfma_f64_16x16x4 (below 64 rows they cost less than reading x does; the entries of x convert exactly).
+// A, P, Q commute and are symmetric: tiles on and below the diagonal are computed and mirrored.
+//   n up to 1024, or many matrices: everything in one workgroup per matrix, one launch (k_orth_small).
+//   longer: partial sums of g g' over slices (k_orth_gram, k_orth_gram_sum), the steps in one workgroup (k_orth_steps), the product.
+#include <algorithm>
+
+#include "dense_dev.h"
+
+namespace scl {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+struct SmallArgs {
+  OrthArgs o;  // coef: device pointer is not needed, the steps' coefficients ride in `coef`
+  int tall, m, slices;
+  int64_t n;
+  double* part;  // [batch][slices][tiles * 256]
+  double* gram;  // [batch][tiles * 256]
+  double* Q;     // [batch][16 MT][16 MT]
+};
+constexpr int MAX_RIDE = 24;  // steps whose coefficients fit the kernel's arguments
+struct Coefs { double v[3 * MAX_RIDE]; };
+
+template <int MT> struct Tiles {
+  static constexpr int R = 16 * MT, LQ = R + 2, LI = R + 1, NL = MT * (MT + 1) / 2;
+};
+// the t-th tile on or below the diagonal, by rows
+__device__ __forceinline__ void lower_tile(int t, int* i, int* j) {
+  int r = 0;
+  while ((r + 1) * (r + 2) / 2 <= t) ++r;
+  *i = r;
+  *j = t - r * (r + 1) / 2;
+}
+
+// 16 NW columns k0 .. of x (R rows, zeros outside) into registers, then into Xs[k][i]
+template <int T, int MT, int NW>
+struct Slab {
+  float v[4 * MT];
+  __device__ __forceinline__ void fetch(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend) {
+    constexpr int R = 16 * MT, CK = 16 * NW;
+    const auto* p = static_cast<const typename Elem<T>::type*>(a.o.x) + b * a.o.sx;
+#pragma unroll
+    for (int e = 0; e < 4 * MT; ++e) {
+      const int id = e * (64 * NW) + (int)threadIdx.x;
+      const int i = a.tall ? id % R : id / CK, k = a.tall ? id / R : id % CK;
+      const bool in = i < a.m && k0 + k < kend;
+      v[e] = in ? Elem<T>::ld(p + (a.tall ? (k0 + k) * a.o.ldx + i : i * a.o.ldx + k0 + k)) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void put(float* Xs, int tall) {
+    constexpr int R = 16 * MT, CK = 16 * NW, LI = R + 1;
+#pragma unroll
+    for (int e = 0; e < 4 * MT; ++e) {
+      const int id = e * (64 * NW) + (int)threadIdx.x;
+      const int i = tall ? id % R : id / CK, k = tall ? id / R : id % CK;
+      Xs[k * LI + i] = v[e];
+    }
+  }
+};
+
+// red[tile][g * 64 + lane] = sum over k0 <= k < kend of x x' (unscaled); every wave takes 16 of the columns in Xs
+template <int T, int MT, int NW>
+__device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, double* red) {
+  constexpr int LI = Tiles<MT>::LI, NL = Tiles<MT>::NL, CK = 16 * NW;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+  f64x4 acc[NL];
+#pragma unroll
+  for (int t = 0; t < NL; ++t) acc[t] = f64x4{0, 0, 0, 0};
+  Slab<T, MT, NW> s;
+  s.fetch(a, b, k0, kend);
+  for (int64_t k = k0; k < kend; k += CK) {
+    s.put(Xs, a.tall);
+    __syncthreads();
+    if (k + CK < kend) s.fetch(a, b, k + CK, kend);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      double f[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) f[i] = (double)Xs[(wid * 16 + ks * 4 + q) * LI + i * 16 + r16];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(f[i], f[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+    }
+    __syncthreads();
+  }
+  for (int w = 0; w < NW; ++w) {  // the waves' sums one after the other: a fixed order
+    if (wid == w) {
+#pragma unroll
+      for (int t = 0; t < NL; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          double* r = red + t * 256 + g * 64 + lane;
+          *r = w == 0 ? acc[t][g] : *r + acc[t][g];
+        }
+    }
+    __syncthreads();
+  }
+}
+
+// C tile (i, j) = X Y for symmetric X, Y in LDS
+template <int MT>
+__device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, int i, int j, int ksteps) {
+  constexpr int LQ = Tiles<MT>::LQ;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+  f64x4 acc = {0, 0, 0, 0};
+  const double *x = X + (i * 16 + r16) * LQ + q, *y = Y + (j * 16 + r16) * LQ + q;
+  for (int s = 0; s < ksteps; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s], y[4 * s], acc, 0, 0, 0);
+  return acc;
+}
+template <int MT>
+__device__ __forceinline__ void tile_store(double* C, int i, int j, f64x4 v) {
+  constexpr int LQ = Tiles<MT>::LQ;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int r = i * 16 + q + 4 * g, c = j * 16 + r16;
+    C[r * LQ + c] = v[g];
+    if (i != j) C[c * LQ + r] = v[g];
+  }
+}
+
+// from the sums in `red` to Q (with the 1 / (|g|_F + eps) of x_0 in it); 8 waves
+template <int MT>
+__device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const double* red, double* A, double* P, double* Q, double* scal) {
+  constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, NL = Tiles<MT>::NL, NT = (NL + 7) / 8;
+  const int tid = threadIdx.x, wid = tid >> 6, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
+  const int ksteps = (a.m + 3) / 4;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const int t = wid + 8 * u;
+    if (t < NL) {
+      int i, j;
+      lower_tile(t, &i, &j);
+      f64x4 v;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) v[g] = red[t * 256 + g * 64 + lane];
+      tile_store<MT>(A, i, j, v);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double s = 0.0;
+    for (int i = 0; i < a.m; ++i) s += A[i * LQ + i];
+    scal[0] = 1.0 / (sqrt(s) + a.o.eps);
+  }
+  __syncthreads();
+  const double f = scal[0];
+  for (int e = tid; e < R * R; e += 512) {
+    const int r = e / R, c = e % R;
+    A[r * LQ + c] *= f * f;
+    Q[r * LQ + c] = r == c && r < a.m ? f : 0.0;
+  }
+  __syncthreads();
+  for (int t = 0; t < a.o.steps; ++t) {
+    const double ca = cf.v[3 * t], cb = cf.v[3 * t + 1], cc = cf.v[3 * t + 2];
+    const bool last = t + 1 == a.o.steps;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < NL) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        f64x4 v = tile_product<MT>(A, A, i, j, ksteps);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int r = i * 16 + q + 4 * g, c = j * 16 + r16;
+          v[g] = cc * v[g] + cb * A[r * LQ + c] + (r == c && r < a.m ? ca : 0.0);
+        }
+        tile_store<MT>(P, i, j, v);
+      }
+    }
+    __syncthreads();
+    f64x4 vq[NT], va[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < NL) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        vq[u] = tile_product<MT>(P, Q, i, j, ksteps);
+        if (!last) va[u] = tile_product<MT>(A, P, i, j, ksteps);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < NL) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        tile_store<MT>(Q, i, j, vq[u]);
+        if (!last) tile_store<MT>(A, i, j, va[u]);
+      }
+    }
+    __syncthreads();
+    if (last) break;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < NL) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        va[u] = tile_product<MT>(A, P, i, j, ksteps);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < NL) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        tile_store<MT>(A, i, j, va[u]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// y = Q x for k0 <= k < kend, 16 NW columns at a time; Q [R][ldq] in LDS
+template <int T, int MT, int NW>
+__device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, const double* Q) {
+  constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, CK = 16 * NW;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+  const int ksteps = (a.m + 3) / 4;
+  auto* y = static_cast<typename Elem<T>::type*>(a.o.y) + b * a.o.sy;
+  Slab<T, MT, NW> s;
+  s.fetch(a, b, k0, kend);
+  for (int64_t k = k0; k < kend; k += CK) {
+    s.put(Xs, a.tall);
+    __syncthreads();
+    if (k + CK < kend) s.fetch(a, b, k + CK, kend);
+    f64x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f64x4{0, 0, 0, 0};
+    float* mine = Xs + (wid * 16 + r16) * LI;
+    for (int st = 0; st < ksteps; ++st) {
+      const double x = (double)mine[st * 4 + q];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64(Q[(i * 16 + r16) * LQ + st * 4 + q], x, acc[i], 0, 0, 0);
+    }
+    __syncthreads();  // (all columns of Xs are read by their own wave; the barrier orders its lanes)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) mine[i * 16 + q + 4 * g] = (float)acc[i][g];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4 * MT; ++e) {
+      const int id = e * (64 * NW) + (int)threadIdx.x;
+      const int i = a.tall ? id % R : id / CK, kk = a.tall ? id / R : id % CK;
+      if (i < a.m && k + kk < kend) Elem<T>::st(y + (a.tall ? (k + kk) * a.o.ldy + i : i * a.o.ldy + k + kk), Xs[kk * LI + i]);
+    }
+    __syncthreads();
+  }
+}
+
+template <int T, int MT>
+__global__ __launch_bounds__(512) void k_orth_small(SmallArgs a, Coefs cf) {
+  constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  double* A = reinterpret_cast<double*>(lds);
+  double *P = A + R * LQ, *Q = P + R * LQ, *scal = Q + R * LQ;
+  float* Xs = reinterpret_cast<float*>(scal + 2);
+  const int64_t b = blockIdx.x;
+  gram_range<T, MT, 8>(a, b, 0, a.n, Xs, P);
+  steps<MT>(a, cf, P, A, P, Q, scal);
+  apply_range<T, MT, 8>(a, b, 0, a.n, Xs, Q);
+}
+template <int T, int MT>
+__global__ __launch_bounds__(256) void k_orth_gram(SmallArgs a) {
+  constexpr int NL = Tiles<MT>::NL, LI = Tiles<MT>::LI;
+  __shared__ float Xs[64 * LI];
+  __shared__ double red[NL * 256];
+  const int64_t b = blockIdx.y, chunks = (a.n + 63) / 64, per = (chunks + a.slices - 1) / a.slices;
+  const int64_t k0 = (int64_t)blockIdx.x * per * 64, kend = min(a.n, k0 + per * 64);
+  gram_range<T, MT, 4>(a, b, k0, max(k0, kend), Xs, red);
+  double* out = a.part + (b * a.slices + blockIdx.x) * (NL * 256);
+  for (int e = threadIdx.x; e < NL * 256; e += 256) out[e] = red[e];
+}
+__global__ __launch_bounds__(256) void k_orth_gram_sum(const double* __restrict__ part, int slices, int elems, double* __restrict__ out) {
+  __shared__ double S[4][64];
+  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t b = blockIdx.y;
+  const int e = blockIdx.x * 64 + c;
+  double s = 0.0;
+  for (int i = g; i < slices; i += 4) s += part[(b * slices + i) * elems + e];
+  S[g][c] = s;
+  __syncthreads();
+  if (g == 0) out[b * elems + e] = (S[0][c] + S[1][c]) + (S[2][c] + S[3][c]);
+}
+template <int MT>
+__global__ __launch_bounds__(512) void k_orth_steps(SmallArgs a, Coefs cf) {
+  constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R, NL = Tiles<MT>::NL;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  double* A = reinterpret_cast<double*>(lds);
+  double *P = A + R * LQ, *Q = P + R * LQ, *scal = Q + R * LQ;
+  const int64_t b = blockIdx.x;
+  steps<MT>(a, cf, a.gram + b * NL * 256, A, P, Q, scal);
+  for (int e = threadIdx.x; e < R * R; e += 512) a.Q[b * R * R + e] = Q[(e / R) * LQ + e % R];
+}
+template <int T, int MT>
+__global__ __launch_bounds__(256) void k_orth_apply(SmallArgs a) {
+  constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R, LI = Tiles<MT>::LI;
+  __shared__ double Q[R * LQ];
+  __shared__ float Xs[64 * LI];
+  const int64_t b = blockIdx.y, chunks = (a.n + 63) / 64, per = (chunks + gridDim.x - 1) / gridDim.x;
+  for (int e = threadIdx.x; e < R * R; e += 256) Q[(e / R) * LQ + e % R] = a.Q[b * R * R + e];
+  const int64_t k0 = (int64_t)blockIdx.x * per * 64, kend = min(a.n, k0 + per * 64);
+  apply_range<T, MT, 4>(a, b, k0, kend, Xs, Q);  // (its first barrier orders Q too)
+}
+
+namespace {
+template <int T, int MT>
+int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
+  constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, NL = Tiles<MT>::NL;
+  constexpr int LDS_STEPS = (3 * R * LQ + 2) * 8, LDS_ALL = LDS_STEPS + 128 * LI * 4;
+  const unsigned batch = (unsigned)a.o.batch;
+  if (a.slices == 1) {
+    if (LDS_ALL > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_small<T, MT>), LDS_ALL));
+    hipLaunchKernelGGL((k_orth_small<T, MT>), dim3(batch), dim3(512), LDS_ALL, st, a, cf);
+  } else {
+    if (LDS_STEPS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_steps<MT>), LDS_STEPS));
+    hipLaunchKernelGGL((k_orth_gram<T, MT>), dim3((unsigned)a.slices, batch), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_orth_gram_sum, dim3(NL * 4, batch), dim3(256), 0, st, a.part, a.slices, NL * 256, a.gram);
+    hipLaunchKernelGGL((k_orth_steps<MT>), dim3(batch), dim3(512), LDS_STEPS, st, a, cf);
+    const int64_t chunks = (a.n + 63) / 64, per = std::max<int64_t>(1, chunks * batch / 2048);
+    hipLaunchKernelGGL((k_orth_apply<T, MT>), dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
+  }
+  SCL_HIP(ctx, hipGetLastError());
+  return SCLENS_OK;
+}
+template <int T>
+int run_small_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
+  if (a.m <= 16) return run_small<T, 1>(ctx, st, a, cf);
+  if (a.m <= 32) return run_small<T, 2>(ctx, st, a, cf);
+  if (a.m <= 48) return run_small<T, 3>(ctx, st, a, cf);
+  return run_small<T, 4>(ctx, st, a, cf);
+}
+}  // namespace
+
+bool orth_is_small(const OrthArgs& o) { return std::min(o.rows, o.cols) <= 64 && o.steps <= MAX_RIDE; }
+
+int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws_bytes, int64_t* need) {
+  SmallArgs a{};
+  a.o = o;
+  a.tall = o.rows > o.cols;
+  a.m = (int)std::min(o.rows, o.cols);
+  a.n = std::max(o.rows, o.cols);
+  const int MT = (a.m + 15) / 16, elems = MT * (MT + 1) / 2 * 256;
+  if (a.n <= 1024 || o.batch >= 128) a.slices = 1;
+  else a.slices = (int)std::max<int64_t>(2, std::min<int64_t>((a.n + 255) / 256, 512 / o.batch));
+  Carve c(ws);
+  if (a.slices > 1) {
+    a.part = c.take<double>(o.batch * a.slices * elems);
+    a.gram = c.take<double>(o.batch * elems);
+    a.Q = c.take<double>(o.batch * 256 * MT * MT);
+  }
+  *need = c.used;
+  if (c.used > ws_bytes) return ctx->fail(SCLENS_ERR_WORKSPACE, "this call needs " + std::to_string(c.used) + " bytes of device workspace");
+  Coefs cf{};
+  for (int i = 0; i < 3 * o.steps; ++i) cf.v[i] = o.coef[i];
+  a.o.coef = nullptr;
+  if (o.dtype == D_F32) return run_small_t<D_F32>(ctx, st, a, cf);
+  if (o.dtype == D_BF16) return run_small_t<D_BF16>(ctx, st, a, cf);
+  return run_small_t<D_F16>(ctx, st, a, cf);
+}
+
+}  // namespace scl

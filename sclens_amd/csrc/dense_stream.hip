@@ -1,0 +1,268 @@
+// Products with one short side: a matrix of many rows is streamed once against at most 16 (k_rows) or 128 (k_stream) rows. Both are
+// bound by reading the long operand; the matrix cores (16 x 16 x 32 tiles, long operand as the rows of the tile) have room to spare:
+// at 128 short rows the fp32 form (six products per term) still keeps up with 6 TB/s.
+#include <algorithm>
+
+#include "dense_dev.h"
+
+namespace scl {
+
+typedef __attribute__((address_space(1))) const void glb_cv;
+typedef __attribute__((address_space(3))) void lds_v;
+__device__ __attribute__((aligned(16))) unsigned short g_zero_chunk_s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+
+// eight elements k .. k+7 of a row that ends at K, at any element address
+template <int T> struct Chunk;
+template <> struct Chunk<D_F32> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* row, int64_t k, int64_t K) {
+    if (k + 8 <= K) {
+      const f32x8_any a = *reinterpret_cast<const f32x8_any*>(row + k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = a.v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k + e < K ? row[k + e] : 0.f;
+    }
+  }
+};
+template <int T> struct Chunk16 {
+  u16x8 v;
+  __device__ __forceinline__ void load(const unsigned short* row, int64_t k, int64_t K) {
+    if (k + 8 <= K) {
+      const u16x8_any a = *reinterpret_cast<const u16x8_any*>(row + k);
+      v = __builtin_bit_cast(u16x8, a);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k + e < K ? row[k + e] : 0;
+    }
+  }
+};
+template <> struct Chunk<D_BF16> : Chunk16<D_BF16> {};
+template <> struct Chunk<D_F16> : Chunk16<D_F16> {};
+
+template <int T>
+__device__ __forceinline__ f32x4 mfma16(u16x8 a, u16x8 b, f32x4 c) {
+  if constexpr (T == D_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// ---- at most 16 rows of x: 16 rows of w per workgroup, the contraction dealt out to its 8 waves in runs of 128 columns
+template <int T>
+__global__ __launch_bounds__(512) void k_rows(LinearArgs a) {
+  typedef typename Elem<T>::type E;
+  __shared__ float S[8][256];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const E* wr = static_cast<const E*>(a.w) + min(n0 + r16, a.N - 1) * a.ldw;  // (rows behind the end: not stored)
+  const E* xr = static_cast<const E*>(a.x) + min((int64_t)r16, a.M - 1) * a.ldx;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t k0 = wid * 128; k0 < a.K; k0 += 8 * 128) {
+    Chunk<T> w[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i].load(wr, k0 + 32 * i + 8 * q, a.K);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i].load(xr, k0 + 32 * i + 8 * q, a.K);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (T == D_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i].v[e], x[i].v[e], acc, 0, 0, 0);
+      } else
+        acc = mfma16<T>(w[i].v, x[i].v, acc);
+    }
+  }
+  *reinterpret_cast<f32x4*>(&S[wid][lane * 4]) = acc;
+  __syncthreads();
+  if (tid >= 256) return;
+  const int nn = tid & 15;
+  const int64_t m = tid >> 4, n = n0 + nn;
+  if (m >= a.M || n >= a.N) return;
+  const int at = ((nn >> 2) * 16 + (int)m) * 4 + (nn & 3);
+  float z = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) z += S[w][at];
+  if (a.bias) z += Elem<T>::ld(static_cast<const E*>(a.bias) + n);
+  if (a.pre) Elem<T>::st(static_cast<E*>(a.pre) + m * a.ldz + n, z);
+  z = act_apply(z, a.act);
+  if (a.res) z += Elem<T>::ld(static_cast<const E*>(a.res) + m * a.ldr + n);
+  Elem<T>::st(static_cast<E*>(a.y) + m * a.ldy + n, z);
+}
+
+int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
+  const dim3 grid((unsigned)((a.N + 15) / 16)), blk(512);
+  if (a.dtype == D_F32) hipLaunchKernelGGL(k_rows<D_F32>, grid, blk, 0, st, a);
+  else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_rows<D_BF16>, grid, blk, 0, st, a);
+  else hipLaunchKernelGGL(k_rows<D_F16>, grid, blk, 0, st, a);
+  SCL_HIP(ctx, hipGetLastError());
+  return SCLENS_OK;
+}
+
+// ---- at most 128 short rows (an image, three planes for fp32): 256 long rows per workgroup, 32 per wave, the contraction cut into
+// grid.y slices of whole 64-column stages. The short operand's stage sits in LDS (two stages in turn, chunk q of row r in slot
+// q ^ ((r >> 1) & 7)), the long one goes from memory to registers a stage ahead, fp32 is taken apart there.
+struct StreamArgs {
+  const void* big;
+  int64_t ldb, R, K;
+  Mat small;
+  int64_t S;
+  float* slabs;       // [slice][M][round_up8(N)]
+  int64_t slab;       // elements of a slice
+  int64_t sr, ss;     // strides of the long and the short index in a slab
+  int kchunk;         // stages per slice
+};
+template <int T, int NT>
+__global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
+  constexpr int NP = T == D_F32 ? 3 : 1, ROWS = NT * 16;
+  constexpr int PLANE = ROWS * 128, STAGE = NP * PLANE, PIECES = STAGE / 1024;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  typedef typename Elem<T>::type E;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
+  const int64_t row0 = (int64_t)blockIdx.x * 256 + wid * 32;
+  const E* rows[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) rows[i] = static_cast<const E*>(a.big) + min(row0 + i * 16 + r16, a.R - 1) * a.ldb;
+  const int nst = (int)((a.K + 63) / 64);
+  const int t0 = (int)blockIdx.y * a.kchunk, t1 = min(nst, t0 + a.kchunk);
+  auto copy = [&](int buf, int t) {
+    for (int p = wid; p < PIECES; p += 8) {  // 1 KB: 8 rows x 64 columns of a plane
+      const int plane = p / (ROWS / 8), r = (p % (ROWS / 8)) * 8 + (lane >> 3);
+      const int c = (lane & 7) ^ ((r >> 1) & 7);
+      const unsigned short* s = static_cast<const unsigned short*>(a.small.p) + plane * a.small.plane +
+                                min((int64_t)r, a.S - 1) * a.small.ld + (int64_t)t * 64 + 8 * c;
+      if ((int64_t)t * 64 + 8 * c >= a.K) s = g_zero_chunk_s;
+      __builtin_amdgcn_global_load_lds((glb_cv*)s, (lds_v*)(lds + buf * STAGE + p * 1024), 16, 0, 0);
+    }
+  };
+  Chunk<T> nx[2][2], cu[2][2];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) nx[i][kk].load(rows[i], (int64_t)t * 64 + kk * 32 + q * 8, a.K);
+  };
+  f32x4 acc[2][NT];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t0 < t1) {
+    copy(0, t0);
+    fetch(t0);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int cur = (t - t0) & 1;
+    __syncthreads();  // this stage has landed; everyone is done with the other buffer
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) cu[i][kk] = nx[i][kk];
+    if (t + 1 < t1) {
+      copy(cur ^ 1, t + 1);
+      fetch(t + 1);
+    }
+    const unsigned char* B = lds + cur * STAGE;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      u16x8 A[2][NP];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (T == D_F32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            unsigned short x, y, z;
+            split3(cu[i][kk].v[e], x, y, z);
+            A[i][0][e] = x; A[i][1][e] = y; A[i][2][e] = z;
+          }
+        } else
+          A[i][0] = cu[i][kk].v;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = j * 16 + r16, c = 4 * kk + q;
+        u16x8 b[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) b[p] = *reinterpret_cast<const u16x8*>(B + p * PLANE + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (T == D_F32) {
+            acc[i][j] = mfma16<D_BF16>(A[i][2], b[0], acc[i][j]);
+            acc[i][j] = mfma16<D_BF16>(A[i][0], b[2], acc[i][j]);
+            acc[i][j] = mfma16<D_BF16>(A[i][1], b[1], acc[i][j]);
+            acc[i][j] = mfma16<D_BF16>(A[i][1], b[0], acc[i][j]);
+            acc[i][j] = mfma16<D_BF16>(A[i][0], b[1], acc[i][j]);
+            acc[i][j] = mfma16<D_BF16>(A[i][0], b[0], acc[i][j]);
+          } else
+            acc[i][j] = mfma16<T>(A[i][0], b[0], acc[i][j]);
+        }
+      }
+    }
+  }
+  float* out = a.slabs + (int64_t)blockIdx.y * a.slab;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t s = j * 16 + r16;
+      if (s >= a.S) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t r = row0 + i * 16 + 4 * q + e;
+        if (r >= a.R) continue;
+        float v = acc[i][j][e];
+        if constexpr (T == D_F32) {
+          if (v != v) {  // an infinity that met a zero piece: this slice's terms again in fp32
+            const E* x = static_cast<const E*>(a.big) + r * a.ldb;
+            const unsigned short* y = static_cast<const unsigned short*>(a.small.p) + s * a.small.ld;
+            v = 0.f;
+            const int64_t k1 = min(a.K, (int64_t)t1 * 64);
+            for (int64_t k = (int64_t)t0 * 64; k < k1; ++k)
+              v = fmaf(x[k], (bf16_to_f32(y[k]) + bf16_to_f32(y[k + a.small.plane])) + bf16_to_f32(y[k + 2 * a.small.plane]), v);
+          }
+        }
+        out[r * a.sr + s * a.ss] = v;
+      }
+    }
+}
+
+namespace {
+template <int T, int NT>
+int launch_stream(Ctx* ctx, hipStream_t st, const StreamArgs& a, int slices) {
+  constexpr int LDS = 2 * (T == D_F32 ? 3 : 1) * NT * 16 * 128;
+  if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_stream<T, NT>), LDS));
+  hipLaunchKernelGGL((k_stream<T, NT>), dim3((unsigned)((a.R + 255) / 256), (unsigned)slices), dim3(512), LDS, st, a);
+  SCL_HIP(ctx, hipGetLastError());
+  return SCLENS_OK;
+}
+template <int T>
+int launch_stream_t(Ctx* ctx, hipStream_t st, const StreamArgs& a, int slices) {
+  if (a.S <= 16) return launch_stream<T, 1>(ctx, st, a, slices);
+  if (a.S <= 32) return launch_stream<T, 2>(ctx, st, a, slices);
+  if (a.S <= 48) return launch_stream<T, 3>(ctx, st, a, slices);
+  if (a.S <= 64) return launch_stream<T, 4>(ctx, st, a, slices);
+  return launch_stream<T, 8>(ctx, st, a, slices);
+}
+}  // namespace
+
+int stream_slices(int64_t R, int64_t K, int* kchunk) {
+  const int64_t nst = (K + 63) / 64, groups = (R + 255) / 256;
+  // about four workgroups of 8 waves per CU, at least four stages each
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(nst / 4, (1024 + groups - 1) / groups));
+  const int64_t kc = (nst + want - 1) / want;
+  *kchunk = (int)kc;
+  return (int)((nst + kc - 1) / kc);
+}
+
+int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t ldb, int64_t R, const Mat& small, int64_t S, int64_t K,
+                   float* slabs, int64_t slab, int64_t sr, int64_t ss) {
+  StreamArgs a{};
+  a.big = big; a.ldb = ldb; a.R = R; a.K = K;
+  a.small = small; a.S = S;
+  a.slabs = slabs; a.slab = slab; a.sr = sr; a.ss = ss;
+  const int slices = stream_slices(R, K, &a.kchunk);
+  if (dtype == D_F32) return launch_stream_t<D_F32>(ctx, st, a, slices);
+  if (dtype == D_BF16) return launch_stream_t<D_BF16>(ctx, st, a, slices);
+  return launch_stream_t<D_F16>(ctx, st, a, slices);
+}
+
+}  // namespace scl
