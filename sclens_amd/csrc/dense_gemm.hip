@@ -3,13 +3,14 @@
 //   * fp32 operands come as three bf16 planes (24 bits, exact): six products per term, smallest first -- p2 p0, p0 p2, p1 p1, p1 p0,
 //     p0 p1, p0 p0; what is left out (2 p1 p2) is at most 2^-23 of the term and 2^-26 in the mean square, the size of fp32's own rounding.
 //   * a workgroup owns one BM x BN tile; both operands go to LDS 64 columns at a time straight from memory (16 bytes per lane), two
-//     stages in turn. Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): the 32 rows a matrix instruction reads at one
-//     column fall into 16 bank groups, two lanes each, which is the rate of a 16-byte read.
-//   * the stage loop is a software pipeline of four units (16 columns each): the reads of the next unit are in flight while the
-//     matrix instructions of this one run, the copies of the next stage are spread over them, one barrier per stage.
+//     stages in turn. Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): 16 rows at one chunk fall into 16 different
+//     16-byte bank groups, so a 16-byte read runs without conflicts.
+//   * the stage loop is a software pipeline of units of 16 columns: the reads of the next unit, and in the stage's last unit the copies
+//     of the stage after the next, are issued one at a time in the shadow of the matrix instructions.
 //   * the epilogue turns the accumulators through LDS so that bias, residual, pre-activation and result move 16 bytes per lane along
 //     the rows; it can also store the transpose and the mirrored half of a symmetric result.
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_dev.h"
 
@@ -18,8 +19,13 @@ namespace scl {
 typedef __attribute__((address_space(1))) const void glb_cv;
 typedef __attribute__((address_space(3))) void lds_v;
 
-// what a lane whose columns lie behind the end of the contraction copies instead
-__device__ __attribute__((aligned(16))) unsigned short g_zero_chunk[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+// the wave's own copies but the N youngest have landed and its LDS reads are done; then everybody's
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 struct ProdArgs {
   Product p;
@@ -36,21 +42,26 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
   return x * q + (x < r ? x : r) + (id >> 3);
 }
 
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    static_for<N, I + 1>(f);
+  }
+}
+
 template <int OT, int RT, bool PART>
 struct Epilogue {
   // 8 columns from col of row `row`, n of them inside (images with `pad`: all 8, those outside as zeros)
   static __device__ __forceinline__ void apply(const Product& p, int64_t b, int64_t row, int64_t col, int nin, bool row_in, float v[8],
-                                               const float* bias8) {
+                                               const float* bias8, const Raw8<RT>& res) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] * p.alpha + bias8[e];
     if (p.pre.p && row_in) store8<OT>(p.pre, b * p.pre.batch + row * p.pre.ld + col, nin, v);
-    if (p.act != ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = act_apply(v[e], p.act);
-    }
+    if (p.act != ACT_NONE) act8<false>(v, p.act);
     if (p.res.p && row_in && nin > 0) {
       float r[8];
-      load8<RT>(p.res, b * p.res.batch + row * p.res.ld + col, nin, r);
+      res.get(r);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += p.beta * r[e];
     }
@@ -73,14 +84,14 @@ __device__ __forceinline__ float recompute_f32(const unsigned short* A, const un
 }
 
 template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
+__global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(ProdArgs g) {
   constexpr int NW = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, NP = PA + PB;  // 1 KB copies (8 rows x 64 columns) per wave and stage
   constexpr int OPA = BM * 128, STAGE = (BM + BN) * 128;
   constexpr bool PL = (MT == D_PL3);
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const Product& p = g.p;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid / WN, wn = wid % WN, l31 = lane & 31, h = lane >> 5;
 
   // ---- the tile
@@ -101,21 +112,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
   }
   const int64_t m0 = (int64_t)ti * BM, n0 = (int64_t)tj * BN, batch = blockIdx.y;
 
-  // ---- sources of this wave's copies
+  // ---- sources of this wave's copies: a uniform base that moves along the contraction, and each lane's place below it (the plan
+  // keeps a tile's rows below 2^32 bytes)
   const int srow = lane >> 3, sq = lane & 7;
-  const unsigned short* src[NP];
-  int chunk8[NP];
+  const char* baseA = static_cast<const char*>(p.A.p) + 2 * (batch * p.A.batch + m0 * p.A.ld);
+  const char* baseB = static_cast<const char*>(p.B.p) + 2 * (batch * p.B.batch + n0 * p.B.ld);
+  unsigned voff[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const bool isA = i < PA;
     const int r = (isA ? wid * PA + i : wid * PB + i - PA) * 8 + srow;
     const int chunk = sq ^ ((r >> 1) & 7);
-    const Mat& m = isA ? p.A : p.B;
-    int64_t row = (isA ? m0 : n0) + r;
-    const int64_t last = (isA ? p.M : p.N) - 1;
-    if (row > last) row = last;  // (its products are not stored)
-    src[i] = static_cast<const unsigned short*>(m.p) + batch * m.batch + row * m.ld + 8 * chunk;
-    chunk8[i] = 8 * chunk;
+    const int64_t last = (isA ? p.M - m0 : p.N - n0) - 1;
+    const int64_t row = r < last ? r : last;  // (products of rows behind the end are not stored)
+    voff[i] = (unsigned)(2 * (row * (isA ? p.A.ld : p.B.ld) + 8 * chunk));
   }
 
   // ---- stages of this slice: stage t = (plane pair t / nkt, columns 64 (t % nkt) ..)
@@ -124,15 +134,26 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
   int ld_t = t0;                             // the stage the copies load
   int ld_seg = PL ? t0 / max(1, g.nkt) : 0;  // its plane pair and column block
   int ld_k = t0 - ld_seg * g.nkt;
-  int64_t offA = 0, offB = 0;
-  auto set_off = [&]() {
-    offA = offB = (int64_t)ld_k * 64;
+  const char *curA = baseA, *curB = baseB;
+  auto set_cur = [&]() {
+    curA = baseA + (int64_t)ld_k * 128;
+    curB = baseB + (int64_t)ld_k * 128;
     if (PL) {
       // (A plane, B plane), smallest products first: 20 02 11 10 01 00
       const int pa = (0x001102 >> (4 * ld_seg)) & 15, pb = (0x010120 >> (4 * ld_seg)) & 15;
-      offA += pa * p.A.plane;
-      offB += pb * p.B.plane;
+      curA += 2 * pa * p.A.plane;
+      curB += 2 * pb * p.B.plane;
     }
+  };
+  // A contraction that is not whole stages: the chunks behind its end are copied from the row's first chunk instead (`back` bytes
+  // before: in bounds whatever the matrix) and overwritten with zeros in LDS when they have landed.
+  const int ktail = (int)(p.K & 63);
+  int back0 = 0, back1 = 0;  // copies of an even / odd group of 8 rows
+  auto set_back = [&]() {
+    const bool tail = ktail != 0 && ld_k + 1 == g.nkt;
+    const int c0 = sq ^ (srow >> 1), c1 = sq ^ (4 | (srow >> 1));
+    back0 = tail && 8 * c0 >= ktail ? 16 * c0 : 0;
+    back1 = tail && 8 * c1 >= ktail ? 16 * c1 : 0;
   };
   auto advance = [&]() {  // past the last stage the copies repeat it; nobody reads the repetition
     if (ld_t + 1 < t1) {
@@ -141,15 +162,25 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
         ld_k = 0;
         ++ld_seg;
       }
-      set_off();
+      set_cur();
+      set_back();
     }
   };
   auto copy = [&](int buf, int i) {
     const bool isA = i < PA;
-    unsigned char* dst = lds + buf * STAGE + (isA ? (wid * PA + i) * 1024 : OPA + (wid * PB + i - PA) * 1024);
-    const unsigned short* s = src[i] + (isA ? offA : offB);
-    if ((int64_t)ld_k * 64 + chunk8[i] >= p.K) s = g_zero_chunk;
-    __builtin_amdgcn_global_load_lds((glb_cv*)s, (lds_v*)dst, 16, 0, 0);
+    const int grp = isA ? wid * PA + i : wid * PB + i - PA;
+    unsigned char* dst = lds + buf * STAGE + (isA ? 0 : OPA) + grp * 1024;
+    // (the groups of a wave start at an even one unless it has a single one per operand)
+    const int back = (isA ? PA : PB) % 2 == 0 ? (((isA ? i : i - PA) & 1) ? back1 : back0) : ((grp & 1) ? back1 : back0);
+    __builtin_amdgcn_global_load_lds((glb_cv*)((isA ? curA : curB) + (voff[i] - (unsigned)back)), (lds_v*)dst, 16, 0, 0);
+  };
+  auto zero_tail = [&](int buf) {
+    const int first = (ktail + 7) / 8, n = 8 - first;
+    for (int e = tid; e < (BM + BN) * n; e += NW * 64) {
+      const int r = e / n, c = first + e % n;  // (row BM + r of the stage is row r of B: BM is a multiple of 16)
+      *reinterpret_cast<u16x8*>(lds + buf * STAGE + r * 128 + ((c ^ ((r >> 1) & 7)) << 4)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    wait_lds_barrier();
   };
 
   f32x16 acc[TM][TN];
@@ -160,32 +191,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  int ra[TM], sa[TM], rb[TN], sb[TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int r = wm * TM * 32 + i * 32 + l31;
-    ra[i] = r * 128;
-    sa[i] = (r >> 1) & 7;
-  }
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int r = wn * TN * 32 + j * 32 + l31;
-    rb[j] = OPA + r * 128;
-    sb[j] = (r >> 1) & 7;
-  }
+  // rows 32 apart have the same swizzle: one address per operand and chunk
+  const int ra = (wm * TM * 32 + l31) * 128, rb = OPA + (wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
   u16x8 av[2][TM], bv[2][TN];
-  auto reads = [&](int set, const unsigned char* S, int kk) {
-    const int c = 2 * kk + h;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) av[set][i] = *reinterpret_cast<const u16x8*>(S + ra[i] + ((c ^ sa[i]) << 4));
-#pragma unroll
-    for (int j = 0; j < TN; ++j) bv[set][j] = *reinterpret_cast<const u16x8*>(S + rb[j] + ((c ^ sb[j]) << 4));
+  // read n of a unit's TM + TN: the operands in the order in which the matrix instructions want them
+  auto read = [&](int set, const unsigned char* S, int kk, int n) {
+    const int c = ((2 * kk + h) ^ sw) << 4;
+    if (n == 0) av[set][0] = *reinterpret_cast<const u16x8*>(S + ra + c);
+    else if (n <= TN) bv[set][n - 1] = *reinterpret_cast<const u16x8*>(S + rb + (n - 1) * 32 * 128 + c);
+    else av[set][n - TN] = *reinterpret_cast<const u16x8*>(S + ra + (n - TN) * 32 * 128 + c);
   };
-  auto unit = [&](int set, auto pre, auto next) {
+  // one matrix instruction at a time, and in its shadow what `beside` issues
+  auto unit = [&](int set, auto beside) {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      pre(i);
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         if constexpr (MT == D_F16)
@@ -194,51 +213,62 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
         else
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, av[set][i]),
                                                               __builtin_bit_cast(bf16x8, bv[set][j]), acc[i][j], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (i == 0) {
-        next();
+        __builtin_amdgcn_sched_barrier(0);
+        beside(i * TN + j);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
-  auto none = [](int) {};
-  // copies 0 .. H-1 of a stage go out in the last unit of the stage before the previous one, H .. NP-1 in the first unit of the previous
-  constexpr int H = NP / 2, Q = (H + TM - 1) / TM;
+  constexpr int NM = TM * TN, NR = TM + TN, QR = (NR + NM - 1) / NM;
+  auto reads = [&](int set, const unsigned char* S, int kk, int m) {
+#pragma unroll
+    for (int q = 0; q < QR; ++q)
+      if (m * QR + q < NR) read(set, S, kk, m * QR + q);
+  };
+  // copies first .. first + n - 1 of a stage, spread evenly over the NM matrix instructions of a unit
+  auto copies = [&](int buf, int first, int n, int m) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (i >= first && i < first + n && (i - first) * NM / n == m) copy(buf, i);
+  };
+  // Units 0, 1, 2 of stage t work on its columns while the next unit's are read. Behind the barrier every wave has the stage's last
+  // columns in registers -- its buffer is free for stage t + 2 -- and stage t + 1 has landed: unit 3 reads the first columns of t + 1
+  // and issues the first half of the copies of t + 2, unit 0 of t + 1 the other half. (A CU takes one copy per 16 cycles: all of them in
+  // one unit stall the waves that issue them; 8192^3 bf16: 62 % of the matrix cores' cycles, 71 % with the halves.)
+  constexpr int H = NP / 2;
   if (t1 > t0) {
-    set_off();
+    int rd_k = ld_k;  // column block of the stage that is read
+    set_cur();
+    set_back();
 #pragma unroll
     for (int i = 0; i < NP; ++i) copy(0, i);
-    __syncthreads();
     advance();
 #pragma unroll
     for (int i = 0; i < H; ++i) copy(1, i);
-    reads(0, lds, 0);
+    wait_barrier<H>();
+    if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(0);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) read(0, lds, 0, n);
     for (int t = t0; t < t1; ++t) {
       const int cur = (t - t0) & 1;
       const unsigned char* S = lds + cur * STAGE;
       const unsigned char* Sn = lds + (cur ^ 1) * STAGE;
-      unit(0,
-           [&](int i) {
-#pragma unroll
-             for (int q = 0; q < Q; ++q)
-               if (H + i * Q + q < NP) copy(cur ^ 1, H + i * Q + q);
-           },
-           [&]() { reads(1, S, 1); });
-      unit(1, none, [&]() { reads(0, S, 2); });
-      unit(0, none, [&]() { reads(1, S, 3); });
-      __syncthreads();  // every wave has its reads of `cur` behind it; the next stage has landed in the other buffer
+      unit(0, [&](int m) {
+        reads(1, S, 1, m);
+        copies(cur ^ 1, H, NP - H, m);
+      });
+      unit(1, [&](int m) { reads(0, S, 2, m); });
+      unit(0, [&](int m) { reads(1, S, 3, m); });
+      wait_barrier<0>();
+      rd_k = rd_k + 1 == g.nkt ? 0 : rd_k + 1;
+      if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(cur ^ 1);
       advance();
-      unit(1,
-           [&](int i) {
-#pragma unroll
-             for (int q = 0; q < Q; ++q)
-               if (i * Q + q < H) copy(cur, i * Q + q);
-           },
-           [&]() { reads(0, Sn, 0); });
+      unit(1, [&](int m) {
+        reads(0, Sn, 0, m);
+        copies(cur, 0, H, m);
+      });
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may land in the epilogue's LDS
-    __syncthreads();
+    wait_barrier<0>();  // no copy may land in the epilogue's LDS
   }
 
   // ---- epilogue: 32 rows x 32 TN columns of the wave at a time. D: column = lane & 31, row = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
@@ -258,8 +288,25 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
         if (e < nin) bias8[e] = Elem<OT>::ld(static_cast<const E*>(p.bias) + col + e);
     }
   }
+  // the residual of a block of 32 rows is loaded while the block before it is worked on (three planes: at the start of its own)
+  constexpr int NS = 32 / RP, DB = RT == D_PL3 ? 0 : 1;
+  Raw8<RT> res[1 + DB][NS];
+  auto fetch_res = [&](int i) {
+    if constexpr (!PART) {
+      if (p.res.p && nin > 0) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
+        for (int s = 0; s < NS; ++s) {
+          const int64_t row = m0 + wm * TM * 32 + i * 32 + s * RP + cr;
+          if (row < p.M) res[(i * DB) & 1][s].load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
+        }
+      }
+    }
+  };
+  if (DB) fetch_res(0);
+  auto rows32 = [&](auto I) {
+    constexpr int i = decltype(I)::value;
+    if constexpr (DB == 0) fetch_res(i);
+    else if constexpr (i + 1 < TM) fetch_res(i + 1);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -293,7 +340,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
                                      p.B.plane, p.K);
           }
         }
-        Epilogue<OT, RT, PART>::apply(p, batch, row, col, nin, row_in, v, bias8);
+        Epilogue<OT, RT, PART>::apply(p, batch, row, col, nin, row_in, v, bias8, res[(i * DB) & 1][s]);
         if (p.out.p) {
           const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
           const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
@@ -328,7 +375,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product(ProdArgs g) {
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-  }
+  };
+  static_for<TM>(rows32);  // (unrolled whatever its length: the accumulators stay in registers)
 }
 
 // the slabs of a split contraction, added in order, through the same epilogue: a 32 x 64 block of C per workgroup
@@ -369,7 +417,9 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
       }
     }
   }
-  Epilogue<OT, RT, false>::apply(p, batch, row, col, nin, row_in, v, bias8);
+  Raw8<RT> res;
+  if (p.res.p && row_in && nin > 0) res.load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
+  Epilogue<OT, RT, false>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
   if (p.out.p) {
     const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
     const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
@@ -399,16 +449,19 @@ struct Tile { int bm, bn; };
 // what a workgroup's tile costs per 64 columns of the contraction, in units of 1e-9 s at full occupancy (measured, see product())
 struct Plan { int tile, ksplit, kchunk, tm, tn; int64_t tiles; };
 
+// a lane's place below its tile's base has 32 bits: 64 rows of 2^25 elements, 256 of 2^23
+constexpr int64_t MAX_LD = (int64_t)1 << 25, MAX_LD_BIG = (int64_t)1 << 22;
+
 Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric, bool may_split) {
   static const int BM[3] = {256, 128, 64};
   const int64_t nst = std::max<int64_t>(1, (type == D_PL3 ? 6 : 1) * ((K + 63) / 64));
   Plan best{};
   double best_t = 1e300;
-  for (int t = 0; t < 3; ++t) {
+  for (int t = K > MAX_LD_BIG ? 2 : 0; t < 3; ++t) {
     const int64_t tm = (M + BM[t] - 1) / BM[t], tn = (N + BM[t] - 1) / BM[t];
     const int64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
     // time of one stage of one workgroup when its CU is full, and workgroups a CU holds at once
-    static const double stage_us[3] = {0.95, 0.36, 0.14};
+    static const double stage_us[3] = {1.3, 0.45, 0.18};
     static const int res[3] = {1, 2, 4};
     for (int ks = 1; ks <= 32; ks *= 2) {
       if (ks > 1 && (!may_split || nst / ks < 4)) break;
@@ -444,7 +497,7 @@ int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
 }
 template <int MT, int OT, int RT, bool PART>
 int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile) {
-  if (tile == 0) return launch<MT, OT, RT, PART, 2, 4, 4, 2>(ctx, st, g, grid);
+  if (tile == 0) return launch<MT, OT, RT, PART, 2, 2, 4, 4>(ctx, st, g, grid);
   if (tile == 1) return launch<MT, OT, RT, PART, 2, 2, 2, 2>(ctx, st, g, grid);
   return launch<MT, OT, RT, PART, 2, 2, 1, 1>(ctx, st, g, grid);
 }
@@ -470,6 +523,7 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return SCLENS_OK;
   const int64_t slab = p.slabs ? product_slab_bytes(p.M, p.N, p.K, p.batch, p.type, p.symmetric) : 0;
   const Plan pl = plan_product(p.M, p.N, p.K, p.batch, p.type, p.symmetric, p.slabs && slab <= p.slab_bytes);
+  if (std::max(p.A.ld, p.B.ld) > MAX_LD) return ctx->fail(SCLENS_ERR_ARG, "product: a contraction of more than 2^25 columns");
   if (pl.tiles > 0x7fffffff || p.batch > 65535) return ctx->fail(SCLENS_ERR_ARG, "product: too many tiles");
   ProdArgs g{};
   g.p = p;

@@ -18,7 +18,7 @@ int no_room(Ctx* ctx, int64_t need) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // a 16-bit matrix whose rows start on 16 bytes and whose contraction is whole 8-column chunks feeds the products as it lies
-bool direct(int dtype, const void* p, int64_t ld, int64_t K) { return dtype != D_F32 && ld % 8 == 0 && K % 8 == 0 && aligned16(p); }
+bool direct(int dtype, const void* p, int64_t ld, int64_t K) { return dtype != D_F32 && ld % 8 == 0 && ld <= ((int64_t)1 << 22) && K % 8 == 0 && aligned16(p); }
 
 Mat user_mat(const void* p, int64_t ld, int64_t batch = 0) {
   Mat m;
@@ -126,9 +126,10 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
       if (act != ACT_NONE) {
         float zz[8];
         load8<T>(z, row * z.ld + col, nin, zz);
+        act8<true>(zz, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < nin) v[e] *= act_grad(zz[e], act);
+          if (e < nin) v[e] *= zz[e];
       }
     }
     if (img.p && row < M) store8<IT>(img, row * img.ld + col, 8, v);
@@ -240,9 +241,12 @@ __global__ __launch_bounds__(256) void k_sumsq(const typename Elem<T>::type* __r
   const auto* p = x + (int64_t)blockIdx.y * batch;
   double s = 0.0;
   for (int64_t r = (int64_t)blockIdx.x * rpb + tr; r < rows; r += (int64_t)gridDim.x * rpb)
-    for (int64_t c = tc; c < cols; c += tpr) {
-      const double v = (double)Elem<T>::ld(p + r * ld + c);
-      s += v * v;
+    for (int64_t c = tc; c < cols; c += 8 * tpr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double v = c + e * tpr < cols ? (double)Elem<T>::ld(p + r * ld + c + e * tpr) : 0.0;
+        s += v * v;
+      }
     }
   S[tid] = s;
   __syncthreads();
@@ -262,10 +266,11 @@ __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64
   const int64_t nb = (cols + 63) / 64, b = blockIdx.y;
   const int64_t m0 = (blockIdx.x / nb) * 64, n0 = (blockIdx.x % nb) * 64;
   const int tid = threadIdx.x, cc = (tid & 7) * 8;
-  if (tid == 0) {
+  if (tid < 64) {
     double s = 0.0;
-    for (int i = 0; i < nparts; ++i) s += part[b * nparts + i];
-    factor = scale / (sqrt(s) + eps);
+    for (int i = tid; i < nparts; i += 64) s += part[b * nparts + i];
+    for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w);
+    if (tid == 0) factor = scale / (sqrt(s) + eps);
   }
   __syncthreads();
   const double f = factor;
@@ -334,7 +339,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   const int IT = f32 ? D_PL3 : D_F16, img_dtype = f32 ? D_F32 : D_F16;
   Carve c(ws);
   const int64_t elems = m * n;
-  const int nparts = (int)std::min<int64_t>(64, std::max<int64_t>(1, elems / 8192));
+  const int nparts = (int)std::min<int64_t>(1024, std::max<int64_t>(1, elems / 8192));
   double* part = c.take<double>(a.batch * nparts);
   Mat X[2], XT[2];
   for (int i = 0; i < (a.steps > 1 ? 2 : 1); ++i) {
