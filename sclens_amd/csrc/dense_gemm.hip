@@ -25,6 +25,10 @@ __device__ __forceinline__ void wait_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 struct ProdArgs {
@@ -50,7 +54,13 @@ __device__ __forceinline__ void static_for(F f) {
   }
 }
 
-template <int OT, int RT, bool PART>
+// LDS traffic between the lanes of one wave, in order
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <int OT, int RT>
 struct Epilogue {
   // 8 columns from col of row `row`, n of them inside (images with `pad`: all 8, those outside as zeros)
   static __device__ __forceinline__ void apply(const Product& p, int64_t b, int64_t row, int64_t col, int nin, bool row_in, float v[8],
@@ -208,11 +218,11 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         if constexpr (MT == D_F16)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, av[set][i]), __builtin_bit_cast(f16x8, bv[set][j]),
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, bv[set][j]), __builtin_bit_cast(f16x8, av[set][i]),
                                                              acc[i][j], 0, 0, 0);
         else
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, av[set][i]),
-                                                              __builtin_bit_cast(bf16x8, bv[set][j]), acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bv[set][j]),
+                                                              __builtin_bit_cast(bf16x8, av[set][i]), acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         beside(i * TN + j);
         __builtin_amdgcn_sched_barrier(0);
@@ -271,65 +281,162 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
     wait_barrier<0>();  // no copy may land in the epilogue's LDS
   }
 
-  // ---- epilogue: 32 rows x 32 TN columns of the wave at a time. D: column = lane & 31, row = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
-  constexpr int C = 32 * TN, LP = C + 4, CH = C / 8, RP = 64 / CH;  // RP rows per pass, 8 columns per lane
+  // ---- epilogue: 32 rows x 32 TN columns of the wave at a time, turned through LDS. D (B's rows are the matrix instruction's rows): row
+  // of C = lane & 31, column = (e & 3) + 8 (e >> 2) + 4 (lane >> 5). The loops stay rolled: unrolled, their 250 KB of instructions (every activation, every edge) cost a workgroup 25 us.
+  constexpr int C = 32 * TN, LP = C + 4, CH = C / 8, RP = 64 / CH, NS = 32 / RP;  // RP rows per pass, 8 columns per lane
   float* T = reinterpret_cast<float*>(lds) + wid * 32 * LP;
   const int cc = (lane % CH) * 8, cr = lane / CH;
-  const int64_t col = n0 + wn * C + cc;
+  const int64_t col = n0 + wn * C + cc, row_w = m0 + wm * TM * 32;
   const int nin = (int)max((int64_t)0, min((int64_t)8, p.N - col));
-  float bias8[8];
+  auto to_lds = [&](int i) {
+    static_for<TM>([&](auto I) {
+      constexpr int n = decltype(I)::value;
+      if (i == n) {
+        // (the two markers keep the branches from being merged into one that picks its accumulators by index, from scratch memory)
+        asm volatile("; rows %0" ::"n"(n) : "memory");
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bias8[e] = 0.f;
-  if constexpr (!PART && OT != D_PL3) {
-    if (p.bias) {
-      typedef typename Elem<OT>::type E;
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < nin) bias8[e] = Elem<OT>::ld(static_cast<const E*>(p.bias) + col + e);
-    }
-  }
-  // the residual of a block of 32 rows is loaded while the block before it is worked on (three planes: at the start of its own)
-  constexpr int NS = 32 / RP, DB = RT == D_PL3 ? 0 : 1;
-  Raw8<RT> res[1 + DB][NS];
-  auto fetch_res = [&](int i) {
-    if constexpr (!PART) {
-      if (p.res.p && nin > 0) {
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<f32x4*>(&T[l31 * LP + j * 32 + 8 * e + 4 * h]) =
+                f32x4{acc[n][j][4 * e], acc[n][j][4 * e + 1], acc[n][j][4 * e + 2], acc[n][j][4 * e + 3]};
+        asm volatile("; rows %0" ::"n"(n) : "memory");
+      }
+    });
+    wave_sync();
+  };
+  auto from_lds = [&](int lr, float v[8]) {
+    const f32x4 va = *reinterpret_cast<const f32x4*>(&T[lr * LP + cc]), vb = *reinterpret_cast<const f32x4*>(&T[lr * LP + cc + 4]);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          const int64_t row = m0 + wm * TM * 32 + i * 32 + s * RP + cr;
-          if (row < p.M) res[(i * DB) & 1][s].load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
+    for (int e = 0; e < 4; ++e) { v[e] = va[e]; v[4 + e] = vb[e]; }
+  };
+  if constexpr (PART) {
+    float* out = p.slabs + (((int64_t)blockIdx.z * p.batch + batch) * p.M + row_w) * round_up8(p.N) + col;
+#pragma unroll 1
+    for (int i = 0; i < TM; ++i) {
+      to_lds(i);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        float v[8];
+        from_lds(s * RP + cr, v);
+        const int64_t r = i * 32 + s * RP + cr;
+        if (row_w + r < p.M && nin > 0) {
+          *reinterpret_cast<f32x4*>(out + r * round_up8(p.N)) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(out + r * round_up8(p.N) + 4) = f32x4{v[4], v[5], v[6], v[7]};
         }
       }
+      wave_sync();
     }
-  };
-  if (DB) fetch_res(0);
-  auto rows32 = [&](auto I) {
-    constexpr int i = decltype(I)::value;
-    if constexpr (DB == 0) fetch_res(i);
-    else if constexpr (i + 1 < TM) fetch_res(i + 1);
+  } else {
+    float bias8[8];
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int e = 0; e < 8; ++e) bias8[e] = 0.f;
+    if constexpr (OT != D_PL3) {
+      if (p.bias) {
+        Mat b;
+        b.p = const_cast<void*>(p.bias);
+        b.vec = reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;  // (col is a multiple of 8)
+        load8<OT>(b, col, nin, bias8);
+      }
+    }
+    const Mat& ot = p.symmetric ? p.out : p.outT;
+    const bool turned = p.outT.p || (p.symmetric && ti != tj);
+    // column c of block i becomes row n0 + c of the transpose: 8 of its 32 entries per lane
+    auto turn = [&](int i) {
+      if (!turned) return;
+      wave_sync();
+#pragma unroll 1
+      for (int s = 0; s < C / 16; ++s) {
+          const int gq = lane & 3, c = s * 16 + (lane >> 2);
+          const int64_t trow = n0 + wn * C + c, tcol = row_w + i * 32 + 8 * gq;
+          float v[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) T[((e & 3) + 8 * (e >> 2) + 4 * h) * LP + j * 32 + l31] = acc[i][j][e];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int64_t row0 = m0 + wm * TM * 32 + i * 32;
-#pragma unroll
-    for (int s = 0; s < 32 / RP; ++s) {
-      const int lr = s * RP + cr;
-      const int64_t row = row0 + lr;
-      float v[8];
-      const f32x4 va = *reinterpret_cast<const f32x4*>(&T[lr * LP + cc]), vb = *reinterpret_cast<const f32x4*>(&T[lr * LP + cc + 4]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { v[e] = va[e]; v[4 + e] = vb[e]; }
-      if constexpr (PART) {
-        float* out = p.slabs + (((int64_t)blockIdx.z * p.batch + batch) * p.M + row) * round_up8(p.N) + col;
-        if (row < p.M && nin > 0) {
-          *reinterpret_cast<f32x4*>(out) = va;
-          *reinterpret_cast<f32x4*>(out + 4) = vb;
+          for (int e = 0; e < 8; ++e) v[e] = T[(8 * gq + e) * LP + c];
+          const int tin = (int)max((int64_t)0, min((int64_t)8, p.M - tcol));
+          const int n = ot.pad ? (tin > 0 ? 8 : 0) : tin;
+          const bool rin = ot.pad ? trow < round_up8(p.N) : trow < p.N;
+          if (rin && n > 0) store8<OT>(ot, batch * ot.batch + trow * ot.ld + tcol, n, v);
         }
-      } else {
+      };
+    // A tile that lies inside the matrix, all its rows on 16 bytes: nothing to guard. Loads and stores share a counter, so a residual
+    // that came through registers would make every pass wait for the stores of the pass before it (32 times a microsecond): it goes to
+    // LDS, the next block's while this one is worked on, and only the copies are waited for (the stores since are counted off).
+    const bool inside = m0 + BM <= p.M && n0 + BN <= p.N && (!p.out.p || p.out.vec) && (!p.pre.p || p.pre.vec) && (!p.res.p || p.res.vec);
+    if constexpr (!PL) {
+      if (inside) {
+        const int64_t row0 = row_w + cr;
+        const char* pr = static_cast<const char*>(p.res.p) + 2 * (batch * p.res.batch + row0 * p.res.ld + col);
+        char* po = static_cast<char*>(p.out.p) + 2 * (batch * p.out.batch + row0 * p.out.ld + col);
+        char* pz = static_cast<char*>(p.pre.p) + 2 * (batch * p.pre.batch + row0 * p.pre.ld + col);
+        const int64_t sr = 2 * RP * p.res.ld, so = 2 * RP * p.out.ld, sz = 2 * RP * p.pre.ld;
+        const bool has_res = p.res.p != nullptr, has_out = p.out.p != nullptr, has_pre = p.pre.p != nullptr;
+        unsigned char* R = lds + NW * 32 * LP * 4 + wid * 2 * NS * 1024;
+        auto copy_res = [&](int buf) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            __builtin_amdgcn_global_load_lds((glb_cv*)pr, (lds_v*)(R + (buf * NS + s) * 1024), 16, 0, 0);
+            pr += sr;
+          }
+        };
+        Mat plain;
+        plain.vec = 1;
+        if (has_res) copy_res(0);
+#pragma unroll 1
+        for (int i = 0; i < TM; ++i) {
+          if (has_res) {
+            if (i == 0 || turned) wait_vm<0>();
+            else if (has_out && has_pre) wait_vm<2 * NS>();
+            else wait_vm<NS>();
+            if (i + 1 < TM) copy_res((i + 1) & 1);
+          }
+          to_lds(i);
+          const unsigned char* Ri = R + (i & 1) * NS * 1024 + lane * 16;
+#pragma unroll 1
+          for (int s = 0; s < NS; ++s) {
+            float v[8];
+            from_lds(s * RP + cr, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], p.alpha, bias8[e]);
+            if (has_pre) {
+              plain.p = pz;
+              store8<OT>(plain, 0, 8, v);
+              pz += sz;
+            }
+            if (p.act != ACT_NONE) act8<false>(v, p.act);
+            if (has_res) {
+              const u16x8 r = *reinterpret_cast<const u16x8*>(Ri + s * 1024);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const unsigned short q = r[e];
+                v[e] = fmaf(p.beta, Elem<RT>::ld(&q), v[e]);
+              }
+            }
+            if (has_out) {
+              plain.p = po;
+              store8<OT>(plain, 0, 8, v);
+              po += so;
+            }
+            if (turned) {
+              *reinterpret_cast<f32x4*>(&T[(s * RP + cr) * LP + cc]) = f32x4{v[0], v[1], v[2], v[3]};
+              *reinterpret_cast<f32x4*>(&T[(s * RP + cr) * LP + cc + 4]) = f32x4{v[4], v[5], v[6], v[7]};
+            }
+          }
+          turn(i);
+          wave_sync();
+        }
+        return;
+      }
+    }
+#pragma unroll 1
+    for (int i = 0; i < TM; ++i) {
+      to_lds(i);
+#pragma unroll 1
+      for (int s = 0; s < NS; ++s) {
+        const int lr = s * RP + cr;
+        const int64_t row = row_w + i * 32 + lr;
         const bool row_in = row < p.M;
+        float v[8];
+        from_lds(lr, v);
         if constexpr (PL) {
           if (row_in) {
 #pragma unroll
@@ -340,43 +447,23 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
                                      p.B.plane, p.K);
           }
         }
-        Epilogue<OT, RT, PART>::apply(p, batch, row, col, nin, row_in, v, bias8, res[(i * DB) & 1][s]);
+        Raw8<RT> res;
+        if (p.res.p && row_in && nin > 0) res.load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
+        Epilogue<OT, RT>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
         if (p.out.p) {
           const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
           const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
           if (rin && n > 0) store8<OT>(p.out, batch * p.out.batch + row * p.out.ld + col, n, v);
         }
-        if (p.outT.p || p.symmetric) {
-          f32x4 wa = {v[0], v[1], v[2], v[3]}, wb = {v[4], v[5], v[6], v[7]};
-          *reinterpret_cast<f32x4*>(&T[lr * LP + cc]) = wa;
-          *reinterpret_cast<f32x4*>(&T[lr * LP + cc + 4]) = wb;
+        if (turned) {
+          *reinterpret_cast<f32x4*>(&T[lr * LP + cc]) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(&T[lr * LP + cc + 4]) = f32x4{v[4], v[5], v[6], v[7]};
         }
       }
+      turn(i);
+      wave_sync();
     }
-    if constexpr (!PART) {
-      if (p.outT.p || (p.symmetric && ti != tj)) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const Mat& o = p.symmetric ? p.out : p.outT;
-        // column c of the block becomes row n0 + c of the transpose: 8 of its 32 entries per lane
-#pragma unroll
-        for (int s = 0; s < C / 16; ++s) {
-          const int gq = lane & 3, c = s * 16 + (lane >> 2);
-          const int64_t trow = n0 + wn * C + c, tcol = row0 + 8 * gq;
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = T[(8 * gq + e) * LP + c];
-          const int tin = (int)max((int64_t)0, min((int64_t)8, p.M - tcol));
-          const int n = o.pad ? (tin > 0 ? 8 : 0) : tin;
-          const bool rin = o.pad ? trow < round_up8(p.N) : trow < p.N;
-          if (rin && n > 0) store8<OT>(o, batch * o.batch + trow * o.ld + tcol, n, v);
-        }
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  };
-  static_for<TM>(rows32);  // (unrolled whatever its length: the accumulators stay in registers)
+  }
 }
 
 // the slabs of a split contraction, added in order, through the same epilogue: a 32 x 64 block of C per workgroup
@@ -419,7 +506,7 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
   }
   Raw8<RT> res;
   if (p.res.p && row_in && nin > 0) res.load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
-  Epilogue<OT, RT, false>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
+  Epilogue<OT, RT>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
   if (p.out.p) {
     const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
     const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
@@ -488,7 +575,8 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
 
 template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN>
 int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
-  constexpr int LDS = 2 * (WM * TM + WN * TN) * 32 * 128;
+  // two stages; the epilogue's blocks of fp32 and two blocks of a 16-bit residual per wave
+  constexpr int LDS = std::max(2 * (WM * TM + WN * TN) * 32 * 128, WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * 32 * TN * 2));
   const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, WM, WN, TM, TN>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
   hipLaunchKernelGGL((k_product<MT, OT, RT, PART, WM, WN, TM, TN>), grid, dim3(WM * WN * 64), LDS, st, g);
