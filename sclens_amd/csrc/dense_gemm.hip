@@ -2,8 +2,9 @@
 // v_mfma_f32_32x32x16_{bf16,f16} with fp32 accumulation.
 //   * fp32 operands come as three bf16 planes (24 bits, exact): six products per term, smallest first -- p2 p0, p0 p2, p1 p1, p1 p0,
 //     p0 p1, p0 p0; what is left out (2 p1 p2) is at most 2^-23 of the term and 2^-26 in the mean square, the size of fp32's own rounding.
-//   * a workgroup owns one BM x BN tile; both operands go to LDS 64 columns at a time straight from memory (16 bytes per lane), two
-//     stages in turn. Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): 16 rows at one chunk fall into 16 different
+//   * a workgroup owns one BM x BN tile; both operands go to LDS 64 columns at a time straight from memory (16 bytes per lane),
+//     S stages in turn: two where two workgroups share a CU or one fills it with 128 x 128 per wave, four where a single workgroup of a
+//     small tile would wait for each stage (0.57 us per stage of a 64 x 64 tile with two, whatever the work in it). Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): 16 rows at one chunk fall into 16 different
 //     16-byte bank groups, so a 16-byte read runs without conflicts.
 //   * the stage loop is a software pipeline of units of 16 columns: the reads of the next unit, and in the stage's last unit the copies
 //     of the stage after the next, are issued one at a time in the shadow of the matrix instructions.
@@ -93,7 +94,7 @@ __device__ __forceinline__ float recompute_f32(const unsigned short* A, const un
   return s;
 }
 
-template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN>
+template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(ProdArgs g) {
   constexpr int NW = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, NP = PA + PB;  // 1 KB copies (8 rows x 64 columns) per wave and stage
@@ -205,11 +206,11 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   const int ra = (wm * TM * 32 + l31) * 128, rb = OPA + (wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
   u16x8 av[2][TM], bv[2][TN];
   // read n of a unit's TM + TN: the operands in the order in which the matrix instructions want them
-  auto read = [&](int set, const unsigned char* S, int kk, int n) {
+  auto read = [&](int set, const unsigned char* B, int kk, int n) {
     const int c = ((2 * kk + h) ^ sw) << 4;
-    if (n == 0) av[set][0] = *reinterpret_cast<const u16x8*>(S + ra + c);
-    else if (n <= TN) bv[set][n - 1] = *reinterpret_cast<const u16x8*>(S + rb + (n - 1) * 32 * 128 + c);
-    else av[set][n - TN] = *reinterpret_cast<const u16x8*>(S + ra + (n - TN) * 32 * 128 + c);
+    if (n == 0) av[set][0] = *reinterpret_cast<const u16x8*>(B + ra + c);
+    else if (n <= TN) bv[set][n - 1] = *reinterpret_cast<const u16x8*>(B + rb + (n - 1) * 32 * 128 + c);
+    else av[set][n - TN] = *reinterpret_cast<const u16x8*>(B + ra + (n - TN) * 32 * 128 + c);
   };
   // one matrix instruction at a time, and in its shadow what `beside` issues
   auto unit = [&](int set, auto beside) {
@@ -230,10 +231,10 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
     }
   };
   constexpr int NM = TM * TN, NR = TM + TN, QR = (NR + NM - 1) / NM;
-  auto reads = [&](int set, const unsigned char* S, int kk, int m) {
+  auto reads = [&](int set, const unsigned char* B, int kk, int m) {
 #pragma unroll
     for (int q = 0; q < QR; ++q)
-      if (m * QR + q < NR) read(set, S, kk, m * QR + q);
+      if (m * QR + q < NR) read(set, B, kk, m * QR + q);
   };
   // copies first .. first + n - 1 of a stage, spread evenly over the NM matrix instructions of a unit
   auto copies = [&](int buf, int first, int n, int m) {
@@ -242,52 +243,59 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
       if (i >= first && i < first + n && (i - first) * NM / n == m) copy(buf, i);
   };
   // Units 0, 1, 2 of stage t work on its columns while the next unit's are read. Behind the barrier every wave has the stage's last
-  // columns in registers -- its buffer is free for stage t + 2 -- and stage t + 1 has landed: unit 3 reads the first columns of t + 1
-  // and issues the first half of the copies of t + 2, unit 0 of t + 1 the other half. (A CU takes one copy per 16 cycles: all of them in
-  // one unit stall the waves that issue them; 8192^3 bf16: 62 % of the matrix cores' cycles, 71 % with the halves.)
+  // columns in registers -- its buffer is free for stage t + S -- and stage t + 1 has landed (of the wave's copies only those of the
+  // stages t + 2 .. t + S - 1 may still be on their way): unit 3 reads the first columns of t + 1 and issues the first half of the copies
+  // of t + S, unit 0 of t + 1 the other half. (A CU takes one copy per 16 cycles: all of them in one unit stall the waves that issue
+  // them; 8192^3 bf16: 62 % of the matrix cores' cycles, 71 % with the halves.)
   constexpr int H = NP / 2;
   if (t1 > t0) {
     int rd_k = ld_k;  // column block of the stage that is read
     set_cur();
     set_back();
 #pragma unroll
-    for (int i = 0; i < NP; ++i) copy(0, i);
-    advance();
+    for (int b = 0; b < S; ++b) {
+      if (b > 0) advance();
 #pragma unroll
-    for (int i = 0; i < H; ++i) copy(1, i);
-    wait_barrier<H>();
+      for (int i = 0; i < (b + 1 < S ? NP : H); ++i) copy(b, i);
+    }
+    wait_barrier<(S - 2) * NP + H>();
     if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(0);
 #pragma unroll
     for (int n = 0; n < NR; ++n) read(0, lds, 0, n);
+    int cur = 0, prev = S - 1;  // buffers of the stage worked on and of the one before it, whose copies are half issued
     for (int t = t0; t < t1; ++t) {
-      const int cur = (t - t0) & 1;
-      const unsigned char* S = lds + cur * STAGE;
-      const unsigned char* Sn = lds + (cur ^ 1) * STAGE;
+      const int nxt = cur + 1 == S ? 0 : cur + 1;
+      const unsigned char* B = lds + cur * STAGE;
+      const unsigned char* Bn = lds + nxt * STAGE;
       unit(0, [&](int m) {
-        reads(1, S, 1, m);
-        copies(cur ^ 1, H, NP - H, m);
+        reads(1, B, 1, m);
+        copies(prev, H, NP - H, m);
       });
-      unit(1, [&](int m) { reads(0, S, 2, m); });
-      unit(0, [&](int m) { reads(1, S, 3, m); });
-      wait_barrier<0>();
+      unit(1, [&](int m) { reads(0, B, 2, m); });
+      unit(0, [&](int m) { reads(1, B, 3, m); });
+      wait_barrier<(S - 2) * NP>();
       rd_k = rd_k + 1 == g.nkt ? 0 : rd_k + 1;
-      if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(cur ^ 1);
+      if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(nxt);
       advance();
       unit(1, [&](int m) {
-        reads(0, Sn, 0, m);
+        reads(0, Bn, 0, m);
         copies(cur, 0, H, m);
       });
+      prev = cur;
+      cur = nxt;
     }
     wait_barrier<0>();  // no copy may land in the epilogue's LDS
   }
 
   // ---- epilogue: 32 rows x 32 TN columns of the wave at a time, turned through LDS. D (B's rows are the matrix instruction's rows): row
   // of C = lane & 31, column = (e & 3) + 8 (e >> 2) + 4 (lane >> 5). The loops stay rolled: unrolled, their 250 KB of instructions (every activation, every edge) cost a workgroup 25 us.
-  constexpr int C = 32 * TN, LP = C + 4, CH = C / 8, RP = 64 / CH, NS = 32 / RP;  // RP rows per pass, 8 columns per lane
+  constexpr int C = 32 * TN, LP = C + 4, CH = TN == 3 ? 16 : C / 8, RP = 64 / CH, NS = 32 / RP;  // RP rows per pass, 8 columns per lane
   float* T = reinterpret_cast<float*>(lds) + wid * 32 * LP;
-  const int cc = (lane % CH) * 8, cr = lane / CH;
+  // (96 columns are twelve lanes of sixteen: the last four repeat the twelfth and store nothing)
+  const bool mine = (lane % CH) * 8 < C;
+  const int cc = mine ? (lane % CH) * 8 : C - 8, cr = lane / CH;
   const int64_t col = n0 + wn * C + cc, row_w = m0 + wm * TM * 32;
-  const int nin = (int)max((int64_t)0, min((int64_t)8, p.N - col));
+  const int nin = mine ? (int)max((int64_t)0, min((int64_t)8, p.N - col)) : 0;
   auto to_lds = [&](int i) {
     static_for<TM>([&](auto I) {
       constexpr int n = decltype(I)::value;
@@ -399,7 +407,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
             for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], p.alpha, bias8[e]);
             if (has_pre) {
               plain.p = pz;
-              store8<OT>(plain, 0, 8, v);
+              if (mine) store8<OT>(plain, 0, 8, v);
               pz += sz;
             }
             if (p.act != ACT_NONE) act8<false>(v, p.act);
@@ -413,10 +421,10 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
             }
             if (has_out) {
               plain.p = po;
-              store8<OT>(plain, 0, 8, v);
+              if (mine) store8<OT>(plain, 0, 8, v);
               po += so;
             }
-            if (turned) {
+            if (turned && mine) {
               *reinterpret_cast<f32x4*>(&T[(s * RP + cr) * LP + cc]) = f32x4{v[0], v[1], v[2], v[3]};
               *reinterpret_cast<f32x4*>(&T[(s * RP + cr) * LP + cc + 4]) = f32x4{v[4], v[5], v[6], v[7]};
             }
@@ -455,7 +463,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
           const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
           if (rin && n > 0) store8<OT>(p.out, batch * p.out.batch + row * p.out.ld + col, n, v);
         }
-        if (turned) {
+        if (turned && mine) {
           *reinterpret_cast<f32x4*>(&T[lr * LP + cc]) = f32x4{v[0], v[1], v[2], v[3]};
           *reinterpret_cast<f32x4*>(&T[lr * LP + cc + 4]) = f32x4{v[4], v[5], v[6], v[7]};
         }
@@ -532,32 +540,38 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
 
 namespace {
 
-struct Tile { int bm, bn; };
-// what a workgroup's tile costs per 64 columns of the contraction, in units of 1e-9 s at full occupancy (measured, see product())
 struct Plan { int tile, ksplit, kchunk, tm, tn; int64_t tiles; };
 
 // a lane's place below its tile's base has 32 bits: 64 rows of 2^25 elements, 256 of 2^23
 constexpr int64_t MAX_LD = (int64_t)1 << 25, MAX_LD_BIG = (int64_t)1 << 22;
 
+struct TileKind {
+  int bm;            // the tile is bm x bm
+  int per_cu;        // workgroups a CU holds (LDS)
+  double stage1_us;  // one stage of a workgroup alone on its CU
+  double stage_us;   // one stage of each of per_cu workgroups of a full CU (the whole chip busy: lower clocks)
+  double fixed_us;   // launch, first stages, epilogue
+};
+// measured at 16 and 64 stages on 64 to 1024 tiles
+constexpr int NTILES = 5;
+const TileKind TILES[NTILES] = {{256, 1, 1.0, 1.48, 15.0}, {192, 1, 0.80, 0.90, 11.0}, {128, 2, 0.73, 1.05, 4.0}, {128, 1, 0.53, 0.55, 6.0}, {64, 2, 0.29, 0.41, 3.5}};
+
+// The tile and the slices of the contraction with the least time by the figures above: rounds of the chip's 256 CUs, the stages of a
+// workgroup, and for slices the slabs written, read and joined by a second launch.
 Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric, bool may_split) {
-  static const int BM[3] = {256, 128, 64};
   const int64_t nst = std::max<int64_t>(1, (type == D_PL3 ? 6 : 1) * ((K + 63) / 64));
   Plan best{};
   double best_t = 1e300;
-  for (int t = K > MAX_LD_BIG ? 2 : 0; t < 3; ++t) {
-    const int64_t tm = (M + BM[t] - 1) / BM[t], tn = (N + BM[t] - 1) / BM[t];
+  for (int t = K > MAX_LD_BIG ? NTILES - 1 : 0; t < NTILES; ++t) {
+    const TileKind& k = TILES[t];
+    const int64_t tm = (M + k.bm - 1) / k.bm, tn = (N + k.bm - 1) / k.bm;
     const int64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
-    // time of one stage of one workgroup when its CU is full, and workgroups a CU holds at once
-    static const double stage_us[3] = {1.3, 0.45, 0.18};
-    static const int res[3] = {1, 2, 4};
     for (int ks = 1; ks <= 32; ks *= 2) {
       if (ks > 1 && (!may_split || nst / ks < 4)) break;
-      const int64_t kc = (nst + ks - 1) / ks, wg = tiles * ks, slots = 256 * res[t];
-      const int64_t rounds = (wg + slots - 1) / slots;
-      // an unfull last round: a CU with fewer workgroups than it can hold runs each of them faster
-      const int64_t in_last = wg - (rounds - 1) * slots, per_cu = (in_last + 255) / 256;
-      double us = ((rounds - 1) * res[t] + per_cu) * (stage_us[t] * kc) + 3.0;
-      if (ks > 1) us += 4.0 + (double)ks * M * N * batch * 8.0 / 4e6;
+      const int64_t kc = (nst + ks - 1) / ks, wg = tiles * ks, slots = 256 * k.per_cu, full = wg / slots, rest = wg - full * slots;
+      double us = full * (k.stage_us * kc + k.fixed_us);
+      if (rest > 0) us += (rest <= 256 ? k.stage1_us : k.stage_us) * kc + k.fixed_us;
+      if (ks > 1) us += 3.0 + 0.4 * ks + (double)ks * M * N * batch * (symmetric ? 4.0 : 8.0) / 4e6;
       if (us < best_t) {
         best_t = us;
         best.tile = t;
@@ -573,21 +587,25 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
   return best;
 }
 
-template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN>
+template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN, int S>
 int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
-  // two stages; the epilogue's blocks of fp32 and two blocks of a 16-bit residual per wave
-  constexpr int LDS = std::max(2 * (WM * TM + WN * TN) * 32 * 128, WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * 32 * TN * 2));
-  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, WM, WN, TM, TN>);
+  // the stages; the epilogue's blocks of fp32 and two blocks of a 16-bit residual per wave
+  constexpr int LDS = std::max(S * (WM * TM + WN * TN) * 32 * 128, WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * 32 * TN * 2));
+  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, WM, WN, TM, TN, S>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
-  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, WM, WN, TM, TN>), grid, dim3(WM * WN * 64), LDS, st, g);
+  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, WM, WN, TM, TN, S>), grid, dim3(WM * WN * 64), LDS, st, g);
   SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
 template <int MT, int OT, int RT, bool PART>
 int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile) {
-  if (tile == 0) return launch<MT, OT, RT, PART, 2, 2, 4, 4>(ctx, st, g, grid);
-  if (tile == 1) return launch<MT, OT, RT, PART, 2, 2, 2, 2>(ctx, st, g, grid);
-  return launch<MT, OT, RT, PART, 2, 2, 1, 1>(ctx, st, g, grid);
+  switch (tile) {
+    case 0: return launch<MT, OT, RT, PART, 2, 2, 4, 4, 2>(ctx, st, g, grid);
+    case 1: return launch<MT, OT, RT, PART, 2, 2, 3, 3, 3>(ctx, st, g, grid);
+    case 2: return launch<MT, OT, RT, PART, 2, 2, 2, 2, 2>(ctx, st, g, grid);
+    case 3: return launch<MT, OT, RT, PART, 2, 2, 2, 2, 4>(ctx, st, g, grid);
+    default: return launch<MT, OT, RT, PART, 2, 2, 1, 1, 4>(ctx, st, g, grid);
+  }
 }
 template <int MT, int OT, int RT>
 int launch_types(Ctx* ctx, hipStream_t st, const ProdArgs& g, const Plan& pl) {

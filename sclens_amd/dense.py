@@ -32,63 +32,75 @@ POLAR_STEP = (1.875, -1.25, 0.375)
 _local = threading.local()
 
 
-def _context(device: torch.device, ctx: Optional[Context]) -> Context:
-    index = device.index if device.index is not None else torch.cuda.current_device()
+def _context(index: int, ctx: Optional[Context]) -> Context:
     if ctx is None:
-        mine = getattr(_local, "contexts", None)
-        if mine is None:
-            mine = _local.contexts = {}
-        ctx = mine.get(index)
-        if ctx is None:
-            ctx = mine[index] = Context(index)  # one host thread per context
-    elif ctx.device != index:
-        raise ValueError(f"the tensors are on device {index}, the context on device {ctx.device}")
+        try:
+            ctx = _local.contexts[index]
+        except (AttributeError, KeyError):
+            if not hasattr(_local, "contexts"):
+                _local.contexts, _local.sizes = {}, {}
+            ctx = _local.contexts[index] = Context(index)  # one host thread per context
+    else:
+        if ctx.device != index:
+            raise ValueError(f"the tensors are on device {index}, the context on device {ctx.device}")
+        if not hasattr(_local, "sizes"):
+            _local.contexts, _local.sizes = {}, {}
     if not _lib.shares_torch_runtime:
         raise RuntimeError("libsclens_hip.so was loaded before torch and runs on another HIP runtime: import torch (or sclens_amd.dense) "
                            "before the first use of sclens_amd")
     return ctx
 
 
-def _check(name: str, t, like=None, shape=None) -> torch.Tensor:
+def _first(name: str, t) -> int:
+    """checks of the tensor that sets the element type and the device; its device's index"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} has to be a torch tensor")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name}: element type {t.dtype} (bfloat16, float16 or float32 expected)")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
+    if not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}, expected a GPU")
+    return t.get_device()
+
+
+def _other(name: str, t, like: torch.Tensor, index: int, shape) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} has to be a torch tensor")
+    if t.dtype is not like.dtype or not t.is_cuda or t.get_device() != index:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name} is on {t.device}, expected a GPU")
-    return t
 
 
-def _rows(name: str, t: torch.Tensor) -> Tuple[int, int]:
-    """(rows, leading dimension) of t as a matrix of rows along its last axis"""
-    cols = t.size(-1)
-    if t.dim() == 2:
-        rows, ld = t.size(0), t.stride(0)
-    elif t.dim() == 1:
-        rows, ld = 1, cols
-    else:
-        rows, ld = t.numel() // cols if cols else 0, cols
-        if not t.is_contiguous():
-            try:
-                v = t.view(-1, cols)
-            except RuntimeError:
-                raise ValueError(f"{name}: the leading axes of strides {t.stride()} do not join into one; call .contiguous()") from None
-            rows, ld = v.size(0), v.stride(0)
-    if t.numel() == 0:
-        return rows, max(1, cols)
-    if cols > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: rows have to be contiguous (strides {t.stride()}); call .contiguous()")
-    if rows <= 1:
+def _ld(name: str, t: torch.Tensor) -> int:
+    """leading dimension of t as a matrix of rows along its last axis"""
+    shape, stride = t.shape, t.stride()
+    cols = shape[-1]
+    if len(shape) == 2:
+        ld = stride[0] if shape[0] > 1 else cols
+    elif t.numel() == 0 or len(shape) == 1 or t.is_contiguous():
         ld = cols
-    if ld < cols:
-        raise ValueError(f"{name}: rows overlap (strides {t.stride()}); call .contiguous()")
-    return rows, ld
+    else:
+        try:
+            v = t.view(-1, cols)
+        except RuntimeError:
+            raise ValueError(f"{name}: the leading axes of strides {stride} do not join into one; call .contiguous()") from None
+        ld = v.stride(0) if v.size(0) > 1 else cols
+    if (cols > 1 and stride[-1] != 1 or ld < cols) and t.numel():
+        if cols > 1 and stride[-1] != 1:
+            raise ValueError(f"{name}: rows have to be contiguous (strides {stride}); call .contiguous()")
+        raise ValueError(f"{name}: rows overlap (strides {stride}); call .contiguous()")
+    return ld if ld > 0 else 1
+
+
+def _rows(shape) -> int:
+    n = 1
+    for s in shape[:-1]:
+        n *= s
+    return n
 
 
 def _activation(name: str) -> int:
@@ -98,23 +110,27 @@ def _activation(name: str) -> int:
 
 
 def _p(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
-def _run(fn, key, ctx: Context, device: torch.device, *args):
+# the raw handle of torch's current stream of a device (the function its own compiled code uses, where there is one)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run(fn, key, ctx: Context, like: torch.Tensor, index: int, *args):
     """the call with its workspace: the size the last call of these sizes needed is tried first, then what the library asks for"""
-    sizes = getattr(_local, "sizes", None)
-    if sizes is None or len(sizes) > 4096:
-        sizes = _local.sizes = {}
+    sizes = _local.sizes
     size = sizes.get(key, 0)
     n = C.c_int64(size)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    rc = fn(ctx.h, stream, *args, _p(ws), C.byref(n))
+    stream = _raw_stream(index)
+    ws = like.new_empty(size, dtype=torch.uint8) if size else None
+    rc = fn(ctx.h, stream, *args, ws.data_ptr() if size else None, n)
     if rc == 8:  # SCLENS_ERR_WORKSPACE: nothing was launched
+        if len(sizes) > 4096:
+            sizes.clear()
         sizes[key] = size = n.value
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        rc = fn(ctx.h, stream, *args, _p(ws), C.byref(n))
+        ws = like.new_empty(size, dtype=torch.uint8)
+        rc = fn(ctx.h, stream, *args, ws.data_ptr(), n)
     if rc != 0:
         ctx.check(rc)
 
@@ -127,31 +143,29 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     `save_preact` also returns the argument of the activation, which `linear_backward` reads. activation: "none", "relu", "silu",
     "gelu" (z Phi(z)) or "gelu_tanh". One row (or a few) streams the weights once: the form for serving."""
     act = _activation(activation)
-    _check("x", x)
-    _check("weight", weight, like=x)
-    if x.dim() < 1 or weight.dim() != 2 or weight.size(1) != x.size(-1):
-        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)}: expected [..., K] and [N, K]")
+    index = _first("x", x)
+    if not isinstance(weight, torch.Tensor) or x.dim() < 1 or weight.dim() != 2 or weight.size(1) != x.size(-1):
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(getattr(weight, 'shape', ()))}: expected [..., K] and [N, K]")
+    _other("weight", weight, x, index, weight.shape)
+    shape = x.shape
     N, K = weight.shape
-    out_shape = tuple(x.shape[:-1]) + (N,)
+    out_shape = (*shape[:-1], N)
     if bias is not None:
-        _check("bias", bias, like=x, shape=(N,))
+        _other("bias", bias, x, index, (N,))
         if N > 1 and bias.stride(0) != 1:
             raise ValueError("bias has to be contiguous")
+    ldr = N
     if residual is not None:
-        _check("residual", residual, like=x, shape=out_shape)
-    M, ldx = _rows("x", x)
-    if K == 0:
-        M = 1
-        for s in out_shape[:-1]:
-            M *= s
-    _, ldw = _rows("weight", weight)
-    _, ldr = _rows("residual", residual) if residual is not None else (0, N)
-    ctx = _context(x.device, ctx)
-    y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(out_shape, dtype=x.dtype, device=x.device) if save_preact else None
+        _other("residual", residual, x, index, out_shape)
+        ldr = _ld("residual", residual)
+    M = shape[0] if len(shape) == 2 else _rows(shape)
+    ldx, ldw = _ld("x", x), _ld("weight", weight)
+    ctx = _context(index, ctx)
+    y = x.new_empty(out_shape)
+    z = x.new_empty(out_shape) if save_preact else None
     dt = DTYPES[x.dtype]
-    _run(ctx.lib.sclens_hip_linear, ("f", dt, M, N, K), ctx, x.device, dt, M, N, K, _p(x), ldx, _p(weight), ldw, _p(bias), _p(residual), ldr,
-         act, _p(y), max(1, N), _p(z), max(1, N))
+    _run(ctx.lib.sclens_hip_linear, (1, dt, M, N, K), ctx, x, index, dt, M, N, K, x.data_ptr(), ldx, weight.data_ptr(), ldw, _p(bias),
+         _p(residual), ldr, act, y.data_ptr(), N or 1, _p(z), N or 1)
     return (y, z) if save_preact else y
 
 
@@ -162,38 +176,37 @@ def linear_backward(grad: torch.Tensor, x: Optional[torch.Tensor], weight: Optio
     of the residual), preact what `linear(save_preact=True)` returned (not needed for "none"; relu'(0) = 0). x may be None if
     need_weight is false, weight if need_x is false. All leading axes are summed over in dweight and dbias, in a fixed order."""
     act = _activation(activation)
-    _check("grad", grad)
-    if grad.dim() < 1:
+    index = _first("grad", grad)
+    shape = grad.shape
+    if len(shape) < 1:
         raise ValueError("grad: expected [..., N]")
-    N = grad.size(-1)
-    lead = tuple(grad.shape[:-1])
-    M = 1
-    for s in lead:
-        M *= s
+    N = shape[-1]
+    lead = shape[:-1]
+    M = _rows(shape)
     if need_weight and x is None or need_x and weight is None:
         raise ValueError("dweight needs x, dx needs weight")
     K = x.size(-1) if x is not None else (weight.size(-1) if weight is not None else 0)
     if x is not None:
-        _check("x", x, like=grad, shape=lead + (K,))
+        _other("x", x, grad, index, (*lead, K))
     if weight is not None:
-        _check("weight", weight, like=grad, shape=(N, K))
+        _other("weight", weight, grad, index, (N, K))
+    ldz = N or 1
     if act:
         if preact is None:
             raise ValueError(f"the gradient of {activation!r} needs preact (linear(..., save_preact=True))")
-        _check("preact", preact, like=grad, shape=grad.shape)
-    _, lddy = _rows("grad", grad)
-    ldx = _rows("x", x)[1] if need_weight else max(1, K)
-    ldw = _rows("weight", weight)[1] if need_x else max(1, K)
-    ldz = _rows("preact", preact)[1] if act else max(1, N)
-    ctx = _context(grad.device, ctx)
-    new = lambda shape: torch.empty(shape, dtype=grad.dtype, device=grad.device)  # noqa: E731
-    dx = new(lead + (K,)) if need_x else None
-    dw = new((N, K)) if need_weight else None
-    db = new((N,)) if need_bias else None
+        _other("preact", preact, grad, index, shape)
+        ldz = _ld("preact", preact)
+    lddy = _ld("grad", grad)
+    ldx = _ld("x", x) if need_weight else K or 1
+    ldw = _ld("weight", weight) if need_x else K or 1
+    ctx = _context(index, ctx)
+    dx = grad.new_empty((*lead, K)) if need_x else None
+    dw = grad.new_empty((N, K)) if need_weight else None
+    db = grad.new_empty((N,)) if need_bias else None
     dt = DTYPES[grad.dtype]
-    _run(ctx.lib.sclens_hip_linear_backward, ("b", dt, M, N, K, need_x, need_weight, need_bias), ctx, grad.device, dt, M, N, K, _p(grad), lddy,
-         _p(x) if need_weight else None, ldx, _p(weight) if need_x else None, ldw, _p(preact) if act else None, ldz, act, _p(dx),
-         max(1, K), _p(dw), max(1, K), _p(db))
+    _run(ctx.lib.sclens_hip_linear_backward, (2, dt, M, N, K, need_x, need_weight, need_bias), ctx, grad, index, dt, M, N, K, grad.data_ptr(),
+         lddy, _p(x) if need_weight else None, ldx, _p(weight) if need_x else None, ldw, _p(preact) if act else None, ldz, act, _p(dx),
+         K or 1, _p(dw), K or 1, _p(db))
     return dx, dw, db
 
 
@@ -205,7 +218,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Union[Sequence[
     `coefficients`: one triple, used `steps` times, or a sequence of triples, one per step. [UPDATE_STEP] * 5 is an optimiser's update;
     [UPDATE_STEP] * 5 + [POLAR_STEP] * 3 converges to the orthogonal factor (singular values well above 1e-2 of the norm). Every matrix
     of the leading axes is worked on by itself."""
-    _check("x", x)
+    index = _first("x", x)
     if x.dim() < 2:
         raise ValueError(f"x {tuple(x.shape)}: expected [..., rows, cols]")
     coef = [float(v) for v in coefficients] if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else None
@@ -231,10 +244,10 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Union[Sequence[
     ld = v.stride(-2) if rows > 1 else cols
     if x.numel() and (cols > 1 and v.stride(-1) != 1 or ld < cols):
         raise ValueError(f"x: rows have to be contiguous and apart (strides {x.stride()}); call .contiguous()")
-    ctx = _context(x.device, ctx)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ctx = _context(index, ctx)
+    y = x.new_empty(x.shape)
     dt = DTYPES[x.dtype]
     arr = (C.c_double * len(coef))(*coef)
-    _run(ctx.lib.sclens_hip_orthogonalize, ("o", dt, batch, rows, cols, len(coef) > 3), ctx, x.device, dt, batch, rows, cols, _p(x), stride,
-         max(1, ld), _p(y), rows * cols, max(1, cols), len(coef) // 3, arr, float(eps))
+    _run(ctx.lib.sclens_hip_orthogonalize, (3, dt, batch, rows, cols, len(coef)), ctx, x, index, dt, batch, rows, cols, x.data_ptr(), stride,
+         ld or 1, y.data_ptr(), rows * cols, cols or 1, len(coef) // 3, arr, float(eps))
     return y

@@ -21,6 +21,13 @@ class _Gpu(torch.Tensor):
     def device(self):
         return torch.device("cuda", 0)
 
+    @property
+    def is_cuda(self):
+        return True
+
+    def get_device(self):
+        return 0
+
 
 def g(*shape, dtype=F32):
     return torch.zeros(*shape, dtype=dtype).as_subclass(_Gpu)
@@ -88,6 +95,6 @@ def test_library_loaded_before_torch_is_refused(monkeypatch):
         device = 0
 
     with pytest.raises(RuntimeError, match="import torch"):
-        dense._context(torch.device("cuda", 0), Ctx())
+        dense._context(0, Ctx())
     with pytest.raises(ValueError, match="context on device"):
-        dense._context(torch.device("cuda", 1), Ctx())
+        dense._context(1, Ctx())
