@@ -14,6 +14,8 @@ struct Mat {
   void* p = nullptr;
   int64_t ld = 0, batch = 0, plane = 0;
   int vec = 0;  // 16-byte loads / stores of 8 columns are aligned
+  int across = 0;  // an operand of a product whose rows run across the contraction: element (row r, column k) at k * ld + r; whole chunks
+                   // of 8 rows have to exist
   int pad = 0;  // rows / columns up to the next multiple of 8 exist and are written as zeros (images of the library)
 };
 

@@ -94,7 +94,24 @@ __device__ __forceinline__ float recompute_f32(const unsigned short* A, const un
   return s;
 }
 
-template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN, int S>
+// rows of W elements across the contraction: the 32-byte pair of chunks that column k keeps in place of pair u is u ^ pair_swz(k). The
+// columns 4 apart or less and 8 apart that one transposing read touches (k & 3, k & 8) then lie in different banks (256 bytes).
+template <int W>
+__device__ __forceinline__ int pair_swz(int k) {
+  return W % 128 == 0 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// (__restrict: the inlined call then carries the alias information without which the compiler lets every such read wait for all copies
+// to LDS that are on their way)
+__device__ __forceinline__ s16x4 read_tr(lds_s16x4* __restrict p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
+template <int ROW>
+__device__ __forceinline__ u16x8 read_across(const unsigned char* p) {
+  const s16x4 a = read_tr((lds_s16x4*)(p)), b = read_tr((lds_s16x4*)(p + 4 * ROW));
+  return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(ProdArgs g) {
   constexpr int NW = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, NP = PA + PB;  // 1 KB copies (8 rows x 64 columns) per wave and stage
@@ -124,20 +141,35 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   const int64_t m0 = (int64_t)ti * BM, n0 = (int64_t)tj * BN, batch = blockIdx.y;
 
   // ---- sources of this wave's copies: a uniform base that moves along the contraction, and each lane's place below it (the plan
-  // keeps a tile's rows below 2^32 bytes)
+  // keeps it below 2^32 bytes). A lane's 16 bytes of copy i land at byte 1024 i' + 16 lane of the operand's stage:
+  //   rows along the contraction (AC / BC false): row r, slot q of 8 chunks, columns 8 (q ^ ((r >> 1) & 7)) ..
+  //   rows across it (true): column k of the contraction, slot of BM / 8 chunks; the 32-byte pair it is in is swizzled by k (pair_swz)
   const int srow = lane >> 3, sq = lane & 7;
-  const char* baseA = static_cast<const char*>(p.A.p) + 2 * (batch * p.A.batch + m0 * p.A.ld);
-  const char* baseB = static_cast<const char*>(p.B.p) + 2 * (batch * p.B.batch + n0 * p.B.ld);
+  const char* baseA = static_cast<const char*>(p.A.p) + 2 * (batch * p.A.batch + (AC ? m0 : m0 * p.A.ld));
+  const char* baseB = static_cast<const char*>(p.B.p) + 2 * (batch * p.B.batch + (BC ? n0 : n0 * p.B.ld));
+  const int64_t stepA = AC ? 128 * p.A.ld : 128, stepB = BC ? 128 * p.B.ld : 128;  // bytes per stage
+  // ktail != 0: the last stage of the contraction, of which only ktail columns exist: the others are copied from the stage's first
+  // chunk / first column (in bounds whatever the matrix) and overwritten with zeros in LDS when they have landed
+  auto place = [&](int i, int ktail) -> unsigned {
+    const bool isA = i < PA;
+    const int grp = isA ? wid * PA + i : wid * PB + i - PA;
+    const int64_t rows = isA ? p.M - m0 : p.N - n0, ld = isA ? p.A.ld : p.B.ld;
+    if (isA ? AC : BC) {
+      const int W = isA ? BM : BN, byte = grp * 1024 + lane * 16;
+      int k = byte / (2 * W);
+      const int slot = (byte - k * 2 * W) >> 4, c = ((slot >> 1) ^ (W == 256 || W == 128 ? pair_swz<256>(k) : pair_swz<64>(k))) * 2 + (slot & 1);
+      if (ktail && k >= ktail) k = 0;
+      return (unsigned)(2 * (k * ld + (8 * c < rows ? 8 * c : 0)));  // (columns behind the end are not stored)
+    }
+    const int r = grp * 8 + srow;
+    int chunk = sq ^ ((r >> 1) & 7);
+    if (ktail && 8 * chunk >= ktail) chunk = 0;
+    const int64_t row = r < rows ? r : rows - 1;  // (products of rows behind the end are not stored)
+    return (unsigned)(2 * (row * ld + 8 * chunk));
+  };
   unsigned voff[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const bool isA = i < PA;
-    const int r = (isA ? wid * PA + i : wid * PB + i - PA) * 8 + srow;
-    const int chunk = sq ^ ((r >> 1) & 7);
-    const int64_t last = (isA ? p.M - m0 : p.N - n0) - 1;
-    const int64_t row = r < last ? r : last;  // (products of rows behind the end are not stored)
-    voff[i] = (unsigned)(2 * (row * (isA ? p.A.ld : p.B.ld) + 8 * chunk));
-  }
+  for (int i = 0; i < NP; ++i) voff[i] = place(i, 0);
 
   // ---- stages of this slice: stage t = (plane pair t / nkt, columns 64 (t % nkt) ..)
   const int ntot = (PL ? 6 : 1) * g.nkt;
@@ -147,8 +179,8 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   int ld_k = t0 - ld_seg * g.nkt;
   const char *curA = baseA, *curB = baseB;
   auto set_cur = [&]() {
-    curA = baseA + (int64_t)ld_k * 128;
-    curB = baseB + (int64_t)ld_k * 128;
+    curA = baseA + ld_k * stepA;
+    curB = baseB + ld_k * stepB;
     if (PL) {
       // (A plane, B plane), smallest products first: 20 02 11 10 01 00
       const int pa = (0x001102 >> (4 * ld_seg)) & 15, pb = (0x010120 >> (4 * ld_seg)) & 15;
@@ -156,15 +188,15 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
       curB += 2 * pb * p.B.plane;
     }
   };
-  // A contraction that is not whole stages: the chunks behind its end are copied from the row's first chunk instead (`back` bytes
-  // before: in bounds whatever the matrix) and overwritten with zeros in LDS when they have landed.
   const int ktail = (int)(p.K & 63);
-  int back0 = 0, back1 = 0;  // copies of an even / odd group of 8 rows
-  auto set_back = [&]() {
+  bool ld_tail = false;
+  auto set_tail = [&]() {
     const bool tail = ktail != 0 && ld_k + 1 == g.nkt;
-    const int c0 = sq ^ (srow >> 1), c1 = sq ^ (4 | (srow >> 1));
-    back0 = tail && 8 * c0 >= ktail ? 16 * c0 : 0;
-    back1 = tail && 8 * c1 >= ktail ? 16 * c1 : 0;
+    if (tail != ld_tail) {
+      ld_tail = tail;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) voff[i] = place(i, tail ? ktail : 0);
+    }
   };
   auto advance = [&]() {  // past the last stage the copies repeat it; nobody reads the repetition
     if (ld_t + 1 < t1) {
@@ -174,23 +206,29 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
         ++ld_seg;
       }
       set_cur();
-      set_back();
+      set_tail();
     }
   };
   auto copy = [&](int buf, int i) {
     const bool isA = i < PA;
-    const int grp = isA ? wid * PA + i : wid * PB + i - PA;
-    unsigned char* dst = lds + buf * STAGE + (isA ? 0 : OPA) + grp * 1024;
-    // (the groups of a wave start at an even one unless it has a single one per operand)
-    const int back = (isA ? PA : PB) % 2 == 0 ? (((isA ? i : i - PA) & 1) ? back1 : back0) : ((grp & 1) ? back1 : back0);
-    __builtin_amdgcn_global_load_lds((glb_cv*)((isA ? curA : curB) + (voff[i] - (unsigned)back)), (lds_v*)dst, 16, 0, 0);
+    unsigned char* dst = lds + buf * STAGE + (isA ? wid * PA + i : OPA / 1024 + wid * PB + i - PA) * 1024;
+    __builtin_amdgcn_global_load_lds((glb_cv*)((isA ? curA : curB) + voff[i]), (lds_v*)dst, 16, 0, 0);
   };
   auto zero_tail = [&](int buf) {
-    const int first = (ktail + 7) / 8, n = 8 - first;
-    for (int e = tid; e < (BM + BN) * n; e += NW * 64) {
-      const int r = e / n, c = first + e % n;  // (row BM + r of the stage is row r of B: BM is a multiple of 16)
-      *reinterpret_cast<u16x8*>(lds + buf * STAGE + r * 128 + ((c ^ ((r >> 1) & 7)) << 4)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+    auto zero = [&](unsigned char* o, auto across, auto w) {
+      constexpr int W = decltype(w)::value;
+      if constexpr (decltype(across)::value) {  // whole columns of the contraction
+        for (int e = ktail * W * 2 + tid * 16; e < 64 * W * 2; e += NW * 64 * 16) *reinterpret_cast<u16x8*>(o + e) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      } else {
+        const int first = (ktail + 7) / 8, n = 8 - first;
+        for (int e = tid; e < W * n; e += NW * 64) {
+          const int r = e / n, c = first + e % n;
+          *reinterpret_cast<u16x8*>(o + r * 128 + ((c ^ ((r >> 1) & 7)) << 4)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+      }
+    };
+    zero(lds + buf * STAGE, std::integral_constant<bool, AC>(), std::integral_constant<int, BM>());
+    zero(lds + buf * STAGE + OPA, std::integral_constant<bool, BC>(), std::integral_constant<int, BN>());
     wait_lds_barrier();
   };
 
@@ -202,15 +240,34 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  // rows 32 apart have the same swizzle: one address per operand and chunk
+  // A fragment of 32 rows x 16 columns: lane (row l31, columns 8 h .. 8 h + 7). Rows along the contraction: 16 bytes, and rows 32 apart
+  // have the same swizzle. Rows across it: two transposing reads of 4 columns each -- 16 lanes name 4 columns x 16 rows (lane i: column
+  // i >> 2, rows 4 (i & 3) ..) and lane i receives row i of all four; lanes 16 .. 31 take the other 16 rows, 32 .. 63 columns 8 .. 15.
   const int ra = (wm * TM * 32 + l31) * 128, rb = OPA + (wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
+  const int tr = (lane & 15) >> 2, tk = 8 * h + tr, th = (lane >> 4) & 1;
+  int ca[AC ? TM : 1], cb[BC ? TN : 1];
+  if constexpr (AC) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ca[i] = tk * 2 * BM + ((wm * TM * 2 + 2 * i + th) ^ pair_swz<BM>(tk)) * 32 + (lane & 3) * 8;
+  }
+  if constexpr (BC) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) cb[j] = OPA + tk * 2 * BN + ((wn * TN * 2 + 2 * j + th) ^ pair_swz<BN>(tk)) * 32 + (lane & 3) * 8;
+  }
   u16x8 av[2][TM], bv[2][TN];
+  auto fragA = [&](const unsigned char* B, int kk, int i) {
+    if constexpr (AC) return read_across<2 * BM>(B + ca[i] + kk * 16 * 2 * BM);
+    else return *reinterpret_cast<const u16x8*>(B + ra + i * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
+  };
+  auto fragB = [&](const unsigned char* B, int kk, int j) {
+    if constexpr (BC) return read_across<2 * BN>(B + cb[j] + kk * 16 * 2 * BN);
+    else return *reinterpret_cast<const u16x8*>(B + rb + j * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
+  };
   // read n of a unit's TM + TN: the operands in the order in which the matrix instructions want them
   auto read = [&](int set, const unsigned char* B, int kk, int n) {
-    const int c = ((2 * kk + h) ^ sw) << 4;
-    if (n == 0) av[set][0] = *reinterpret_cast<const u16x8*>(B + ra + c);
-    else if (n <= TN) bv[set][n - 1] = *reinterpret_cast<const u16x8*>(B + rb + (n - 1) * 32 * 128 + c);
-    else av[set][n - TN] = *reinterpret_cast<const u16x8*>(B + ra + (n - TN) * 32 * 128 + c);
+    if (n == 0) av[set][0] = fragA(B, kk, 0);
+    else if (n <= TN) bv[set][n - 1] = fragB(B, kk, n - 1);
+    else av[set][n - TN] = fragA(B, kk, n - TN);
   };
   // one matrix instruction at a time, and in its shadow what `beside` issues
   auto unit = [&](int set, auto beside) {
@@ -251,7 +308,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   if (t1 > t0) {
     int rd_k = ld_k;  // column block of the stage that is read
     set_cur();
-    set_back();
+    set_tail();
 #pragma unroll
     for (int b = 0; b < S; ++b) {
       if (b > 0) advance();
@@ -587,31 +644,31 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
   return best;
 }
 
-template <int MT, int OT, int RT, bool PART, int WM, int WN, int TM, int TN, int S>
+template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
 int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
   // the stages; the epilogue's blocks of fp32 and two blocks of a 16-bit residual per wave
   constexpr int LDS = std::max(S * (WM * TM + WN * TN) * 32 * 128, WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * 32 * TN * 2));
-  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, WM, WN, TM, TN, S>);
+  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
-  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, WM, WN, TM, TN, S>), grid, dim3(WM * WN * 64), LDS, st, g);
+  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>), grid, dim3(WM * WN * 64), LDS, st, g);
   SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
-template <int MT, int OT, int RT, bool PART>
+template <int MT, int OT, int RT, bool PART, bool AC, bool BC>
 int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile) {
   switch (tile) {
-    case 0: return launch<MT, OT, RT, PART, 2, 2, 4, 4, 2>(ctx, st, g, grid);
-    case 1: return launch<MT, OT, RT, PART, 2, 2, 3, 3, 3>(ctx, st, g, grid);
-    case 2: return launch<MT, OT, RT, PART, 2, 2, 2, 2, 2>(ctx, st, g, grid);
-    case 3: return launch<MT, OT, RT, PART, 2, 2, 2, 2, 4>(ctx, st, g, grid);
-    default: return launch<MT, OT, RT, PART, 2, 2, 1, 1, 4>(ctx, st, g, grid);
+    case 0: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 4, 4, 2>(ctx, st, g, grid);
+    case 1: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 3, 3, 3>(ctx, st, g, grid);
+    case 2: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 2>(ctx, st, g, grid);
+    case 3: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 4>(ctx, st, g, grid);
+    default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, 4>(ctx, st, g, grid);
   }
 }
-template <int MT, int OT, int RT>
+template <int MT, int OT, int RT, bool AC = false, bool BC = false>
 int launch_types(Ctx* ctx, hipStream_t st, const ProdArgs& g, const Plan& pl) {
   const dim3 grid((unsigned)pl.tiles, (unsigned)g.p.batch, (unsigned)pl.ksplit);
-  if (pl.ksplit == 1) return launch_tile<MT, OT, RT, false>(ctx, st, g, grid, pl.tile);
-  SCL_TRY((launch_tile<MT, D_F32, D_F32, true>(ctx, st, g, grid, pl.tile)));
+  if (pl.ksplit == 1) return launch_tile<MT, OT, RT, false, AC, BC>(ctx, st, g, grid, pl.tile);
+  SCL_TRY((launch_tile<MT, D_F32, D_F32, true, AC, BC>(ctx, st, g, grid, pl.tile)));
   const int64_t blocks = ((g.p.M + 31) / 32) * ((g.p.N + 63) / 64);
   hipLaunchKernelGGL((k_product_join<OT, RT, MT == D_PL3>), dim3((unsigned)blocks, (unsigned)g.p.batch), dim3(256), 0, st, g);
   SCL_HIP(ctx, hipGetLastError());
@@ -638,15 +695,23 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   g.ksplit = pl.ksplit;
   g.kchunk = pl.kchunk;
   g.nkt = (int)((p.K + 63) / 64);
+  const int form = (p.A.across ? 2 : 0) + (p.B.across ? 1 : 0);
   if (p.type == D_F16) {
-    if (p.out_type == D_F16) return launch_types<D_F16, D_F16, D_F16>(ctx, st, g, pl);
-    if (p.out_type == D_BF16) return launch_types<D_F16, D_BF16, D_F16>(ctx, st, g, pl);
-  } else if (p.type == D_BF16) {
-    if (p.out_type == D_BF16) return launch_types<D_BF16, D_BF16, D_BF16>(ctx, st, g, pl);
-  } else if (p.type == D_PL3) {
-    if (p.out_type == D_PL3) return launch_types<D_PL3, D_PL3, D_PL3>(ctx, st, g, pl);
-    if (p.out_type == D_F32 && p.res_type == D_PL3) return launch_types<D_PL3, D_F32, D_PL3>(ctx, st, g, pl);
-    if (p.out_type == D_F32) return launch_types<D_PL3, D_F32, D_F32>(ctx, st, g, pl);
+    if (p.out_type == D_F16) {
+      if (form == 0) return launch_types<D_F16, D_F16, D_F16>(ctx, st, g, pl);
+      if (form == 1) return launch_types<D_F16, D_F16, D_F16, false, true>(ctx, st, g, pl);
+      if (form == 3) return launch_types<D_F16, D_F16, D_F16, true, true>(ctx, st, g, pl);
+    }
+    if (p.out_type == D_BF16 && form == 0) return launch_types<D_F16, D_BF16, D_F16>(ctx, st, g, pl);
+    if (p.out_type == D_BF16 && form == 1) return launch_types<D_F16, D_BF16, D_F16, false, true>(ctx, st, g, pl);
+  } else if (p.type == D_BF16 && p.out_type == D_BF16) {
+    if (form == 0) return launch_types<D_BF16, D_BF16, D_BF16>(ctx, st, g, pl);
+    if (form == 1) return launch_types<D_BF16, D_BF16, D_BF16, false, true>(ctx, st, g, pl);
+    if (form == 3) return launch_types<D_BF16, D_BF16, D_BF16, true, true>(ctx, st, g, pl);
+  } else if (form == 0) {
+    if (p.type == D_PL3 && p.out_type == D_PL3) return launch_types<D_PL3, D_PL3, D_PL3>(ctx, st, g, pl);
+    if (p.type == D_PL3 && p.out_type == D_F32 && p.res_type == D_PL3) return launch_types<D_PL3, D_F32, D_PL3>(ctx, st, g, pl);
+    if (p.type == D_PL3 && p.out_type == D_F32) return launch_types<D_PL3, D_F32, D_F32>(ctx, st, g, pl);
   }
   return ctx->fail(SCLENS_ERR_ARG, "product: element types");
 }

@@ -172,15 +172,15 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   Carve c(ws);
   const int64_t nmb = (a.M + 63) / 64;
   const bool as_is = a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
+  const bool f32 = a.dtype == D_F32;
+  // 16 bits: dz, w and x feed both products as they lie (w and x with their rows across the contraction), through a padded copy if they
+  // are not on 16 bytes. fp32: three planes with the contraction contiguous, so dz both ways, w and x transposed.
   Mat dz, dzT, wT, xT;
-  if (a.dx) {
-    dz = as_is ? user_mat(a.dy, a.lddy) : image_of(c, a.dtype, a.M, a.N);
-    wT = image_of(c, a.dtype, a.K, a.N);
-  }
-  if (a.dw) {
-    dzT = image_of(c, a.dtype, a.N, a.M);
-    xT = image_of(c, a.dtype, a.K, a.M);
-  }
+  const bool w_as_is = direct(a.dtype, a.w, a.ldw, a.K), x_as_is = direct(a.dtype, a.x, a.ldx, a.K);
+  if (a.dx || (a.dw && !f32)) dz = as_is ? user_mat(a.dy, a.lddy) : image_of(c, a.dtype, a.M, a.N);
+  if (a.dx) wT = f32 ? image_of(c, a.dtype, a.K, a.N) : (w_as_is ? user_mat(a.w, a.ldw) : image_of(c, a.dtype, a.N, a.K));
+  if (a.dw && f32) dzT = image_of(c, a.dtype, a.N, a.M);
+  if (a.dw) xT = f32 ? image_of(c, a.dtype, a.K, a.M) : (x_as_is ? user_mat(a.x, a.ldx) : image_of(c, a.dtype, a.M, a.K));
   float* part = a.db ? c.take<float>(std::max<int64_t>(1, nmb * a.N)) : nullptr;
   const int type = image_type(a.dtype);
   const int64_t slab_dx = a.dx ? product_slab_bytes(a.M, a.K, a.N, 1, type, 0) : 0;
@@ -190,11 +190,11 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
 
-  if (a.M > 0 && a.N > 0 && (a.dw || a.db || (a.dx && !as_is))) {
+  if (a.M > 0 && a.N > 0 && (a.db || (a.dw && f32) || ((a.dx || a.dw) && !as_is))) {
     const int64_t blocks = nmb * ((a.N + 63) / 64);
     if (blocks > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
-    Mat img = as_is || !a.dx ? Mat() : dz;
+    Mat img = as_is ? Mat() : dz;
 #define SCL_DZ(T) hipLaunchKernelGGL(k_dz<T>, dim3((unsigned)blocks), dim3(256), 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part)
     if (a.dtype == D_F32) SCL_DZ(D_F32);
     else if (a.dtype == D_BF16) SCL_DZ(D_BF16);
@@ -215,16 +215,22 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   p.slabs = slabs;
   p.slab_bytes = slab;
   if (a.dx && a.M > 0 && a.K > 0) {
-    SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, true, a.K, a.N, &wT));
+    if (f32) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, true, a.K, a.N, &wT));
+    else if (!w_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, false, a.N, a.K, &wT));
+    wT.across = !f32;
     p.M = a.M; p.N = a.K; p.K = a.N;
     p.A = dz; p.B = wT;
     p.out = user_mat(a.dx, a.lddx);
     SCL_TRY(product(ctx, st, p));
   }
   if (a.dw && a.N > 0 && a.K > 0) {
-    SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, true, a.K, a.M, &xT));
+    if (f32) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, true, a.K, a.M, &xT));
+    else if (!x_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, false, a.M, a.K, &xT));
+    xT.across = !f32;
     p.M = a.N; p.N = a.K; p.K = a.M;
-    p.A = dzT; p.B = xT;
+    p.A = f32 ? dzT : dz;
+    p.A.across = !f32;
+    p.B = xT;
     p.out = user_mat(a.dw, a.lddw);
     SCL_TRY(product(ctx, st, p));
   }
@@ -292,6 +298,7 @@ __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64
 #pragma unroll
     for (int e = 0; e < 8; ++e) L[lr][cc + e] = v[e];
   }
+  if (!imgT.p) return;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -343,12 +350,13 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   double* part = c.take<double>(a.batch * nparts);
   Mat X[2], XT[2];
   for (int i = 0; i < (a.steps > 1 ? 2 : 1); ++i) {
-    X[i] = image_of(c, img_dtype, m, n, a.batch);
-    XT[i] = image_of(c, img_dtype, n, m, a.batch);
+    // fp32: x and its transpose, so that every product has the contraction contiguous; 16 bits: x as it lies in memory
+    X[i] = f32 ? image_of(c, img_dtype, m, n, a.batch) : image_of(c, img_dtype, a.rows, a.cols, a.batch);
+    if (f32) XT[i] = image_of(c, img_dtype, n, m, a.batch);
   }
   Mat A = image_of(c, img_dtype, m, m, a.batch), P = image_of(c, img_dtype, m, m, a.batch);
   int64_t slab = std::max(product_slab_bytes(m, m, n, (int)a.batch, IT, 1), product_slab_bytes(m, m, m, (int)a.batch, IT, 1));
-  slab = std::max(slab, product_slab_bytes(m, n, m, (int)a.batch, IT, 0));
+  slab = std::max(slab, f32 ? product_slab_bytes(m, n, m, (int)a.batch, IT, 0) : product_slab_bytes(a.rows, a.cols, m, (int)a.batch, IT, 0));
   float* slabs = slab ? c.take<float>(slab / 4) : nullptr;
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
@@ -362,8 +370,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   double s_x = f32 ? 1.0 : pow2_scale(bound);
   {
     const dim3 g1((unsigned)nparts, (unsigned)a.batch), g2((unsigned)tiles, (unsigned)a.batch), blk(256);
-    Mat& i0 = tall ? XT[0] : X[0];
-    Mat& i1 = tall ? X[0] : XT[0];
+    const Mat i0 = tall && f32 ? XT[0] : X[0], i1 = tall && f32 ? X[0] : XT[0];
 #define SCL_START(T, I)                                                                                                             \
   do {                                                                                                                              \
     hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, static_cast<const Elem<T>::type*>(a.x), a.sx, a.ldx, a.rows, a.cols, tpr, part); \
@@ -394,6 +401,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     // A = x x'
     p.K = n;
     p.A = p.B = x;
+    p.A.across = p.B.across = tall && !f32;
     p.out = A;
     p.alpha = (float)(s_a / (s_x * s_x));
     SCL_TRY(product(ctx, st, p));
@@ -404,18 +412,26 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     p.alpha = (float)(cc * s_p / (s_a * s_a));
     p.beta = (float)(cb * s_p / s_a);
     SCL_TRY(product(ctx, st, p));
-    // x <- a x + P x
+    // x <- a x + P x (16 bits, tall: the transpose of it, a x + x P, in the layout of the caller)
     p.symmetric = 0;
-    p.N = n;
-    p.A = P;
-    p.B = xt;
     p.res = x;
     p.alpha = (float)(s_n / (s_p * s_x));
     p.beta = (float)(ca * s_n / s_x);
+    if (f32) {
+      p.N = n;
+      p.A = P;
+      p.B = xt;
+    } else {
+      p.M = a.rows;
+      p.N = a.cols;
+      p.A = tall ? x : P;
+      p.B = tall ? P : x;
+      p.B.across = !tall;
+    }
     if (last) {
       p.out_type = a.dtype;
-      p.out = tall ? Mat() : dst;
-      p.outT = tall ? dst : Mat();
+      p.out = f32 && tall ? Mat() : dst;
+      p.outT = f32 && tall ? dst : Mat();
     } else {
       p.out = X[(t + 1) & 1];
       p.outT = XT[(t + 1) & 1];
