@@ -41,24 +41,26 @@ int image_type(int dtype) { return dtype == D_F32 ? D_PL3 : dtype; }
 }  // namespace
 
 // ------------------------------------------------------------------ linear
-// One short side: at most 16 rows of x stream w past them in one launch; up to 128 rows of x (or of w) stream the longer operand and
-// join the slices of the contraction. Short contractions or few long rows are left to the tiles, which then have as little to read.
-static bool streams(int64_t S, int64_t R, int64_t K) { return S <= STREAM_SHORT && R >= 4 * S && R >= 256 && K >= 256; }
+// One short side: at most 16 rows of x go past w in one launch. Where the tiles would need a packed copy of the longer operand (fp32, or
+// rows that do not start on 16 bytes) up to 128 rows of the other stream it as it lies and join the slices of the contraction. Short
+// contractions or few long rows are left to the tiles, which then have as little to read.
+static bool streams(int dtype, const void* big, int64_t ldb, int64_t S, int64_t R, int64_t K) {
+  return !direct(dtype, big, ldb, K) && S <= STREAM_SHORT && R >= 4 * S && R >= 256 && K >= 256;
+}
 
 static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big_x, void* ws, int64_t ws_bytes, int64_t* need) {
   Carve c(ws);
   const int64_t R = big_x ? a.M : a.N, S = big_x ? a.N : a.M;
   const void *big = big_x ? a.x : a.w, *small = big_x ? a.w : a.x;
   const int64_t ldb = big_x ? a.ldx : a.ldw, lds = big_x ? a.ldw : a.ldx;
-  const bool as_is = direct(a.dtype, small, lds, a.K);
-  Mat img = as_is ? user_mat(small, lds) : image_of(c, a.dtype, S, a.K);
+  Mat img = image_of(c, a.dtype, S, a.K);
   int kchunk;
-  const int slices = stream_slices(R, a.K, &kchunk);
+  const int slices = stream_slices(R, S, a.K, &kchunk);
   const int64_t n8 = round_up8(a.N);
   float* slabs = c.take<float>(slices * a.M * n8);
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
-  if (!as_is) SCL_TRY(pack_image(ctx, st, a.dtype, small, lds, false, S, a.K, &img));
+  SCL_TRY(pack_image(ctx, st, a.dtype, small, lds, false, S, a.K, &img));
   SCL_TRY(stream_product(ctx, st, a.dtype, big, ldb, R, img, S, a.K, slabs, a.M * n8, big_x ? n8 : 1, big_x ? 1 : n8));
   Product p;
   p.M = a.M; p.N = a.N; p.K = a.K;
@@ -75,8 +77,8 @@ static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big
 int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
   if (a.M > 0 && a.N > 0 && a.K > 0) {
     if (a.M <= 16) return linear_rows(ctx, st, a);
-    if (streams(a.M, a.N, a.K)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
-    if (streams(a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
+    if (streams(a.dtype, a.w, a.ldw, a.M, a.N, a.K)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
+    if (streams(a.dtype, a.x, a.ldx, a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
   Carve c(ws);
   const bool dx = direct(a.dtype, a.x, a.ldx, a.K), dw = direct(a.dtype, a.w, a.ldw, a.K);

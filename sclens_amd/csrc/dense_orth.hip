@@ -28,6 +28,8 @@ struct Coefs { double v[3 * MAX_RIDE]; };
 
 template <int MT> struct Tiles {
   static constexpr int R = 16 * MT, LQ = R + 2, LI = R + 1, NL = MT * (MT + 1) / 2;
+  // doubles of LDS for A, P, Q, which hold the waves' partial sums of A first
+  static constexpr int WORK = 3 * R * LQ > 4 * NL * 256 ? 3 * R * LQ : 4 * NL * 256;
 };
 // the t-th tile on or below the diagonal, by rows
 __device__ __forceinline__ void lower_tile(int t, int* i, int* j) {
@@ -63,54 +65,72 @@ struct Slab {
   }
 };
 
-// red[tile][g * 64 + lane] = sum over k0 <= k < kend of x x' (unscaled); every wave takes 16 of the columns in Xs
+// red[tile][g * 64 + lane] = sum over k0 <= k < kend of x x' (unscaled); every wave takes 16 of the columns in Xs. Loads run three slabs
+// ahead. part: 4 * NL * 256 doubles of LDS (the waves' sums, waves 4 .. 7 added to 0 .. 3 first, then those in order).
 template <int T, int MT, int NW>
-__device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, double* red) {
+__device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, double* part, double* red) {
   constexpr int LI = Tiles<MT>::LI, NL = Tiles<MT>::NL, CK = 16 * NW;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
   f64x4 acc[NL];
 #pragma unroll
   for (int t = 0; t < NL; ++t) acc[t] = f64x4{0, 0, 0, 0};
-  Slab<T, MT, NW> s;
-  s.fetch(a, b, k0, kend);
-  for (int64_t k = k0; k < kend; k += CK) {
-    s.put(Xs, a.tall);
-    __syncthreads();
-    if (k + CK < kend) s.fetch(a, b, k + CK, kend);
+  Slab<T, MT, NW> s[3];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      double f[MT];
+  for (int u = 0; u < 3; ++u)
+    if (k0 + u * CK < kend) s[u].fetch(a, b, k0 + u * CK, kend);
+  for (int64_t k = k0; k < kend; k += 3 * CK) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) f[i] = (double)Xs[(wid * 16 + ks * 4 + q) * LI + i * 16 + r16];
+    for (int u = 0; u < 3; ++u) {
+      const int64_t ku = k + u * CK;
+      if (ku < kend) {
+        s[u].put(Xs, a.tall);
+        __syncthreads();
+        if (ku + 3 * CK < kend) s[u].fetch(a, b, ku + 3 * CK, kend);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+        for (int ks = 0; ks < 4; ++ks) {
+          double f[MT];
 #pragma unroll
-        for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(f[i], f[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+          for (int i = 0; i < MT; ++i) f[i] = (double)Xs[(wid * 16 + ks * 4 + q) * LI + i * 16 + r16];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(f[i], f[j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+        }
+        __syncthreads();
+      }
     }
-    __syncthreads();
   }
-  for (int w = 0; w < NW; ++w) {  // the waves' sums one after the other: a fixed order
-    if (wid == w) {
+  auto slot = [&](int t, int g) -> double& { return part[((wid & 3) * NL + t) * 256 + g * 64 + lane]; };
+#pragma unroll
+  for (int r = NW / 4 - 1; r >= 0; --r) {
+    if (wid / 4 == r) {
 #pragma unroll
       for (int t = 0; t < NL; ++t)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          double* r = red + t * 256 + g * 64 + lane;
-          *r = w == 0 ? acc[t][g] : *r + acc[t][g];
-        }
+        for (int g = 0; g < 4; ++g) slot(t, g) = r == NW / 4 - 1 ? acc[t][g] : acc[t][g] + slot(t, g);
     }
     __syncthreads();
   }
+  for (int e = threadIdx.x; e < NL * 256; e += 64 * NW)
+    red[e] = (part[e] + part[NL * 256 + e]) + (part[2 * NL * 256 + e] + part[3 * NL * 256 + e]);
+  __syncthreads();
 }
 
-// C tile (i, j) = X Y for symmetric X, Y in LDS
+// C tile (i, j) = X Y for symmetric X, Y in LDS (zeros behind m: whole tiles of the contraction, all reads in flight at once)
 template <int MT>
-__device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, int i, int j, int ksteps) {
-  constexpr int LQ = Tiles<MT>::LQ;
+__device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, int i, int j) {
+  constexpr int LQ = Tiles<MT>::LQ, KS = 4 * MT;
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
-  f64x4 acc = {0, 0, 0, 0};
   const double *x = X + (i * 16 + r16) * LQ + q, *y = Y + (j * 16 + r16) * LQ + q;
-  for (int s = 0; s < ksteps; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s], y[4 * s], acc, 0, 0, 0);
+  double xv[KS], yv[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    xv[s] = x[4 * s];
+    yv[s] = y[4 * s];
+  }
+  f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc, 0, 0, 0);
   return acc;
 }
 template <int MT>
@@ -130,7 +150,6 @@ template <int MT>
 __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const double* red, double* A, double* P, double* Q, double* scal) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, NL = Tiles<MT>::NL, NT = (NL + 7) / 8;
   const int tid = threadIdx.x, wid = tid >> 6, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
-  const int ksteps = (a.m + 3) / 4;
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     const int t = wid + 8 * u;
@@ -166,7 +185,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        f64x4 v = tile_product<MT>(A, A, i, j, ksteps);
+        f64x4 v = tile_product<MT>(A, A, i, j);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int r = i * 16 + q + 4 * g, c = j * 16 + r16;
@@ -183,8 +202,8 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        vq[u] = tile_product<MT>(P, Q, i, j, ksteps);
-        if (!last) va[u] = tile_product<MT>(A, P, i, j, ksteps);
+        vq[u] = tile_product<MT>(P, Q, i, j);
+        if (!last) va[u] = tile_product<MT>(A, P, i, j);
       }
     }
     __syncthreads();
@@ -206,7 +225,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        va[u] = tile_product<MT>(A, P, i, j, ksteps);
+        va[u] = tile_product<MT>(A, P, i, j);
       }
     }
     __syncthreads();
@@ -228,7 +247,7 @@ template <int T, int MT, int NW>
 __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, const double* Q) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, CK = 16 * NW;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-  const int ksteps = (a.m + 3) / 4;
+  constexpr int KS = 4 * MT;
   auto* y = static_cast<typename Elem<T>::type*>(a.o.y) + b * a.o.sy;
   Slab<T, MT, NW> s;
   s.fetch(a, b, k0, kend);
@@ -240,7 +259,8 @@ __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f64x4{0, 0, 0, 0};
     float* mine = Xs + (wid * 16 + r16) * LI;
-    for (int st = 0; st < ksteps; ++st) {
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
       const double x = (double)mine[st * 4 + q];
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64(Q[(i * 16 + r16) * LQ + st * 4 + q], x, acc[i], 0, 0, 0);
@@ -266,34 +286,38 @@ __global__ __launch_bounds__(512) void k_orth_small(SmallArgs a, Coefs cf) {
   constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   double* A = reinterpret_cast<double*>(lds);
-  double *P = A + R * LQ, *Q = P + R * LQ, *scal = Q + R * LQ;
-  float* Xs = reinterpret_cast<float*>(scal + 2);
+  double *P = A + R * LQ, *Q = P + R * LQ, *scal = A + Tiles<MT>::WORK, *red = scal + 2;
+  float* Xs = reinterpret_cast<float*>(red + Tiles<MT>::NL * 256);
   const int64_t b = blockIdx.x;
-  gram_range<T, MT, 8>(a, b, 0, a.n, Xs, P);
-  steps<MT>(a, cf, P, A, P, Q, scal);
+  gram_range<T, MT, 8>(a, b, 0, a.n, Xs, A, red);
+  steps<MT>(a, cf, red, A, P, Q, scal);
   apply_range<T, MT, 8>(a, b, 0, a.n, Xs, Q);
 }
 template <int T, int MT>
 __global__ __launch_bounds__(256) void k_orth_gram(SmallArgs a) {
   constexpr int NL = Tiles<MT>::NL, LI = Tiles<MT>::LI;
   __shared__ float Xs[64 * LI];
-  __shared__ double red[NL * 256];
+  __shared__ double part[4 * NL * 256];
   const int64_t b = blockIdx.y, chunks = (a.n + 63) / 64, per = (chunks + a.slices - 1) / a.slices;
   const int64_t k0 = (int64_t)blockIdx.x * per * 64, kend = min(a.n, k0 + per * 64);
-  gram_range<T, MT, 4>(a, b, k0, max(k0, kend), Xs, red);
-  double* out = a.part + (b * a.slices + blockIdx.x) * (NL * 256);
-  for (int e = threadIdx.x; e < NL * 256; e += 256) out[e] = red[e];
+  gram_range<T, MT, 4>(a, b, k0, max(k0, kend), Xs, part, a.part + (b * a.slices + blockIdx.x) * (NL * 256));
 }
-__global__ __launch_bounds__(256) void k_orth_gram_sum(const double* __restrict__ part, int slices, int elems, double* __restrict__ out) {
-  __shared__ double S[4][64];
-  const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+// 32 sums per workgroup, 32 threads to each
+__global__ __launch_bounds__(1024) void k_orth_gram_sum(const double* __restrict__ part, int slices, int elems, double* __restrict__ out) {
+  __shared__ double S[32][33];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t b = blockIdx.y;
-  const int e = blockIdx.x * 64 + c;
+  const int e = blockIdx.x * 32 + c;
   double s = 0.0;
-  for (int i = g; i < slices; i += 4) s += part[(b * slices + i) * elems + e];
+#pragma unroll 4
+  for (int i = g; i < slices; i += 32) s += part[(b * slices + i) * elems + e];
   S[g][c] = s;
   __syncthreads();
-  if (g == 0) out[b * elems + e] = (S[0][c] + S[1][c]) + (S[2][c] + S[3][c]);
+  for (int w = 16; w > 0; w >>= 1) {
+    if (g < w) S[g][c] += S[g + w][c];
+    __syncthreads();
+  }
+  if (g == 0) out[b * elems + e] = S[0][c];
 }
 template <int MT>
 __global__ __launch_bounds__(512) void k_orth_steps(SmallArgs a, Coefs cf) {
@@ -320,7 +344,7 @@ namespace {
 template <int T, int MT>
 int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, NL = Tiles<MT>::NL;
-  constexpr int LDS_STEPS = (3 * R * LQ + 2) * 8, LDS_ALL = LDS_STEPS + 128 * LI * 4;
+  constexpr int LDS_STEPS = (3 * R * LQ + 2) * 8, LDS_ALL = (Tiles<MT>::WORK + 2 + NL * 256) * 8 + 128 * LI * 4;
   const unsigned batch = (unsigned)a.o.batch;
   if (a.slices == 1) {
     if (LDS_ALL > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_small<T, MT>), LDS_ALL));
@@ -328,9 +352,9 @@ int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   } else {
     if (LDS_STEPS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_steps<MT>), LDS_STEPS));
     hipLaunchKernelGGL((k_orth_gram<T, MT>), dim3((unsigned)a.slices, batch), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_orth_gram_sum, dim3(NL * 4, batch), dim3(256), 0, st, a.part, a.slices, NL * 256, a.gram);
+    hipLaunchKernelGGL(k_orth_gram_sum, dim3(NL * 8, batch), dim3(1024), 0, st, a.part, a.slices, NL * 256, a.gram);
     hipLaunchKernelGGL((k_orth_steps<MT>), dim3(batch), dim3(512), LDS_STEPS, st, a, cf);
-    const int64_t chunks = (a.n + 63) / 64, per = std::max<int64_t>(1, chunks * batch / 2048);
+    const int64_t chunks = (a.n + 63) / 64, per = std::max<int64_t>(1, chunks * batch / 768);
     hipLaunchKernelGGL((k_orth_apply<T, MT>), dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
   }
   SCL_HIP(ctx, hipGetLastError());

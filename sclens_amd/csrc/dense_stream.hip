@@ -1,6 +1,6 @@
-// Products with one short side: a matrix of many rows is streamed once against at most 16 (k_rows) or 128 (k_stream) rows. Both are
-// bound by reading the long operand; the matrix cores (16 x 16 x 32 tiles, long operand as the rows of the tile) have room to spare:
-// at 128 short rows the fp32 form (six products per term) still keeps up with 6 TB/s.
+// Products with one short side: the long operand is streamed once past at most 16 rows (k_rows, any type) or, in fp32 or from rows
+// that do not start on 16 bytes, at most 128 rows (k_stream). Both are bound by reading the long operand; the matrix cores (16 x 16 x 32 tiles, the long operand as the rows of the tile)
+// have room to spare: at 128 short rows the fp32 form (six products per term) still keeps up with 6 TB/s.
 #include <algorithm>
 
 #include "dense_dev.h"
@@ -9,7 +9,6 @@ namespace scl {
 
 typedef __attribute__((address_space(1))) const void glb_cv;
 typedef __attribute__((address_space(3))) void lds_v;
-__device__ __attribute__((aligned(16))) unsigned short g_zero_chunk_s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 
 // eight elements k .. k+7 of a row that ends at K, at any element address
 template <int T> struct Chunk;
@@ -45,6 +44,29 @@ template <int T>
 __device__ __forceinline__ f32x4 mfma16(u16x8 a, u16x8 b, f32x4 c) {
   if constexpr (T == D_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Eight fp32 values as three bf16 pieces each, without a look at infinities: those (and what would round up to one) leave NaN in the
+// second piece, and a result that comes out NaN is formed again in fp32.
+__device__ __forceinline__ void split8(const float v[8], u16x8 out[3]) {
+  unsigned d[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      const bf16x2 h = {(__bf16)a, (__bf16)b};
+      const unsigned w = __builtin_bit_cast(unsigned, h);
+      d[p][i] = w;
+      if (p < 2) {
+        a -= __uint_as_float(w << 16);
+        b -= __uint_as_float(w & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p) __builtin_memcpy(&out[p], d[p], 16);
 }
 
 // ---- at most 16 rows of x: 16 rows of w per workgroup, the contraction dealt out to its 8 waves in runs of 128 columns
@@ -104,9 +126,11 @@ int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
   return SCLENS_OK;
 }
 
-// ---- at most 128 short rows (an image, three planes for fp32): 256 long rows per workgroup, 32 per wave, the contraction cut into
+// ---- at most 128 short rows (an image: three bf16 planes for fp32): 256 long rows per workgroup, 32 per wave, the contraction cut into
 // grid.y slices of whole 64-column stages. The short operand's stage sits in LDS (two stages in turn, chunk q of row r in slot
-// q ^ ((r >> 1) & 7)), the long one goes from memory to registers a stage ahead, fp32 is taken apart there.
+// q ^ ((r >> 1) & 7)); the long one goes from memory to registers two stages ahead and, in fp32, is taken apart
+// there. A packed copy of it, which the tiled product would read, costs three times the traffic: fp32 20 000 x 10 000 onto 40 took 949 us
+// that way, bf16 20 001 x 10 001 (rows on 2 bytes) 281 us.
 struct StreamArgs {
   const void* big;
   int64_t ldb, R, K;
@@ -119,11 +143,12 @@ struct StreamArgs {
 };
 template <int T, int NT>
 __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
+  typedef typename Elem<T>::type E;
   constexpr int NP = T == D_F32 ? 3 : 1, ROWS = NT * 16;
   constexpr int PLANE = ROWS * 128, STAGE = NP * PLANE, PIECES = STAGE / 1024;
+  constexpr int LOADS = T == D_F32 ? 8 : 4;  // 16-byte loads of a stage's fetch, at least
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  typedef typename Elem<T>::type E;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.x * 256 + wid * 32;
   const E* rows[2];
 #pragma unroll
@@ -133,76 +158,77 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
   auto copy = [&](int buf, int t) {
     for (int p = wid; p < PIECES; p += 8) {  // 1 KB: 8 rows x 64 columns of a plane
       const int plane = p / (ROWS / 8), r = (p % (ROWS / 8)) * 8 + (lane >> 3);
-      const int c = (lane & 7) ^ ((r >> 1) & 7);
+      const int c = (lane & 7) ^ ((r >> 1) & 7);  // (an image's rows are whole stages)
       const unsigned short* s = static_cast<const unsigned short*>(a.small.p) + plane * a.small.plane +
                                 min((int64_t)r, a.S - 1) * a.small.ld + (int64_t)t * 64 + 8 * c;
-      if ((int64_t)t * 64 + 8 * c >= a.K) s = g_zero_chunk_s;
       __builtin_amdgcn_global_load_lds((glb_cv*)s, (lds_v*)(lds + buf * STAGE + p * 1024), 16, 0, 0);
     }
   };
-  Chunk<T> nx[2][2], cu[2][2];
-  auto fetch = [&](int t) {
+  Chunk<T> n1[2][2], n2[2][2];
+  auto fetch = [&](Chunk<T>(&n)[2][2], int t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) nx[i][kk].load(rows[i], (int64_t)t * 64 + kk * 32 + q * 8, a.K);
+      for (int kk = 0; kk < 2; ++kk) n[i][kk].load(rows[i], (int64_t)t * 64 + kk * 32 + q * 8, a.K);
   };
   f32x4 acc[2][NT];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (t0 < t1) {
-    copy(0, t0);
-    fetch(t0);
-  }
-  for (int t = t0; t < t1; ++t) {
+  auto stage = [&](Chunk<T>(&n)[2][2], int t) {
     const int cur = (t - t0) & 1;
-    __syncthreads();  // this stage has landed; everyone is done with the other buffer
+    // this stage has landed on all sides; only the fetch of the stage after it may still be on its way
+    if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    u16x8 A[2][2][NP];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) cu[i][kk] = nx[i][kk];
-    if (t + 1 < t1) {
-      copy(cur ^ 1, t + 1);
-      fetch(t + 1);
-    }
+      for (int kk = 0; kk < 2; ++kk) {
+        if constexpr (T == D_F32) split8(n[i][kk].v, A[i][kk]);
+        else A[i][kk][0] = n[i][kk].v;
+      }
+    if (t + 1 < t1) copy(cur ^ 1, t + 1);
+    if (t + 2 < t1) fetch(n, t + 2);
     const unsigned char* B = lds + cur * STAGE;
+    // up to four column tiles together, so that six products of one accumulator are not issued one after the other
+    constexpr int G = NT <= 4 ? NT : NT / 2;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      u16x8 A[2][NP];
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (T == D_F32) {
+      for (int j0 = 0; j0 < NT; j0 += G) {
+        u16x8 b[G][NP];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            unsigned short x, y, z;
-            split3(cu[i][kk].v[e], x, y, z);
-            A[i][0][e] = x; A[i][1][e] = y; A[i][2][e] = z;
-          }
-        } else
-          A[i][0] = cu[i][kk].v;
-      }
+        for (int j = 0; j < G; ++j) {
+          const int r = (j0 + j) * 16 + r16, c = 4 * kk + q;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int r = j * 16 + r16, c = 4 * kk + q;
-        u16x8 b[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) b[p] = *reinterpret_cast<const u16x8*>(B + p * PLANE + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (T == D_F32) {
-            acc[i][j] = mfma16<D_BF16>(A[i][2], b[0], acc[i][j]);
-            acc[i][j] = mfma16<D_BF16>(A[i][0], b[2], acc[i][j]);
-            acc[i][j] = mfma16<D_BF16>(A[i][1], b[1], acc[i][j]);
-            acc[i][j] = mfma16<D_BF16>(A[i][1], b[0], acc[i][j]);
-            acc[i][j] = mfma16<D_BF16>(A[i][0], b[1], acc[i][j]);
-            acc[i][j] = mfma16<D_BF16>(A[i][0], b[0], acc[i][j]);
-          } else
-            acc[i][j] = mfma16<T>(A[i][0], b[0], acc[i][j]);
+          for (int p = 0; p < NP; ++p) b[j][p] = *reinterpret_cast<const u16x8*>(B + p * PLANE + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
         }
+        auto term = [&](int pa, int pb) {
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[i][j0 + j] = mfma16<T>(A[i][kk][pa], b[j][pb], acc[i][j0 + j]);
+        };
+        if constexpr (T == D_F32) {
+          term(2, 0);
+          term(0, 2);
+          term(1, 1);
+          term(1, 0);
+          term(0, 1);
+        }
+        term(0, 0);
       }
-    }
+  };
+  if (t0 < t1) {
+    copy(0, t0);
+    fetch(n1, t0);
+    if (t0 + 1 < t1) fetch(n2, t0 + 1);
+  }
+  for (int t = t0; t < t1; t += 2) {
+    stage(n1, t);
+    if (t + 1 < t1) stage(n2, t + 1);
   }
   float* out = a.slabs + (int64_t)blockIdx.y * a.slab;
 #pragma unroll
@@ -216,15 +242,13 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
         const int64_t r = row0 + i * 16 + 4 * q + e;
         if (r >= a.R) continue;
         float v = acc[i][j][e];
-        if constexpr (T == D_F32) {
-          if (v != v) {  // an infinity that met a zero piece: this slice's terms again in fp32
-            const E* x = static_cast<const E*>(a.big) + r * a.ldb;
-            const unsigned short* y = static_cast<const unsigned short*>(a.small.p) + s * a.small.ld;
-            v = 0.f;
-            const int64_t k1 = min(a.K, (int64_t)t1 * 64);
-            for (int64_t k = (int64_t)t0 * 64; k < k1; ++k)
-              v = fmaf(x[k], (bf16_to_f32(y[k]) + bf16_to_f32(y[k + a.small.plane])) + bf16_to_f32(y[k + 2 * a.small.plane]), v);
-          }
+        if (T == D_F32 && v != v) {  // an infinity that met a zero piece, or was taken apart: this slice's terms again in fp32
+          const float* x = static_cast<const float*>(a.big) + r * a.ldb;
+          const unsigned short* y = static_cast<const unsigned short*>(a.small.p) + s * a.small.ld;
+          v = 0.f;
+          const int64_t k1 = min(a.K, (int64_t)t1 * 64);
+          for (int64_t k = (int64_t)t0 * 64; k < k1; ++k)
+            v = fmaf(x[k], (bf16_to_f32(y[k]) + bf16_to_f32(y[k + a.small.plane])) + bf16_to_f32(y[k + 2 * a.small.plane]), v);
         }
         out[r * a.sr + s * a.ss] = v;
       }
@@ -246,17 +270,27 @@ int launch_stream_t(Ctx* ctx, hipStream_t st, const StreamArgs& a, int slices) {
   if (a.S <= 32) return launch_stream<T, 2>(ctx, st, a, slices);
   if (a.S <= 48) return launch_stream<T, 3>(ctx, st, a, slices);
   if (a.S <= 64) return launch_stream<T, 4>(ctx, st, a, slices);
+  if (a.S <= 96) return launch_stream<T, 6>(ctx, st, a, slices);
   return launch_stream<T, 8>(ctx, st, a, slices);
 }
 }  // namespace
 
-int stream_slices(int64_t R, int64_t K, int* kchunk) {
+// The slices with the least time: rounds of the 256 CUs (one workgroup each), 2 us per stage and 6 per workgroup, the slabs written and
+// read at 4 TB/s, their join.
+int stream_slices(int64_t R, int64_t S, int64_t K, int* kchunk) {
   const int64_t nst = (K + 63) / 64, groups = (R + 255) / 256;
-  // about four workgroups of 8 waves per CU, at least four stages each
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(nst / 4, (1024 + groups - 1) / groups));
-  const int64_t kc = (nst + want - 1) / want;
-  *kchunk = (int)kc;
-  return (int)((nst + kc - 1) / kc);
+  double best = 1e300;
+  int slices = 1;
+  for (int64_t s = 1; s <= std::min<int64_t>(nst, 64); ++s) {
+    const int64_t kc = (nst + s - 1) / s, n = (nst + kc - 1) / kc;
+    const double us = (double)((groups * n + 255) / 256) * (kc * 2.0 + 6.0) + n * (0.4 + (double)R * S * 8.0 / 4e6);
+    if (us < best) {
+      best = us;
+      slices = (int)n;
+      *kchunk = (int)kc;
+    }
+  }
+  return slices;
 }
 
 int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t ldb, int64_t R, const Mat& small, int64_t S, int64_t K,
@@ -265,7 +299,7 @@ int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t
   a.big = big; a.ldb = ldb; a.R = R; a.K = K;
   a.small = small; a.S = S;
   a.slabs = slabs; a.slab = slab; a.sr = sr; a.ss = ss;
-  const int slices = stream_slices(R, K, &a.kchunk);
+  const int slices = stream_slices(R, S, K, &a.kchunk);
   if (dtype == D_F32) return launch_stream_t<D_F32>(ctx, st, a, slices);
   if (dtype == D_BF16) return launch_stream_t<D_BF16>(ctx, st, a, slices);
   return launch_stream_t<D_F16>(ctx, st, a, slices);
