@@ -79,7 +79,7 @@ struct OrthArgs {
   const double* coef = nullptr;  // steps x (a, b, c), host
   double eps = 0;
 };
-bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: a short side of at most 64
+bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: both sides at most 128, or a short side of at most 64
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
 int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a);  // M <= 16
 

@@ -1,4 +1,9 @@
-// Orthogonalisation with a short side m of at most 64. All steps of x <- (a + b A + c A A) x, A = x x', act on x from the short side, so
+// Orthogonalisation of small matrices and of matrices with one short side.
+//
+// Both sides at most 128 (k_orth_direct): x and A stay in LDS in fp32, a workgroup per matrix does all steps as they are defined on
+// v_mfma_f32_16x16x4, one launch. Bound by the matrix instructions (40 x 40: 21 tiles of 10 per step, 0.9 us).
+//
+// A short side m of at most 64, the other longer: all steps of x <- (a + b A + c A A) x, A = x x', act on x from the short side, so
 //   x_T = Q x_0,   P = a I + b A + c A A,   Q <- P Q,   A <- P A P
 // needs the m x n matrix twice (for A_0 = x_0 x_0' and for the last product) whatever the number of steps; |g|_F^2 is the trace of g g'.
 // In exact arithmetic that is the definition. In floating point an error of A_0 grows with the square of a small singular value's growth
@@ -39,29 +44,38 @@ __device__ __forceinline__ void lower_tile(int t, int* i, int* j) {
   *j = t - r * (r + 1) / 2;
 }
 
-// 16 NW columns k0 .. of x (R rows, zeros outside) into registers, then into Xs[k][i]
-template <int T, int MT, int NW>
-struct Slab {
-  float v[4 * MT];
-  __device__ __forceinline__ void fetch(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend) {
-    constexpr int R = 16 * MT, CK = 16 * NW;
-    const auto* p = static_cast<const typename Elem<T>::type*>(a.o.x) + b * a.o.sx;
-#pragma unroll
-    for (int e = 0; e < 4 * MT; ++e) {
-      const int id = e * (64 * NW) + (int)threadIdx.x;
-      const int i = a.tall ? id % R : id / CK, k = a.tall ? id / R : id % CK;
-      const bool in = i < a.m && k0 + k < kend;
-      v[e] = in ? Elem<T>::ld(p + (a.tall ? (k0 + k) * a.o.ldx + i : i * a.o.ldx + k0 + k)) : 0.f;
-    }
-  }
-  __device__ __forceinline__ void put(float* Xs, int tall) {
+// Where a thread's 4 MT elements of 16 NW columns of x lie: below the columns' first element in x and y (in 32 bits: orth_is_small), and
+// in Xs[k][i]. Computed once: the divisions by R cost more than the loads.
+template <int MT, int NW>
+struct Places {
+  unsigned in[4 * MT], out[4 * MT];
+  unsigned short at[4 * MT], k[4 * MT];  // k: column, 0xffff for rows behind m
+  __device__ __forceinline__ Places(const SmallArgs& a) {
     constexpr int R = 16 * MT, CK = 16 * NW, LI = R + 1;
 #pragma unroll
     for (int e = 0; e < 4 * MT; ++e) {
       const int id = e * (64 * NW) + (int)threadIdx.x;
-      const int i = tall ? id % R : id / CK, k = tall ? id / R : id % CK;
-      Xs[k * LI + i] = v[e];
+      const int i = a.tall ? id % R : id / CK, c = a.tall ? id / R : id % CK;
+      at[e] = (unsigned short)(c * LI + i);
+      k[e] = (unsigned short)(i < a.m ? c : 0xffff);
+      in[e] = (unsigned)(a.tall ? c * a.o.ldx + i : i * a.o.ldx + c);
+      out[e] = (unsigned)(a.tall ? c * a.o.ldy + i : i * a.o.ldy + c);
     }
+  }
+};
+// columns k0 .. of x (zeros outside) into registers, then into Xs
+template <int T, int MT, int NW>
+struct Slab {
+  float v[4 * MT];
+  __device__ __forceinline__ void fetch(const SmallArgs& a, const Places<MT, NW>& pl, int64_t b, int64_t k0, int64_t kend) {
+    const auto* p = static_cast<const typename Elem<T>::type*>(a.o.x) + b * a.o.sx + (a.tall ? k0 * a.o.ldx : k0);
+    const int n = (int)min((int64_t)(16 * NW), kend - k0);
+#pragma unroll
+    for (int e = 0; e < 4 * MT; ++e) v[e] = pl.k[e] < n ? Elem<T>::ld(p + pl.in[e]) : 0.f;
+  }
+  __device__ __forceinline__ void put(const Places<MT, NW>& pl, float* Xs) {
+#pragma unroll
+    for (int e = 0; e < 4 * MT; ++e) Xs[pl.at[e]] = v[e];
   }
 };
 
@@ -74,18 +88,19 @@ __device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_
   f64x4 acc[NL];
 #pragma unroll
   for (int t = 0; t < NL; ++t) acc[t] = f64x4{0, 0, 0, 0};
+  const Places<MT, NW> pl(a);
   Slab<T, MT, NW> s[3];
 #pragma unroll
   for (int u = 0; u < 3; ++u)
-    if (k0 + u * CK < kend) s[u].fetch(a, b, k0 + u * CK, kend);
+    if (k0 + u * CK < kend) s[u].fetch(a, pl, b, k0 + u * CK, kend);
   for (int64_t k = k0; k < kend; k += 3 * CK) {
 #pragma unroll
     for (int u = 0; u < 3; ++u) {
       const int64_t ku = k + u * CK;
       if (ku < kend) {
-        s[u].put(Xs, a.tall);
+        s[u].put(pl, Xs);
         __syncthreads();
-        if (ku + 3 * CK < kend) s[u].fetch(a, b, ku + 3 * CK, kend);
+        if (ku + 3 * CK < kend) s[u].fetch(a, pl, b, ku + 3 * CK, kend);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           double f[MT];
@@ -116,9 +131,9 @@ __device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_
   __syncthreads();
 }
 
-// C tile (i, j) = X Y for symmetric X, Y in LDS (zeros behind m: whole tiles of the contraction, all reads in flight at once)
+// C tile (i, j) = X Y for symmetric X, Y in LDS: all reads first, then the chain of matrix instructions (64 cycles each) up to column m
 template <int MT>
-__device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, int i, int j) {
+__device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, int i, int j, int m) {
   constexpr int LQ = Tiles<MT>::LQ, KS = 4 * MT;
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const double *x = X + (i * 16 + r16) * LQ + q, *y = Y + (j * 16 + r16) * LQ + q;
@@ -128,9 +143,11 @@ __device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, 
     xv[s] = x[4 * s];
     yv[s] = y[4 * s];
   }
+  __builtin_amdgcn_sched_barrier(0);
   f64x4 acc = {0, 0, 0, 0};
 #pragma unroll
-  for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc, 0, 0, 0);
+  for (int s = 0; s < KS; ++s)
+    if (s < 4 * (MT - 1) || 4 * s < m) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc, 0, 0, 0);
   return acc;
 }
 template <int MT>
@@ -176,6 +193,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
     Q[r * LQ + c] = r == c && r < a.m ? f : 0.0;
   }
   __syncthreads();
+  // (tiles are dealt out to the 8 waves, two of which share a SIMD: the 12 of the second phase at m = 40 are 3 per SIMD)
   for (int t = 0; t < a.o.steps; ++t) {
     const double ca = cf.v[3 * t], cb = cf.v[3 * t + 1], cc = cf.v[3 * t + 2];
     const bool last = t + 1 == a.o.steps;
@@ -185,7 +203,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        f64x4 v = tile_product<MT>(A, A, i, j);
+        f64x4 v = tile_product<MT>(A, A, i, j, a.m);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int r = i * 16 + q + 4 * g, c = j * 16 + r16;
@@ -195,37 +213,38 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       }
     }
     __syncthreads();
-    f64x4 vq[NT], va[NT];
+    // P Q and, but for the last step, A P
+    constexpr int N2 = (2 * NL + 7) / 8;
+    f64x4 v2[N2];
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
+    for (int u = 0; u < N2; ++u) {
       const int w = wid + 8 * u;
-      if (w < NL) {
+      if (w < (last ? NL : 2 * NL)) {
         int i, j;
-        lower_tile(w, &i, &j);
-        vq[u] = tile_product<MT>(P, Q, i, j);
-        if (!last) va[u] = tile_product<MT>(A, P, i, j);
+        lower_tile(w < NL ? w : w - NL, &i, &j);
+        v2[u] = tile_product<MT>(w < NL ? Q : A, P, i, j, a.m);
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
+    for (int u = 0; u < N2; ++u) {
       const int w = wid + 8 * u;
-      if (w < NL) {
+      if (w < (last ? NL : 2 * NL)) {
         int i, j;
-        lower_tile(w, &i, &j);
-        tile_store<MT>(Q, i, j, vq[u]);
-        if (!last) tile_store<MT>(A, i, j, va[u]);
+        lower_tile(w < NL ? w : w - NL, &i, &j);
+        tile_store<MT>(w < NL ? Q : A, i, j, v2[u]);
       }
     }
     __syncthreads();
     if (last) break;
+    f64x4 va[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int w = wid + 8 * u;
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        va[u] = tile_product<MT>(A, P, i, j);
+        va[u] = tile_product<MT>(A, P, i, j, a.m);
       }
     }
     __syncthreads();
@@ -249,12 +268,13 @@ __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
   constexpr int KS = 4 * MT;
   auto* y = static_cast<typename Elem<T>::type*>(a.o.y) + b * a.o.sy;
+  const Places<MT, NW> pl(a);
   Slab<T, MT, NW> s;
-  s.fetch(a, b, k0, kend);
+  s.fetch(a, pl, b, k0, kend);
   for (int64_t k = k0; k < kend; k += CK) {
-    s.put(Xs, a.tall);
+    s.put(pl, Xs);
     __syncthreads();
-    if (k + CK < kend) s.fetch(a, b, k + CK, kend);
+    if (k + CK < kend) s.fetch(a, pl, b, k + CK, kend);
     f64x4 acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f64x4{0, 0, 0, 0};
@@ -271,13 +291,135 @@ __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64
 #pragma unroll
       for (int g = 0; g < 4; ++g) mine[i * 16 + q + 4 * g] = (float)acc[i][g];
     __syncthreads();
+    auto* yk = y + (a.tall ? k * a.o.ldy : k);
+    const int n = (int)min((int64_t)CK, kend - k);
 #pragma unroll
-    for (int e = 0; e < 4 * MT; ++e) {
-      const int id = e * (64 * NW) + (int)threadIdx.x;
-      const int i = a.tall ? id % R : id / CK, kk = a.tall ? id / R : id % CK;
-      if (i < a.m && k + kk < kend) Elem<T>::st(y + (a.tall ? (k + kk) * a.o.ldy + i : i * a.o.ldy + k + kk), Xs[kk * LI + i]);
+    for (int e = 0; e < 4 * MT; ++e)
+      if (pl.k[e] < n) Elem<T>::st(yk + pl.out[e], Xs[pl.at[e]]);
+    __syncthreads();
+  }
+}
+
+// ---- both sides at most D = 16 MT <= 128: x [m][n] (m <= n, zeros behind both) and A, which P = b A + c A A replaces, in LDS
+template <int T, int MT>
+__global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
+  // D + 4 floats between rows: 16 rows at one group of four columns fall into 16 different 16-byte bank groups
+  constexpr int D = 16 * MT, L = D + 4, NL = MT * (MT + 1) / 2, NT = (NL + 7) / 8, NX = (MT * MT + 7) / 8;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  float* X = reinterpret_cast<float*>(lds);
+  float* A = X + D * L;
+  double* S = reinterpret_cast<double*>(A + D * L);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
+  const int64_t b = blockIdx.x;
+  const int n = (int)a.n, rows = (int)a.o.rows, cols = (int)a.o.cols;
+  const auto* x = static_cast<const typename Elem<T>::type*>(a.o.x) + b * a.o.sx;
+  double sq = 0.0;
+  for (int e = tid; e < D * L; e += 512) X[e] = 0.f;
+  __syncthreads();
+  for (int e = tid; e < rows * cols; e += 512) {
+    const int r = e / cols, c = e - r * cols;
+    const float v = Elem<T>::ld(x + r * a.o.ldx + c);
+    X[a.tall ? c * L + r : r * L + c] = v;
+    sq += (double)v * (double)v;
+  }
+  for (int w = 32; w > 0; w >>= 1) sq += __shfl_xor(sq, w);
+  if (lane == 0) S[wid] = sq;
+  __syncthreads();
+  const double f = 1.0 / (sqrt(((S[0] + S[1]) + (S[2] + S[3])) + ((S[4] + S[5]) + (S[6] + S[7]))) + a.o.eps);
+  for (int e = tid; e < D * L; e += 512) X[e] = (float)((double)X[e] * f);
+  __syncthreads();
+  // four matrix instructions per 16 columns of the contraction: lane group q takes columns 4 q .. 4 q + 3, one per instruction
+  auto rows_product = [&](const float* M, int i, int j, int len) {  // rows i of M against rows j of M
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const float *u = M + (i * 16 + r16) * L + 4 * q, *v = M + (j * 16 + r16) * L + 4 * q;
+#pragma unroll 4
+    for (int s = 0; s < MT; ++s)
+      if (16 * s < len) {
+        const f32x4 uu = *reinterpret_cast<const f32x4*>(u + 16 * s), vv = *reinterpret_cast<const f32x4*>(v + 16 * s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(uu[e], vv[e], acc, 0, 0, 0);
+      }
+    return acc;
+  };
+  auto store_sym = [&](int i, int j, f32x4 v) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = i * 16 + 4 * q + g, c = j * 16 + r16;
+      A[r * L + c] = v[g];
+      if (i != j) A[c * L + r] = v[g];
+    }
+  };
+  const int mt = (a.m + 15) / 16, nt = (n + 15) / 16, nl = mt * (mt + 1) / 2;
+  for (int t = 0; t < a.o.steps; ++t) {
+    const float ca = (float)cf.v[3 * t], cb = (float)cf.v[3 * t + 1], cc = (float)cf.v[3 * t + 2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < nl) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        store_sym(i, j, rows_product(X, i, j, n));
+      }
     }
     __syncthreads();
+    f32x4 p[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < nl) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        p[u] = rows_product(A, i, j, a.m);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) p[u][g] = cc * p[u][g] + cb * A[(i * 16 + 4 * q + g) * L + j * 16 + r16];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int w = wid + 8 * u;
+      if (w < nl) {
+        int i, j;
+        lower_tile(w, &i, &j);
+        store_sym(i, j, p[u]);
+      }
+    }
+    __syncthreads();
+    f32x4 xn[NX];
+#pragma unroll
+    for (int u = 0; u < NX; ++u) {
+      const int w = wid + 8 * u;
+      if (w < mt * nt) {
+        const int i = w / nt, j = w - i * nt;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        const float *pu = A + (i * 16 + r16) * L + 4 * q, *xv = X + 4 * q * L + j * 16 + r16;
+#pragma unroll 4
+        for (int s = 0; s < MT; ++s)
+          if (16 * s < a.m) {
+            const f32x4 uu = *reinterpret_cast<const f32x4*>(pu + 16 * s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(uu[e], xv[(16 * s + e) * L], acc, 0, 0, 0);
+          }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) xn[u][g] = acc[g] + ca * X[(i * 16 + 4 * q + g) * L + j * 16 + r16];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NX; ++u) {
+      const int w = wid + 8 * u;
+      if (w < mt * nt) {
+        const int i = w / nt, j = w - i * nt;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) X[(i * 16 + 4 * q + g) * L + j * 16 + r16] = xn[u][g];
+      }
+    }
+    __syncthreads();
+  }
+  auto* y = static_cast<typename Elem<T>::type*>(a.o.y) + b * a.o.sy;
+  for (int e = tid; e < rows * cols; e += 512) {
+    const int r = e / cols, c = e - r * cols;
+    Elem<T>::st(y + r * a.o.ldy + c, X[a.tall ? c * L + r : r * L + c]);
   }
 }
 
@@ -360,6 +502,23 @@ int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
+template <int T, int MT>
+int run_direct(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
+  constexpr int LDS = 2 * 16 * MT * (16 * MT + 4) * 4 + 64;
+  if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_direct<T, MT>), LDS));
+  hipLaunchKernelGGL((k_orth_direct<T, MT>), dim3((unsigned)a.o.batch), dim3(512), LDS, st, a, cf);
+  SCL_HIP(ctx, hipGetLastError());
+  return SCLENS_OK;
+}
+template <int T>
+int run_direct_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
+  if (a.n <= 16) return run_direct<T, 1>(ctx, st, a, cf);
+  if (a.n <= 32) return run_direct<T, 2>(ctx, st, a, cf);
+  if (a.n <= 48) return run_direct<T, 3>(ctx, st, a, cf);
+  if (a.n <= 64) return run_direct<T, 4>(ctx, st, a, cf);
+  if (a.n <= 96) return run_direct<T, 6>(ctx, st, a, cf);
+  return run_direct<T, 8>(ctx, st, a, cf);
+}
 template <int T>
 int run_small_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   if (a.m <= 16) return run_small<T, 1>(ctx, st, a, cf);
@@ -369,7 +528,10 @@ int run_small_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
 }
 }  // namespace
 
-bool orth_is_small(const OrthArgs& o) { return std::min(o.rows, o.cols) <= 64 && o.steps <= MAX_RIDE; }
+bool orth_is_small(const OrthArgs& o) {
+  const int64_t m = std::min(o.rows, o.cols), n = std::max(o.rows, o.cols), ld = std::max(o.ldx, o.ldy);
+  return o.steps <= MAX_RIDE && (n <= 128 || m <= 64) && ld < ((int64_t)1 << 25);
+}
 
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws_bytes, int64_t* need) {
   SmallArgs a{};
@@ -378,7 +540,8 @@ int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws
   a.m = (int)std::min(o.rows, o.cols);
   a.n = std::max(o.rows, o.cols);
   const int MT = (a.m + 15) / 16, elems = MT * (MT + 1) / 2 * 256;
-  if (a.n <= 1024 || o.batch >= 128) a.slices = 1;
+  const bool direct = a.n <= 128;
+  if (direct || a.n <= 1024 || o.batch >= 128) a.slices = 1;
   else a.slices = (int)std::max<int64_t>(2, std::min<int64_t>((a.n + 255) / 256, 512 / o.batch));
   Carve c(ws);
   if (a.slices > 1) {
@@ -391,6 +554,11 @@ int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws
   Coefs cf{};
   for (int i = 0; i < 3 * o.steps; ++i) cf.v[i] = o.coef[i];
   a.o.coef = nullptr;
+  if (direct) {
+    if (o.dtype == D_F32) return run_direct_t<D_F32>(ctx, st, a, cf);
+    if (o.dtype == D_BF16) return run_direct_t<D_BF16>(ctx, st, a, cf);
+    return run_direct_t<D_F16>(ctx, st, a, cf);
+  }
   if (o.dtype == D_F32) return run_small_t<D_F32>(ctx, st, a, cf);
   if (o.dtype == D_BF16) return run_small_t<D_BF16>(ctx, st, a, cf);
   return run_small_t<D_F16>(ctx, st, a, cf);
