@@ -83,6 +83,11 @@ bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: both sides at most 12
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
 int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a);  // M <= 16
 
+bool linear_is_small(const LinearArgs& a);  // dense_small.hip: one launch, any address, no scratch
+bool backward_is_small(const LinearBwdArgs& a);
+int linear_small(Ctx* ctx, hipStream_t st, const LinearArgs& a);
+int backward_small(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a);
+
 // *need: bytes of scratch the call wants; launched only if ws_bytes >= *need (SCLENS_ERR_WORKSPACE otherwise)
 int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
 int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need);

@@ -234,4 +234,15 @@ __device__ __forceinline__ void act8(float v[8], int act) {
   }
 }
 
+template <bool GRAD>
+__device__ __forceinline__ float act_any(float z, int act) {
+  switch (act) {
+    case ACT_RELU: return GRAD ? act_grad<ACT_RELU>(z) : act_apply<ACT_RELU>(z);
+    case ACT_SILU: return GRAD ? act_grad<ACT_SILU>(z) : act_apply<ACT_SILU>(z);
+    case ACT_GELU: return GRAD ? act_grad<ACT_GELU>(z) : act_apply<ACT_GELU>(z);
+    case ACT_GELU_TANH: return GRAD ? act_grad<ACT_GELU_TANH>(z) : act_apply<ACT_GELU_TANH>(z);
+    default: return GRAD ? 1.f : z;
+  }
+}
+
 }  // namespace scl

@@ -77,6 +77,8 @@ static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big
 int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
   if (a.M > 0 && a.N > 0 && a.K > 0) {
     if (a.M <= 16) return linear_rows(ctx, st, a);
+    const bool tiles_as_is = direct(a.dtype, a.x, a.ldx, a.K) && direct(a.dtype, a.w, a.ldw, a.K);
+    if (!tiles_as_is && linear_is_small(a)) return linear_small(ctx, st, a);
     if (streams(a.dtype, a.w, a.ldw, a.M, a.N, a.K)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
     if (streams(a.dtype, a.x, a.ldx, a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
@@ -104,12 +106,65 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
 }
 
 // ------------------------------------------------------------------ linear, backward
-// dz = dy act'(z) for a 64 x 64 block: its image (contraction over the columns), the image of its transpose (contraction over the
-// rows) and the block's column sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the
-// saved pre-activation and the gradient that comes in already are.
+// dz in 16 bits: 128 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the
+// block's column sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
+// pre-activation and the gradient that comes in already are. Bound by HBM: two reads and a write per element.
+constexpr int DZ_ROWS = 128;
 template <int T>
-__global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, Mat imgT, float* __restrict__ part) {
-  constexpr int IT = T == D_F32 ? D_PL3 : T;
+__global__ __launch_bounds__(256) void k_dz16(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
+  __shared__ float L[16][132];
+  const int64_t nb = (N + 127) / 128, mb = blockIdx.x / nb;
+  const int64_t m0 = mb * DZ_ROWS, n0 = (blockIdx.x % nb) * 128;
+  const int tid = threadIdx.x, cc = (tid & 15) * 8, r0 = tid >> 4;
+  const int64_t col = n0 + cc;
+  const int nin = (int)max((int64_t)0, min((int64_t)8, N - col));
+  float sum[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  if (nin > 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Raw8<T> g[4], zz[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = m0 + r0 + 16 * (4 * h + i);
+        if (row < M) {
+          g[i].load(dy, row * dy.ld + col, nin);
+          if (act != ACT_NONE) zz[i].load(z, row * z.ld + col, nin);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = m0 + r0 + 16 * (4 * h + i);
+        if (row >= M) continue;
+        float v[8];
+        g[i].get(v);
+        if (act != ACT_NONE) {
+          float d[8];
+          zz[i].get(d);
+          act8<true>(d, act);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = e < nin ? v[e] * d[e] : 0.f;
+        }
+        if (img.p) store8<T>(img, row * img.ld + col, 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+      }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) L[r0][cc + e] = sum[e];
+  __syncthreads();
+  if (tid < 128 && n0 + tid < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += L[r][tid];
+    part[mb * N + n0 + tid] = s;
+  }
+}
+// fp32, a 64 x 64 block: the planes of dz (contraction over the columns), those of its transpose (over the rows) and the column sums
+__global__ __launch_bounds__(256) void k_dz32(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, Mat imgT, float* __restrict__ part) {
   __shared__ float L[64][65];
   const int64_t nb = (N + 63) / 64, mb = blockIdx.x / nb;
   const int64_t m0 = mb * 64, n0 = (blockIdx.x % nb) * 64;
@@ -124,17 +179,17 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     if (row < M && nin > 0) {
-      load8<T>(dy, row * dy.ld + col, nin, v);
+      load8<D_F32>(dy, row * dy.ld + col, nin, v);
       if (act != ACT_NONE) {
         float zz[8];
-        load8<T>(z, row * z.ld + col, nin, zz);
+        load8<D_F32>(z, row * z.ld + col, nin, zz);
         act8<true>(zz, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (e < nin) v[e] *= zz[e];
       }
     }
-    if (img.p && row < M) store8<IT>(img, row * img.ld + col, 8, v);
+    if (img.p && row < M) store8<D_PL3>(img, row * img.ld + col, 8, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) L[lr][cc + e] = v[e];
   }
@@ -147,7 +202,7 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = L[lr + e][lc];
-        store8<IT>(imgT, (n0 + lc) * imgT.ld + m0 + lr, 8, v);
+        store8<D_PL3>(imgT, (n0 + lc) * imgT.ld + m0 + lr, 8, v);
       }
     }
   }
@@ -171,10 +226,12 @@ __global__ __launch_bounds__(256) void k_colsum_join(const float* __restrict__ p
 }
 
 int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
+  if (a.M > 0 && a.N > 0 && backward_is_small(a)) return backward_small(ctx, st, a);
   Carve c(ws);
-  const int64_t nmb = (a.M + 63) / 64;
   const bool as_is = a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
   const bool f32 = a.dtype == D_F32;
+  const int rows_per = f32 ? 64 : DZ_ROWS, cols_per = f32 ? 64 : 128;
+  const int64_t nmb = (a.M + rows_per - 1) / rows_per;
   // 16 bits: dz, w and x feed both products as they lie (w and x with their rows across the contraction), through a padded copy if they
   // are not on 16 bytes. fp32: three planes with the contraction contiguous, so dz both ways, w and x transposed.
   Mat dz, dzT, wT, xT;
@@ -193,15 +250,14 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   if (c.used > ws_bytes) return no_room(ctx, c.used);
 
   if (a.M > 0 && a.N > 0 && (a.db || (a.dw && f32) || ((a.dx || a.dw) && !as_is))) {
-    const int64_t blocks = nmb * ((a.N + 63) / 64);
+    const int64_t blocks = nmb * ((a.N + cols_per - 1) / cols_per);
     if (blocks > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
     Mat img = as_is ? Mat() : dz;
-#define SCL_DZ(T) hipLaunchKernelGGL(k_dz<T>, dim3((unsigned)blocks), dim3(256), 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part)
-    if (a.dtype == D_F32) SCL_DZ(D_F32);
-    else if (a.dtype == D_BF16) SCL_DZ(D_BF16);
-    else SCL_DZ(D_F16);
-#undef SCL_DZ
+    const dim3 grid((unsigned)blocks), blk(256);
+    if (f32) hipLaunchKernelGGL(k_dz32, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
+    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_dz16<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else hipLaunchKernelGGL(k_dz16<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
     SCL_HIP(ctx, hipGetLastError());
   }
   if (a.db && a.N > 0) {

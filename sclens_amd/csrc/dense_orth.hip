@@ -79,8 +79,8 @@ struct Slab {
   }
 };
 
-// red[tile][g * 64 + lane] = sum over k0 <= k < kend of x x' (unscaled); every wave takes 16 of the columns in Xs. Loads run three slabs
-// ahead. part: 4 * NL * 256 doubles of LDS (the waves' sums, waves 4 .. 7 added to 0 .. 3 first, then those in order).
+// red[tile][g * 64 + lane] = sum over k0 <= k < kend of x x' (unscaled); every wave takes 16 of the columns in Xs. Loads run up to three
+// slabs ahead. part: 4 * NL * 256 doubles of LDS (the waves' sums, waves 4 .. 7 added to 0 .. 3 first, then those in order).
 template <int T, int MT, int NW>
 __device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, double* part, double* red) {
   constexpr int LI = Tiles<MT>::LI, NL = Tiles<MT>::NL, CK = 16 * NW;
@@ -89,18 +89,19 @@ __device__ __forceinline__ void gram_range(const SmallArgs& a, int64_t b, int64_
 #pragma unroll
   for (int t = 0; t < NL; ++t) acc[t] = f64x4{0, 0, 0, 0};
   const Places<MT, NW> pl(a);
-  Slab<T, MT, NW> s[3];
+  constexpr int PF = MT == 4 && NW == 8 ? 1 : 3;  // (more would not fit the registers)
+  Slab<T, MT, NW> s[PF];
 #pragma unroll
-  for (int u = 0; u < 3; ++u)
+  for (int u = 0; u < PF; ++u)
     if (k0 + u * CK < kend) s[u].fetch(a, pl, b, k0 + u * CK, kend);
-  for (int64_t k = k0; k < kend; k += 3 * CK) {
+  for (int64_t k = k0; k < kend; k += PF * CK) {
 #pragma unroll
-    for (int u = 0; u < 3; ++u) {
+    for (int u = 0; u < PF; ++u) {
       const int64_t ku = k + u * CK;
       if (ku < kend) {
         s[u].put(pl, Xs);
         __syncthreads();
-        if (ku + 3 * CK < kend) s[u].fetch(a, pl, b, ku + 3 * CK, kend);
+        if (ku + PF * CK < kend) s[u].fetch(a, pl, b, ku + PF * CK, kend);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           double f[MT];
@@ -144,11 +145,11 @@ __device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, 
     yv[s] = y[4 * s];
   }
   __builtin_amdgcn_sched_barrier(0);
-  f64x4 acc = {0, 0, 0, 0};
+  f64x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // (two chains: one alone waits for itself)
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    if (s < 4 * (MT - 1) || 4 * s < m) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc, 0, 0, 0);
-  return acc;
+    if (s < 4 * (MT - 1) || 4 * s < m) acc[s & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc[s & 1], 0, 0, 0);
+  return acc[0] + acc[1];
 }
 template <int MT>
 __device__ __forceinline__ void tile_store(double* C, int i, int j, f64x4 v) {
@@ -166,7 +167,7 @@ __device__ __forceinline__ void tile_store(double* C, int i, int j, f64x4 v) {
 template <int MT>
 __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const double* red, double* A, double* P, double* Q, double* scal) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, NL = Tiles<MT>::NL, NT = (NL + 7) / 8;
-  const int tid = threadIdx.x, wid = tid >> 6, lane = tid & 63, r16 = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     const int t = wid + 8 * u;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
   float* X = reinterpret_cast<float*>(lds);
   float* A = X + D * L;
   double* S = reinterpret_cast<double*>(A + D * L);
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
   const int64_t b = blockIdx.x;
   const int n = (int)a.n, rows = (int)a.o.rows, cols = (int)a.o.cols;
   const auto* x = static_cast<const typename Elem<T>::type*>(a.o.x) + b * a.o.sx;
@@ -350,14 +351,22 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
     }
   };
   const int mt = (a.m + 15) / 16, nt = (n + 15) / 16, nl = mt * (mt + 1) / 2;
+  // this wave's tiles of A and P, and of x
+  int li[NT], lj[NT], xi[NX], xj[NX];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) lower_tile(min(wid + 8 * u, nl - 1), &li[u], &lj[u]);
+#pragma unroll
+  for (int u = 0; u < NX; ++u) {
+    xi[u] = (wid + 8 * u) / nt;
+    xj[u] = wid + 8 * u - xi[u] * nt;
+  }
   for (int t = 0; t < a.o.steps; ++t) {
     const float ca = (float)cf.v[3 * t], cb = (float)cf.v[3 * t + 1], cc = (float)cf.v[3 * t + 2];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const int w = wid + 8 * u;
       if (w < nl) {
-        int i, j;
-        lower_tile(w, &i, &j);
+        const int i = li[u], j = lj[u];
         store_sym(i, j, rows_product(X, i, j, n));
       }
     }
@@ -367,8 +376,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
     for (int u = 0; u < NT; ++u) {
       const int w = wid + 8 * u;
       if (w < nl) {
-        int i, j;
-        lower_tile(w, &i, &j);
+        const int i = li[u], j = lj[u];
         p[u] = rows_product(A, i, j, a.m);
 #pragma unroll
         for (int g = 0; g < 4; ++g) p[u][g] = cc * p[u][g] + cb * A[(i * 16 + 4 * q + g) * L + j * 16 + r16];
@@ -379,8 +387,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
     for (int u = 0; u < NT; ++u) {
       const int w = wid + 8 * u;
       if (w < nl) {
-        int i, j;
-        lower_tile(w, &i, &j);
+        const int i = li[u], j = lj[u];
         store_sym(i, j, p[u]);
       }
     }
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
     for (int u = 0; u < NX; ++u) {
       const int w = wid + 8 * u;
       if (w < mt * nt) {
-        const int i = w / nt, j = w - i * nt;
+        const int i = xi[u], j = xj[u];
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         const float *pu = A + (i * 16 + r16) * L + 4 * q, *xv = X + 4 * q * L + j * 16 + r16;
 #pragma unroll 4
@@ -409,7 +416,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
     for (int u = 0; u < NX; ++u) {
       const int w = wid + 8 * u;
       if (w < mt * nt) {
-        const int i = w / nt, j = w - i * nt;
+        const int i = xi[u], j = xj[u];
 #pragma unroll
         for (int g = 0; g < 4; ++g) X[(i * 16 + 4 * q + g) * L + j * 16 + r16] = xn[u][g];
       }

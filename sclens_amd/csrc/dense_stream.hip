@@ -106,13 +106,7 @@ __global__ __launch_bounds__(512) void k_rows(LinearArgs a) {
   for (int w = 0; w < 8; ++w) z += S[w][at];
   if (a.bias) z += Elem<T>::ld(static_cast<const E*>(a.bias) + n);
   if (a.pre) Elem<T>::st(static_cast<E*>(a.pre) + m * a.ldz + n, z);
-  switch (a.act) {
-    case ACT_RELU: z = act_apply<ACT_RELU>(z); break;
-    case ACT_SILU: z = act_apply<ACT_SILU>(z); break;
-    case ACT_GELU: z = act_apply<ACT_GELU>(z); break;
-    case ACT_GELU_TANH: z = act_apply<ACT_GELU_TANH>(z); break;
-    default: break;
-  }
+  z = act_any<false>(z, a.act);
   if (a.res) z += Elem<T>::ld(static_cast<const E*>(a.res) + m * a.ldr + n);
   Elem<T>::st(static_cast<E*>(a.y) + m * a.ldy + n, z);
 }
