@@ -106,10 +106,10 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
 }
 
 // ------------------------------------------------------------------ linear, backward
-// dz in 16 bits: 128 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the
+// dz in 16 bits: 64 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the
 // block's column sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
 // pre-activation and the gradient that comes in already are. Bound by HBM: two reads and a write per element.
-constexpr int DZ_ROWS = 128;
+constexpr int DZ_ROWS = 64;
 template <int T>
 __global__ __launch_bounds__(256) void k_dz16(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
   __shared__ float L[16][132];
@@ -122,34 +122,32 @@ __global__ __launch_bounds__(256) void k_dz16(Mat dy, Mat z, int act, int64_t M,
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
   if (nin > 0) {
+    constexpr int NR = DZ_ROWS / 16;
+    Raw8<T> g[NR], zz[NR];  // all loads first
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      Raw8<T> g[4], zz[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t row = m0 + r0 + 16 * (4 * h + i);
-        if (row < M) {
-          g[i].load(dy, row * dy.ld + col, nin);
-          if (act != ACT_NONE) zz[i].load(z, row * z.ld + col, nin);
-        }
+    for (int i = 0; i < NR; ++i) {
+      const int64_t row = m0 + r0 + 16 * i;
+      if (row < M) {
+        g[i].load(dy, row * dy.ld + col, nin);
+        if (act != ACT_NONE) zz[i].load(z, row * z.ld + col, nin);
       }
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t row = m0 + r0 + 16 * (4 * h + i);
-        if (row >= M) continue;
-        float v[8];
-        g[i].get(v);
-        if (act != ACT_NONE) {
-          float d[8];
-          zz[i].get(d);
-          act8<true>(d, act);
+    for (int i = 0; i < NR; ++i) {
+      const int64_t row = m0 + r0 + 16 * i;
+      if (row >= M) continue;
+      float v[8];
+      g[i].get(v);
+      if (act != ACT_NONE) {
+        float d[8];
+        zz[i].get(d);
+        act8<true>(d, act);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = e < nin ? v[e] * d[e] : 0.f;
-        }
-        if (img.p) store8<T>(img, row * img.ld + col, 8, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+        for (int e = 0; e < 8; ++e) v[e] = e < nin ? v[e] * d[e] : 0.f;
       }
+      if (img.p) store8<T>(img, row * img.ld + col, 8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += v[e];
     }
   }
   if (!part) return;
