@@ -21,7 +21,7 @@ struct Mat {
 
 // C[b] = epilogue(alpha * A[b] B[b]'), A [M][K], B [N][K], K contiguous.
 struct Product {
-  int type = D_BF16;  // D_BF16 / D_F16: what the 16-bit images hold; D_PL3: three bf16 planes each, six products per term
+  int type = D_BF16;  // of the operands; D_PL3: fp32 as three bf16 planes each, six products per term
   Mat A, B;
   int64_t M = 0, N = 0, K = 0;
   int batch = 1;
@@ -37,6 +37,7 @@ struct Product {
   int64_t slab_bytes = 0;
 };
 int64_t product_slab_bytes(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric);
+double product_us(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric);  // the plan's estimate
 int product(Ctx* ctx, hipStream_t st, const Product& p);
 
 // the join of slabs [slices][M][round_up8(N)] written by somebody else, through p's epilogue (p.slabs set; operands only for fp32 NaN)
@@ -48,12 +49,11 @@ int stream_slices(int64_t R, int64_t S, int64_t K, int* kchunk);
 int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t ldb, int64_t R, const Mat& small, int64_t S, int64_t K,
                    float* slabs, int64_t slab, int64_t sr, int64_t ss);
 
-// 16-bit image (D_F32: three bf16 planes) of src (element (r, k) at r * ld + k, transposed: k * ld + r), rows x K, K padded with zeros
-// to image_ld(K)
+// Image of src (element (r, k) at r * ld + k, transposed: k * ld + r), rows x K, K padded with zeros to image_ld(K): of its own type, or
+// (D_PL3, from fp32) three bf16 planes
 static inline int64_t image_ld(int64_t K) { return round_up(K > 0 ? K : 1, 64); }
 static inline int64_t image_elems(int64_t rows, int64_t K) { return round_up(rows, 8) * image_ld(K); }
-static inline int planes_of(int dtype) { return dtype == D_F32 ? 3 : 1; }
-int pack_image(Ctx* ctx, hipStream_t st, int dtype, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img);
+int pack_image(Ctx* ctx, hipStream_t st, int dtype, int image, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img);
 
 struct LinearArgs {
   int dtype = D_F32, act = ACT_NONE;

@@ -111,12 +111,21 @@ __device__ __forceinline__ u16x8 read_across(const unsigned char* p) {
   return __builtin_bit_cast(u16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+template <int ROW>
+__device__ __forceinline__ u16x8 read_words(const unsigned char* p) {
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(p + e * ROW);
+  return __builtin_bit_cast(u16x8, v);
+}
+
 template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
 __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(ProdArgs g) {
   constexpr int NW = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, NP = PA + PB;  // 1 KB copies (8 rows x 64 columns) per wave and stage
   constexpr int OPA = BM * 128, STAGE = (BM + BN) * 128;
-  constexpr bool PL = (MT == D_PL3);
+  constexpr bool PL = (MT == D_PL3), F32 = (MT == D_F32);
+  constexpr int ES = F32 ? 4 : 2, CE = 16 / ES, SC = 128 / ES;  // bytes of an element, elements of a chunk, columns of a stage
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const Product& p = g.p;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,10 +152,11 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   // ---- sources of this wave's copies: a uniform base that moves along the contraction, and each lane's place below it (the plan
   // keeps it below 2^32 bytes). A lane's 16 bytes of copy i land at byte 1024 i' + 16 lane of the operand's stage:
   //   rows along the contraction (AC / BC false): row r, slot q of 8 chunks, columns 8 (q ^ ((r >> 1) & 7)) ..
-  //   rows across it (true): column k of the contraction, slot of BM / 8 chunks; the 32-byte pair it is in is swizzled by k (pair_swz)
+  //   rows across it (true): column k of the contraction, slot of its chunks; in 16 bits the 32-byte pair it is in is swizzled by k
+  //   (pair_swz)
   const int srow = lane >> 3, sq = lane & 7;
-  const char* baseA = static_cast<const char*>(p.A.p) + 2 * (batch * p.A.batch + (AC ? m0 : m0 * p.A.ld));
-  const char* baseB = static_cast<const char*>(p.B.p) + 2 * (batch * p.B.batch + (BC ? n0 : n0 * p.B.ld));
+  const char* baseA = static_cast<const char*>(p.A.p) + ES * (batch * p.A.batch + (AC ? m0 : m0 * p.A.ld));
+  const char* baseB = static_cast<const char*>(p.B.p) + ES * (batch * p.B.batch + (BC ? n0 : n0 * p.B.ld));
   const int64_t stepA = AC ? 128 * p.A.ld : 128, stepB = BC ? 128 * p.B.ld : 128;  // bytes per stage
   // ktail != 0: the last stage of the contraction, of which only ktail columns exist: the others are copied from the stage's first
   // chunk / first column (in bounds whatever the matrix) and overwritten with zeros in LDS when they have landed
@@ -156,16 +166,17 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
     const int64_t rows = isA ? p.M - m0 : p.N - n0, ld = isA ? p.A.ld : p.B.ld;
     if (isA ? AC : BC) {
       const int W = isA ? BM : BN, byte = grp * 1024 + lane * 16;
-      int k = byte / (2 * W);
-      const int slot = (byte - k * 2 * W) >> 4, c = ((slot >> 1) ^ (W == 256 || W == 128 ? pair_swz<256>(k) : pair_swz<64>(k))) * 2 + (slot & 1);
+      int k = byte / (ES * W);
+      const int slot = (byte - k * ES * W) >> 4;
+      const int c = F32 ? slot : ((slot >> 1) ^ (W == 256 || W == 128 ? pair_swz<256>(k) : pair_swz<64>(k))) * 2 + (slot & 1);
       if (ktail && k >= ktail) k = 0;
-      return (unsigned)(2 * (k * ld + (8 * c < rows ? 8 * c : 0)));  // (columns behind the end are not stored)
+      return (unsigned)(ES * (k * ld + (CE * c < rows ? CE * c : 0)));  // (columns behind the end are not stored)
     }
     const int r = grp * 8 + srow;
     int chunk = sq ^ ((r >> 1) & 7);
-    if (ktail && 8 * chunk >= ktail) chunk = 0;
+    if (ktail && CE * chunk >= ktail) chunk = 0;
     const int64_t row = r < rows ? r : rows - 1;  // (products of rows behind the end are not stored)
-    return (unsigned)(2 * (row * ld + 8 * chunk));
+    return (unsigned)(ES * (row * ld + CE * chunk));
   };
   unsigned voff[NP];
 #pragma unroll
@@ -188,7 +199,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
       curB += 2 * pb * p.B.plane;
     }
   };
-  const int ktail = (int)(p.K & 63);
+  const int ktail = (int)(p.K % SC);
   bool ld_tail = false;
   auto set_tail = [&]() {
     const bool tail = ktail != 0 && ld_k + 1 == g.nkt;
@@ -218,9 +229,9 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
     auto zero = [&](unsigned char* o, auto across, auto w) {
       constexpr int W = decltype(w)::value;
       if constexpr (decltype(across)::value) {  // whole columns of the contraction
-        for (int e = ktail * W * 2 + tid * 16; e < 64 * W * 2; e += NW * 64 * 16) *reinterpret_cast<u16x8*>(o + e) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        for (int e = ktail * W * ES + tid * 16; e < SC * W * ES; e += NW * 64 * 16) *reinterpret_cast<u16x8*>(o + e) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
       } else {
-        const int first = (ktail + 7) / 8, n = 8 - first;
+        const int first = (ktail + CE - 1) / CE, n = 8 - first;
         for (int e = tid; e < W * n; e += NW * 64) {
           const int r = e / n, c = first + e % n;
           *reinterpret_cast<u16x8*>(o + r * 128 + ((c ^ ((r >> 1) & 7)) << 4)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -244,23 +255,34 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   // have the same swizzle. Rows across it: two transposing reads of 4 columns each -- 16 lanes name 4 columns x 16 rows (lane i: column
   // i >> 2, rows 4 (i & 3) ..) and lane i receives row i of all four; lanes 16 .. 31 take the other 16 rows, 32 .. 63 columns 8 .. 15.
   const int ra = (wm * TM * 32 + l31) * 128, rb = OPA + (wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
+  // fp32: the chunk of 4 columns 8 kk + 4 h .. of the row, its e-th column in the e-th of four matrix instructions; across, four words.
   const int tr = (lane & 15) >> 2, tk = 8 * h + tr, th = (lane >> 4) & 1;
   int ca[AC ? TM : 1], cb[BC ? TN : 1];
-  if constexpr (AC) {
+  if constexpr (AC && F32) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ca[i] = 4 * h * 4 * BM + (wm * TM * 32 + i * 32 + l31) * 4;
+  }
+  if constexpr (BC && F32) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) cb[j] = OPA + 4 * h * 4 * BN + (wn * TN * 32 + j * 32 + l31) * 4;
+  }
+  if constexpr (AC && !F32) {
 #pragma unroll
     for (int i = 0; i < TM; ++i) ca[i] = tk * 2 * BM + ((wm * TM * 2 + 2 * i + th) ^ pair_swz<BM>(tk)) * 32 + (lane & 3) * 8;
   }
-  if constexpr (BC) {
+  if constexpr (BC && !F32) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) cb[j] = OPA + tk * 2 * BN + ((wn * TN * 2 + 2 * j + th) ^ pair_swz<BN>(tk)) * 32 + (lane & 3) * 8;
   }
   u16x8 av[2][TM], bv[2][TN];
   auto fragA = [&](const unsigned char* B, int kk, int i) {
-    if constexpr (AC) return read_across<2 * BM>(B + ca[i] + kk * 16 * 2 * BM);
+    if constexpr (AC && F32) return read_words<4 * BM>(B + ca[i] + kk * 8 * 4 * BM);
+    else if constexpr (AC) return read_across<2 * BM>(B + ca[i] + kk * 16 * 2 * BM);
     else return *reinterpret_cast<const u16x8*>(B + ra + i * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
   };
   auto fragB = [&](const unsigned char* B, int kk, int j) {
-    if constexpr (BC) return read_across<2 * BN>(B + cb[j] + kk * 16 * 2 * BN);
+    if constexpr (BC && F32) return read_words<4 * BN>(B + cb[j] + kk * 8 * 4 * BN);
+    else if constexpr (BC) return read_across<2 * BN>(B + cb[j] + kk * 16 * 2 * BN);
     else return *reinterpret_cast<const u16x8*>(B + rb + j * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
   };
   // read n of a unit's TM + TN: the operands in the order in which the matrix instructions want them
@@ -272,20 +294,24 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   // one matrix instruction at a time, and in its shadow what `beside` issues
   auto unit = [&](int set, auto beside) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int e = 0; e < (F32 ? 4 : 1); ++e)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (MT == D_F16)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, bv[set][j]), __builtin_bit_cast(f16x8, av[set][i]),
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          if constexpr (F32)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, bv[set][j])[e], __builtin_bit_cast(f32x4, av[set][i])[e],
                                                              acc[i][j], 0, 0, 0);
-        else
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bv[set][j]),
-                                                              __builtin_bit_cast(bf16x8, av[set][i]), acc[i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        beside(i * TN + j);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+          else if constexpr (MT == D_F16)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, bv[set][j]), __builtin_bit_cast(f16x8, av[set][i]),
+                                                               acc[i][j], 0, 0, 0);
+          else
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bv[set][j]),
+                                                                __builtin_bit_cast(bf16x8, av[set][i]), acc[i][j], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (e == 0) beside(i * TN + j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
   };
   constexpr int NM = TM * TN, NR = TM + TN, QR = (NR + NM - 1) / NM;
   auto reads = [&](int set, const unsigned char* B, int kk, int m) {
@@ -430,16 +456,21 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
     if constexpr (!PL) {
       if (inside) {
         const int64_t row0 = row_w + cr;
-        const char* pr = static_cast<const char*>(p.res.p) + 2 * (batch * p.res.batch + row0 * p.res.ld + col);
-        char* po = static_cast<char*>(p.out.p) + 2 * (batch * p.out.batch + row0 * p.out.ld + col);
-        char* pz = static_cast<char*>(p.pre.p) + 2 * (batch * p.pre.batch + row0 * p.pre.ld + col);
-        const int64_t sr = 2 * RP * p.res.ld, so = 2 * RP * p.out.ld, sz = 2 * RP * p.pre.ld;
+        const char* pr = static_cast<const char*>(p.res.p) + ES * (batch * p.res.batch + row0 * p.res.ld + col);
+        constexpr int OS = OT == D_F32 ? 4 : 2, NST = NS * OS / 2;  // 16-byte stores of a block per result
+        static_assert(PART || PL || (RT == D_F32 ? 4 : 2) == ES, "the residual has the operands' size");
+        char* po = static_cast<char*>(p.out.p) + OS * (batch * p.out.batch + row0 * p.out.ld + col);
+        char* pz = static_cast<char*>(p.pre.p) + OS * (batch * p.pre.batch + row0 * p.pre.ld + col);
+        const int64_t sr = ES * RP * p.res.ld, so = OS * RP * p.out.ld, sz = OS * RP * p.pre.ld;
         const bool has_res = p.res.p != nullptr, has_out = p.out.p != nullptr, has_pre = p.pre.p != nullptr;
-        unsigned char* R = lds + NW * 32 * LP * 4 + wid * 2 * NS * 1024;
+        constexpr int RB = NS * 1024 * ES / 2;  // bytes of a block's residual
+        unsigned char* R = lds + NW * 32 * LP * 4 + wid * 2 * RB;
         auto copy_res = [&](int buf) {
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
-            __builtin_amdgcn_global_load_lds((glb_cv*)pr, (lds_v*)(R + (buf * NS + s) * 1024), 16, 0, 0);
+#pragma unroll
+            for (int q = 0; q < ES / 2; ++q)
+              __builtin_amdgcn_global_load_lds((glb_cv*)(pr + 16 * q), (lds_v*)(R + buf * RB + (s * (ES / 2) + q) * 1024), 16, 0, 0);
             pr += sr;
           }
         };
@@ -450,12 +481,12 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
         for (int i = 0; i < TM; ++i) {
           if (has_res) {
             if (i == 0 || turned) wait_vm<0>();
-            else if (has_out && has_pre) wait_vm<2 * NS>();
-            else wait_vm<NS>();
+            else if (has_out && has_pre) wait_vm<2 * NST>();
+            else wait_vm<NST>();
             if (i + 1 < TM) copy_res((i + 1) & 1);
           }
           to_lds(i);
-          const unsigned char* Ri = R + (i & 1) * NS * 1024 + lane * 16;
+          const unsigned char* Ri = R + (i & 1) * RB + lane * 16;
 #pragma unroll 1
           for (int s = 0; s < NS; ++s) {
             float v[8];
@@ -469,12 +500,13 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
             }
             if (p.act != ACT_NONE) act8<false>(v, p.act);
             if (has_res) {
-              const u16x8 r = *reinterpret_cast<const u16x8*>(Ri + s * 1024);
+              Raw8<RT> r;
+              float f[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const unsigned short q = r[e];
-                v[e] = fmaf(p.beta, Elem<RT>::ld(&q), v[e]);
-              }
+              for (int q = 0; q < ES / 2; ++q) r.r[q] = *reinterpret_cast<const u16x8*>(Ri + (s * (ES / 2) + q) * 1024);
+              r.get(f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = fmaf(p.beta, f[e], v[e]);
             }
             if (has_out) {
               plain.p = po;
@@ -597,7 +629,7 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
 
 namespace {
 
-struct Plan { int tile, ksplit, kchunk, tm, tn; int64_t tiles; };
+struct Plan { int tile, ksplit, kchunk, tm, tn; int64_t tiles; double us; };
 
 // a lane's place below its tile's base has 32 bits: 64 rows of 2^25 elements, 256 of 2^23
 constexpr int64_t MAX_LD = (int64_t)1 << 25, MAX_LD_BIG = (int64_t)1 << 22;
@@ -612,15 +644,19 @@ struct TileKind {
 // measured at 16 and 64 stages on 64 to 1024 tiles
 constexpr int NTILES = 5;
 const TileKind TILES[NTILES] = {{256, 1, 1.0, 1.48, 15.0}, {192, 1, 0.80, 0.90, 11.0}, {128, 2, 0.73, 1.05, 4.0}, {128, 1, 0.53, 0.55, 6.0}, {64, 2, 0.29, 0.41, 3.5}};
+// fp32 on the fp32 matrix cores, stages of 32 columns: bound by the matrix instructions in every tile (two workgroups on a CU take twice as
+// long), so the two smallest do; the larger ones' residual would not fit LDS beside the accumulators
+const TileKind TILES_F32[NTILES] = {{0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {128, 1, 2.0, 2.1, 6.0}, {64, 2, 0.55, 1.05, 4.0}};
 
 // The tile and the slices of the contraction with the least time by the figures above: rounds of the chip's 256 CUs, the stages of a
 // workgroup, and for slices the slabs written, read and joined by a second launch.
 Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric, bool may_split) {
-  const int64_t nst = std::max<int64_t>(1, (type == D_PL3 ? 6 : 1) * ((K + 63) / 64));
+  const int64_t nst = std::max<int64_t>(1, type == D_F32 ? (K + 31) / 32 : (type == D_PL3 ? 6 : 1) * ((K + 63) / 64));
   Plan best{};
   double best_t = 1e300;
   for (int t = K > MAX_LD_BIG ? NTILES - 1 : 0; t < NTILES; ++t) {
-    const TileKind& k = TILES[t];
+    const TileKind& k = (type == D_F32 ? TILES_F32 : TILES)[t];
+    if (k.bm == 0) continue;
     const int64_t tm = (M + k.bm - 1) / k.bm, tn = (N + k.bm - 1) / k.bm;
     const int64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
     for (int ks = 1; ks <= 32; ks *= 2) {
@@ -637,6 +673,7 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
         best.tm = (int)tm;
         best.tn = (int)tn;
         best.tiles = tiles / batch;
+        best.us = us;
       }
     }
   }
@@ -646,8 +683,10 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
 
 template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
 int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
-  // the stages; the epilogue's blocks of fp32 and two blocks of a 16-bit residual per wave
-  constexpr int LDS = std::max(S * (WM * TM + WN * TN) * 32 * 128, WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * 32 * TN * 2));
+  // the stages; the epilogue's block of fp32 and two blocks of the residual per wave
+  constexpr int LDS = std::max(S * (WM * TM + WN * TN) * 32 * 128,
+                               WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * (TN == 3 ? 128 : 32 * TN) * (MT == D_F32 ? 4 : 2)));
+  static_assert(LDS <= 163840, "LDS of a CU");
   const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
   hipLaunchKernelGGL((k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>), grid, dim3(WM * WN * 64), LDS, st, g);
@@ -656,10 +695,12 @@ int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
 }
 template <int MT, int OT, int RT, bool PART, bool AC, bool BC>
 int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile) {
+  if constexpr (MT != D_F32) {
+    if (tile == 0) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 4, 4, 2>(ctx, st, g, grid);
+    if (tile == 1) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 3, 3, 3>(ctx, st, g, grid);
+    if (tile == 2) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 2>(ctx, st, g, grid);
+  }
   switch (tile) {
-    case 0: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 4, 4, 2>(ctx, st, g, grid);
-    case 1: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 3, 3, 3>(ctx, st, g, grid);
-    case 2: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 2>(ctx, st, g, grid);
     case 3: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 4>(ctx, st, g, grid);
     default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, 4>(ctx, st, g, grid);
   }
@@ -682,6 +723,10 @@ int64_t product_slab_bytes(int64_t M, int64_t N, int64_t K, int batch, int type,
   return pl.ksplit > 1 ? (int64_t)pl.ksplit * batch * M * round_up8(N) * 4 : 0;
 }
 
+double product_us(int64_t M, int64_t N, int64_t K, int batch, int type, int symmetric) {
+  return plan_product(M, N, K, batch, type, symmetric, true).us;
+}
+
 int product(Ctx* ctx, hipStream_t st, const Product& p) {
   if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return SCLENS_OK;
   const int64_t slab = p.slabs ? product_slab_bytes(p.M, p.N, p.K, p.batch, p.type, p.symmetric) : 0;
@@ -694,7 +739,7 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   g.tiles_n = pl.tn;
   g.ksplit = pl.ksplit;
   g.kchunk = pl.kchunk;
-  g.nkt = (int)((p.K + 63) / 64);
+  g.nkt = (int)(p.type == D_F32 ? (p.K + 31) / 32 : (p.K + 63) / 64);
   const int form = (p.A.across ? 2 : 0) + (p.B.across ? 1 : 0);
   if (p.type == D_F16) {
     if (p.out_type == D_F16) {
@@ -708,6 +753,10 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
     if (form == 0) return launch_types<D_BF16, D_BF16, D_BF16>(ctx, st, g, pl);
     if (form == 1) return launch_types<D_BF16, D_BF16, D_BF16, false, true>(ctx, st, g, pl);
     if (form == 3) return launch_types<D_BF16, D_BF16, D_BF16, true, true>(ctx, st, g, pl);
+  } else if (p.type == D_F32 && p.out_type == D_F32) {
+    if (form == 0) return launch_types<D_F32, D_F32, D_F32>(ctx, st, g, pl);
+    if (form == 1) return launch_types<D_F32, D_F32, D_F32, false, true>(ctx, st, g, pl);
+    if (form == 3) return launch_types<D_F32, D_F32, D_F32, true, true>(ctx, st, g, pl);
   } else if (form == 0) {
     if (p.type == D_PL3 && p.out_type == D_PL3) return launch_types<D_PL3, D_PL3, D_PL3>(ctx, st, g, pl);
     if (p.type == D_PL3 && p.out_type == D_F32 && p.res_type == D_PL3) return launch_types<D_PL3, D_F32, D_PL3>(ctx, st, g, pl);
@@ -730,10 +779,9 @@ int product_join(Ctx* ctx, hipStream_t st, const Product& p, int slices) {
 
 // ------------------------------------------------------------------ images
 // 64 rows x 64 columns of the image per workgroup. Straight: 8 columns per lane. Transposed: through LDS, reads along the source's rows.
-template <int T, bool TRANS>
+template <int T, int IT, bool TRANS>
 __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __restrict__ src, int64_t ld, int64_t rows, int64_t K, int src_vec,
                                               Mat img) {
-  constexpr int IT = T == D_F32 ? D_PL3 : T;
   typedef typename Elem<T>::type E;
   const int64_t r0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 64;
   const int tid = threadIdx.x;
@@ -782,7 +830,7 @@ __global__ __launch_bounds__(256) void k_pack(const typename Elem<T>::type* __re
   }
 }
 
-int pack_image(Ctx* ctx, hipStream_t st, int dtype, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img) {
+int pack_image(Ctx* ctx, hipStream_t st, int dtype, int image, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img) {
   // img->p, plane are the caller's; the leading dimension is that of an image
   img->ld = image_ld(K);
   img->vec = img->pad = 1;
@@ -795,10 +843,16 @@ int pack_image(Ctx* ctx, hipStream_t st, int dtype, const void* src, int64_t ld,
     const dim3 grid((unsigned)kb, (unsigned)nb), block(256);
     const char* s = static_cast<const char*>(src) + (transposed ? y0 * 64 : y0 * 64 * ld) * size;
     Mat m = *img;
-    m.p = static_cast<unsigned short*>(img->p) + y0 * 64 * img->ld;
+    m.p = static_cast<char*>(img->p) + y0 * 64 * img->ld * (image == D_F32 ? 4 : 2);
     const int64_t nr = std::min<int64_t>(rows - y0 * 64, nb * 64);
-#define SCL_PACK(T)                                                                                                                     if (transposed)                                                                                                                         hipLaunchKernelGGL((k_pack<T, true>), grid, block, 0, st, reinterpret_cast<const Elem<T>::type*>(s), ld, nr, K, vec, m);            else                                                                                                                                    hipLaunchKernelGGL((k_pack<T, false>), grid, block, 0, st, reinterpret_cast<const Elem<T>::type*>(s), ld, nr, K, vec, m);
-    if (dtype == D_F32) { SCL_PACK(D_F32) } else if (dtype == D_BF16) { SCL_PACK(D_BF16) } else { SCL_PACK(D_F16) }
+#define SCL_PACK(T, I, TR) \
+  hipLaunchKernelGGL((k_pack<T, I, TR>), grid, block, 0, st, reinterpret_cast<const Elem<T>::type*>(s), ld, nr, K, vec, m)
+    if (image == D_PL3 && transposed) SCL_PACK(D_F32, D_PL3, true);
+    else if (image == D_PL3) SCL_PACK(D_F32, D_PL3, false);
+    else if (transposed) return ctx->fail(SCLENS_ERR_ARG, "pack_image: transposed only into planes");
+    else if (dtype == D_F32) SCL_PACK(D_F32, D_F32, false);
+    else if (dtype == D_BF16) SCL_PACK(D_BF16, D_BF16, false);
+    else SCL_PACK(D_F16, D_F16, false);
 #undef SCL_PACK
   }
   SCL_HIP(ctx, hipGetLastError());

@@ -17,8 +17,11 @@ int no_room(Ctx* ctx, int64_t need) {
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// a 16-bit matrix whose rows start on 16 bytes and whose contraction is whole 8-column chunks feeds the products as it lies
-bool direct(int dtype, const void* p, int64_t ld, int64_t K) { return dtype != D_F32 && ld % 8 == 0 && ld <= ((int64_t)1 << 22) && K % 8 == 0 && aligned16(p); }
+// a matrix whose rows start on 16 bytes and are whole 16-byte chunks feeds the products of its own type as it lies
+bool direct(int dtype, const void* p, int64_t ld, int64_t K) {
+  const int64_t chunk = dtype == D_F32 ? 4 : 8;
+  return ld % chunk == 0 && ld <= ((int64_t)1 << (dtype == D_F32 ? 21 : 22)) && K % chunk == 0 && aligned16(p);
+}
 
 Mat user_mat(const void* p, int64_t ld, int64_t batch = 0) {
   Mat m;
@@ -28,16 +31,20 @@ Mat user_mat(const void* p, int64_t ld, int64_t batch = 0) {
   m.vec = ld % 8 == 0 && batch % 8 == 0 && aligned16(p);
   return m;
 }
-Mat image_of(Carve& c, int dtype, int64_t rows, int64_t K, int64_t batch = 1) {
+Mat image_of(Carve& c, int image, int64_t rows, int64_t K, int64_t batch = 1) {
   Mat m;
   m.batch = image_elems(rows, K);
   m.plane = m.batch * batch;
   m.ld = image_ld(K);
   m.vec = m.pad = 1;
-  m.p = c.take<unsigned short>(m.plane * planes_of(dtype));
+  m.p = image == D_F32 ? static_cast<void*>(c.take<float>(m.plane)) : c.take<unsigned short>(m.plane * (image == D_PL3 ? 3 : 1));
   return m;
 }
-int image_type(int dtype) { return dtype == D_F32 ? D_PL3 : dtype; }
+// fp32 products: on the fp32 matrix cores as the matrices lie, or from three bf16 planes each at 1.5 times the rate, which first have to
+// be written (4 bytes read, 6 written per element and operand, 4 TB/s)
+bool planes_pay(int64_t M, int64_t N, int64_t K, int64_t packed_elems, int batch = 1, int symmetric = 0) {
+  return product_us(M, N, K, batch, D_PL3, symmetric) + (double)packed_elems * 10.0 / 4e6 + 6.0 < product_us(M, N, K, batch, D_F32, symmetric);
+}
 }  // namespace
 
 // ------------------------------------------------------------------ linear
@@ -45,7 +52,7 @@ int image_type(int dtype) { return dtype == D_F32 ? D_PL3 : dtype; }
 // rows that do not start on 16 bytes) up to 128 rows of the other stream it as it lies and join the slices of the contraction. Short
 // contractions or few long rows are left to the tiles, which then have as little to read.
 static bool streams(int dtype, const void* big, int64_t ldb, int64_t S, int64_t R, int64_t K) {
-  return !direct(dtype, big, ldb, K) && S <= STREAM_SHORT && R >= 4 * S && R >= 256 && K >= 256;
+  return (dtype == D_F32 || !direct(dtype, big, ldb, K)) && S <= STREAM_SHORT && R >= 4 * S && R >= 256 && K >= 256;
 }
 
 static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big_x, void* ws, int64_t ws_bytes, int64_t* need) {
@@ -53,14 +60,15 @@ static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big
   const int64_t R = big_x ? a.M : a.N, S = big_x ? a.N : a.M;
   const void *big = big_x ? a.x : a.w, *small = big_x ? a.w : a.x;
   const int64_t ldb = big_x ? a.ldx : a.ldw, lds = big_x ? a.ldw : a.ldx;
-  Mat img = image_of(c, a.dtype, S, a.K);
+  const int image = a.dtype == D_F32 ? D_PL3 : a.dtype;
+  Mat img = image_of(c, image, S, a.K);
   int kchunk;
   const int slices = stream_slices(R, S, a.K, &kchunk);
   const int64_t n8 = round_up8(a.N);
   float* slabs = c.take<float>(slices * a.M * n8);
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
-  SCL_TRY(pack_image(ctx, st, a.dtype, small, lds, false, S, a.K, &img));
+  SCL_TRY(pack_image(ctx, st, a.dtype, image, small, lds, false, S, a.K, &img));
   SCL_TRY(stream_product(ctx, st, a.dtype, big, ldb, R, img, S, a.K, slabs, a.M * n8, big_x ? n8 : 1, big_x ? 1 : n8));
   Product p;
   p.M = a.M; p.N = a.N; p.K = a.K;
@@ -83,20 +91,22 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
     if (streams(a.dtype, a.x, a.ldx, a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
   Carve c(ws);
-  const bool dx = direct(a.dtype, a.x, a.ldx, a.K), dw = direct(a.dtype, a.w, a.ldw, a.K);
+  const bool planes = a.dtype == D_F32 && planes_pay(a.M, a.N, a.K, (a.M + a.N) * a.K);
+  const int image = planes ? D_PL3 : a.dtype;
+  const bool dx = !planes && direct(a.dtype, a.x, a.ldx, a.K), dw = !planes && direct(a.dtype, a.w, a.ldw, a.K);
   Product p;
-  p.type = image_type(a.dtype);
+  p.type = image;
   p.out_type = p.res_type = a.dtype;
   p.M = a.M; p.N = a.N; p.K = a.K;
-  p.A = dx ? user_mat(a.x, a.ldx) : image_of(c, a.dtype, a.M, a.K);
-  p.B = dw ? user_mat(a.w, a.ldw) : image_of(c, a.dtype, a.N, a.K);
+  p.A = dx ? user_mat(a.x, a.ldx) : image_of(c, image, a.M, a.K);
+  p.B = dw ? user_mat(a.w, a.ldw) : image_of(c, image, a.N, a.K);
   p.slab_bytes = product_slab_bytes(a.M, a.N, a.K, 1, p.type, 0);
   if (p.slab_bytes) p.slabs = c.take<float>(p.slab_bytes / 4);
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
   if (a.M == 0 || a.N == 0) return SCLENS_OK;
-  if (!dx) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, false, a.M, a.K, &p.A));
-  if (!dw) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, false, a.N, a.K, &p.B));
+  if (!dx) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, false, a.M, a.K, &p.A));
+  if (!dw) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, false, a.N, a.K, &p.B));
   p.bias = a.bias;
   p.act = a.act;
   if (a.res) { p.res = user_mat(a.res, a.ldr); p.beta = 1.f; }
@@ -106,12 +116,12 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
 }
 
 // ------------------------------------------------------------------ linear, backward
-// dz in 16 bits: 64 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the
-// block's column sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
+// dz: 64 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the block's column
+// sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
 // pre-activation and the gradient that comes in already are. Bound by HBM: two reads and a write per element.
 constexpr int DZ_ROWS = 64;
 template <int T>
-__global__ __launch_bounds__(256) void k_dz16(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
+__global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
   __shared__ float L[16][132];
   const int64_t nb = (N + 127) / 128, mb = blockIdx.x / nb;
   const int64_t m0 = mb * DZ_ROWS, n0 = (blockIdx.x % nb) * 128;
@@ -161,8 +171,8 @@ __global__ __launch_bounds__(256) void k_dz16(Mat dy, Mat z, int act, int64_t M,
     part[mb * N + n0 + tid] = s;
   }
 }
-// fp32, a 64 x 64 block: the planes of dz (contraction over the columns), those of its transpose (over the rows) and the column sums
-__global__ __launch_bounds__(256) void k_dz32(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, Mat imgT, float* __restrict__ part) {
+// fp32 in planes, a 64 x 64 block: those of dz (contraction over the columns), those of its transpose (over the rows) and the column sums
+__global__ __launch_bounds__(256) void k_dz_planes(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, Mat imgT, float* __restrict__ part) {
   __shared__ float L[64][65];
   const int64_t nb = (N + 63) / 64, mb = blockIdx.x / nb;
   const int64_t m0 = mb * 64, n0 = (blockIdx.x % nb) * 64;
@@ -226,20 +236,23 @@ __global__ __launch_bounds__(256) void k_colsum_join(const float* __restrict__ p
 int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
   if (a.M > 0 && a.N > 0 && backward_is_small(a)) return backward_small(ctx, st, a);
   Carve c(ws);
-  const bool as_is = a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
-  const bool f32 = a.dtype == D_F32;
-  const int rows_per = f32 ? 64 : DZ_ROWS, cols_per = f32 ? 64 : 128;
+  // fp32 in planes if both products together gain by it (dz both ways, w and x are taken apart)
+  const bool planes = a.dtype == D_F32 && a.dx && a.dw && planes_pay(a.M, a.K, a.N, 2 * a.M * a.N / 2 + a.N * a.K) &&
+                      planes_pay(a.N, a.K, a.M, 2 * a.M * a.N / 2 + a.M * a.K);
+  const int image = planes ? D_PL3 : a.dtype;
+  const bool as_is = !planes && a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
+  const int rows_per = planes ? 64 : DZ_ROWS, cols_per = planes ? 64 : 128;
   const int64_t nmb = (a.M + rows_per - 1) / rows_per;
-  // 16 bits: dz, w and x feed both products as they lie (w and x with their rows across the contraction), through a padded copy if they
-  // are not on 16 bytes. fp32: three planes with the contraction contiguous, so dz both ways, w and x transposed.
+  // dz, w and x feed both products as they lie (w and x with their rows across the contraction), through a padded copy if they are not
+  // on 16 bytes. Planes: the contraction contiguous, so dz both ways, w and x transposed.
   Mat dz, dzT, wT, xT;
-  const bool w_as_is = direct(a.dtype, a.w, a.ldw, a.K), x_as_is = direct(a.dtype, a.x, a.ldx, a.K);
-  if (a.dx || (a.dw && !f32)) dz = as_is ? user_mat(a.dy, a.lddy) : image_of(c, a.dtype, a.M, a.N);
-  if (a.dx) wT = f32 ? image_of(c, a.dtype, a.K, a.N) : (w_as_is ? user_mat(a.w, a.ldw) : image_of(c, a.dtype, a.N, a.K));
-  if (a.dw && f32) dzT = image_of(c, a.dtype, a.N, a.M);
-  if (a.dw) xT = f32 ? image_of(c, a.dtype, a.K, a.M) : (x_as_is ? user_mat(a.x, a.ldx) : image_of(c, a.dtype, a.M, a.K));
+  const bool w_as_is = !planes && direct(a.dtype, a.w, a.ldw, a.K), x_as_is = !planes && direct(a.dtype, a.x, a.ldx, a.K);
+  if (a.dx || (a.dw && !planes)) dz = as_is ? user_mat(a.dy, a.lddy) : image_of(c, image, a.M, a.N);
+  if (a.dx) wT = planes ? image_of(c, image, a.K, a.N) : (w_as_is ? user_mat(a.w, a.ldw) : image_of(c, image, a.N, a.K));
+  if (a.dw && planes) dzT = image_of(c, image, a.N, a.M);
+  if (a.dw) xT = planes ? image_of(c, image, a.K, a.M) : (x_as_is ? user_mat(a.x, a.ldx) : image_of(c, image, a.M, a.K));
   float* part = a.db ? c.take<float>(std::max<int64_t>(1, nmb * a.N)) : nullptr;
-  const int type = image_type(a.dtype);
+  const int type = image;
   const int64_t slab_dx = a.dx ? product_slab_bytes(a.M, a.K, a.N, 1, type, 0) : 0;
   const int64_t slab_dw = a.dw ? product_slab_bytes(a.N, a.K, a.M, 1, type, 0) : 0;
   const int64_t slab = std::max(slab_dx, slab_dw);
@@ -247,15 +260,16 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
 
-  if (a.M > 0 && a.N > 0 && (a.db || (a.dw && f32) || ((a.dx || a.dw) && !as_is))) {
+  if (a.M > 0 && a.N > 0 && (a.db || (a.dw && planes) || ((a.dx || a.dw) && !as_is))) {
     const int64_t blocks = nmb * ((a.N + cols_per - 1) / cols_per);
     if (blocks > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
     Mat img = as_is ? Mat() : dz;
     const dim3 grid((unsigned)blocks), blk(256);
-    if (f32) hipLaunchKernelGGL(k_dz32, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
-    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_dz16<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    else hipLaunchKernelGGL(k_dz16<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    if (planes) hipLaunchKernelGGL(k_dz_planes, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
+    else if (a.dtype == D_F32) hipLaunchKernelGGL(k_dz<D_F32>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_dz<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else hipLaunchKernelGGL(k_dz<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
     SCL_HIP(ctx, hipGetLastError());
   }
   if (a.db && a.N > 0) {
@@ -271,21 +285,21 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   p.slabs = slabs;
   p.slab_bytes = slab;
   if (a.dx && a.M > 0 && a.K > 0) {
-    if (f32) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, true, a.K, a.N, &wT));
-    else if (!w_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, a.w, a.ldw, false, a.N, a.K, &wT));
-    wT.across = !f32;
+    if (planes) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, true, a.K, a.N, &wT));
+    else if (!w_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, false, a.N, a.K, &wT));
+    wT.across = !planes;
     p.M = a.M; p.N = a.K; p.K = a.N;
     p.A = dz; p.B = wT;
     p.out = user_mat(a.dx, a.lddx);
     SCL_TRY(product(ctx, st, p));
   }
   if (a.dw && a.N > 0 && a.K > 0) {
-    if (f32) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, true, a.K, a.M, &xT));
-    else if (!x_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, a.x, a.ldx, false, a.M, a.K, &xT));
-    xT.across = !f32;
+    if (planes) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, true, a.K, a.M, &xT));
+    else if (!x_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, false, a.M, a.K, &xT));
+    xT.across = !planes;
     p.M = a.N; p.N = a.K; p.K = a.M;
-    p.A = f32 ? dzT : dz;
-    p.A.across = !f32;
+    p.A = planes ? dzT : dz;
+    p.A.across = !planes;
     p.B = xT;
     p.out = user_mat(a.dw, a.lddw);
     SCL_TRY(product(ctx, st, p));
@@ -397,16 +411,17 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   const int64_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
   // 16-bit inputs: x, A and b A + c A A between the products are fp16 under power-of-two scales from the bound of the singular values
   // (11 bits: eight times finer than bf16, so that what five steps amplify stays below the rounding of a bf16 result). fp32 inputs:
-  // three bf16 planes, exact.
-  const bool f32 = a.dtype == D_F32;
-  const int IT = f32 ? D_PL3 : D_F16, img_dtype = f32 ? D_F32 : D_F16;
+  // fp32, as it is or as three bf16 planes, exact.
+  const bool wide = a.dtype == D_F32;
+  const bool f32 = wide && planes_pay(m, n, m, 0, (int)a.batch) && planes_pay(m, m, n, 0, (int)a.batch, 1);  // planes
+  const int IT = f32 ? D_PL3 : (wide ? D_F32 : D_F16), img_dtype = IT;
   Carve c(ws);
   const int64_t elems = m * n;
   const int nparts = (int)std::min<int64_t>(1024, std::max<int64_t>(1, elems / 8192));
   double* part = c.take<double>(a.batch * nparts);
   Mat X[2], XT[2];
   for (int i = 0; i < (a.steps > 1 ? 2 : 1); ++i) {
-    // fp32: x and its transpose, so that every product has the contraction contiguous; 16 bits: x as it lies in memory
+    // planes: x and its transpose, so that every product has the contraction contiguous; else x as it lies in memory
     X[i] = f32 ? image_of(c, img_dtype, m, n, a.batch) : image_of(c, img_dtype, a.rows, a.cols, a.batch);
     if (f32) XT[i] = image_of(c, img_dtype, n, m, a.batch);
   }
@@ -423,7 +438,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   const int64_t tiles = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
   if (tiles > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: too many elements");
   double bound = 1.0;
-  double s_x = f32 ? 1.0 : pow2_scale(bound);
+  double s_x = wide ? 1.0 : pow2_scale(bound);
   {
     const dim3 g1((unsigned)nparts, (unsigned)a.batch), g2((unsigned)tiles, (unsigned)a.batch), blk(256);
     const Mat i0 = tall && f32 ? XT[0] : X[0], i1 = tall && f32 ? X[0] : XT[0];
@@ -432,7 +447,8 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, static_cast<const Elem<T>::type*>(a.x), a.sx, a.ldx, a.rows, a.cols, tpr, part); \
     hipLaunchKernelGGL((k_orth_start<T, I>), g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
   } while (0)
-    if (a.dtype == D_F32) SCL_START(D_F32, D_PL3);
+    if (f32) SCL_START(D_F32, D_PL3);
+    else if (wide) SCL_START(D_F32, D_F32);
     else if (a.dtype == D_BF16) SCL_START(D_BF16, D_F16);
     else SCL_START(D_F16, D_F16);
 #undef SCL_START
@@ -443,9 +459,9 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     const bool last = t + 1 == a.steps;
     const Mat &x = X[t & 1], &xt = XT[t & 1];
     const double next = step_bound(ca, cb, cc, bound);
-    const double s_a = f32 ? 1.0 : pow2_scale(bound * bound);
-    const double s_p = f32 ? 1.0 : pow2_scale(std::fabs(cb) * bound * bound + std::fabs(cc) * bound * bound * bound * bound);
-    const double s_n = f32 || last ? 1.0 : pow2_scale(next);
+    const double s_a = wide ? 1.0 : pow2_scale(bound * bound);
+    const double s_p = wide ? 1.0 : pow2_scale(std::fabs(cb) * bound * bound + std::fabs(cc) * bound * bound * bound * bound);
+    const double s_n = wide || last ? 1.0 : pow2_scale(next);
     Product p;
     p.type = IT;
     p.batch = (int)a.batch;
@@ -468,7 +484,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     p.alpha = (float)(cc * s_p / (s_a * s_a));
     p.beta = (float)(cb * s_p / s_a);
     SCL_TRY(product(ctx, st, p));
-    // x <- a x + P x (16 bits, tall: the transpose of it, a x + x P, in the layout of the caller)
+    // x <- a x + P x (no planes, tall: the transpose of it, a x + x P, in the layout of the caller)
     p.symmetric = 0;
     p.res = x;
     p.alpha = (float)(s_n / (s_p * s_x));
