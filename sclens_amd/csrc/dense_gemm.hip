@@ -90,6 +90,7 @@ __device__ __forceinline__ float recompute_f32(const unsigned short* A, const un
     const float a = (bf16_to_f32(A[k]) + bf16_to_f32(A[k + planeA])) + bf16_to_f32(A[k + 2 * planeA]);
     const float b = (bf16_to_f32(B[k]) + bf16_to_f32(B[k + planeB])) + bf16_to_f32(B[k + 2 * planeB]);
     s = fmaf(a, b, s);
+    if (s != s) break;
   }
   return s;
 }

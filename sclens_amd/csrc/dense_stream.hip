@@ -241,7 +241,7 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
           const unsigned short* y = static_cast<const unsigned short*>(a.small.p) + s * a.small.ld;
           v = 0.f;
           const int64_t k1 = min(a.K, (int64_t)t1 * 64);
-          for (int64_t k = (int64_t)t0 * 64; k < k1; ++k)
+          for (int64_t k = (int64_t)t0 * 64; k < k1 && v == v; ++k)
             v = fmaf(x[k], (bf16_to_f32(y[k]) + bf16_to_f32(y[k + a.small.plane])) + bf16_to_f32(y[k + 2 * a.small.plane]), v);
         }
         out[r * a.sr + s * a.ss] = v;

@@ -84,6 +84,38 @@ def test_linear_whole_numbers_are_exact(dense, M, K, N, dtype):
     assert torch.equal(dense.linear(x, w), (x.double() @ w.double().t()).float().to(dtype))
 
 
+# sizes that reach every tile (256, 192, 128 with two and four stages, 64), split contractions with few results, planes of fp32 (the
+# second and third), rows that do not start on 16 bytes, streams past a short side
+LARGE = [(4096, 72, 4096), (4096, 1024, 4096), (4100, 1030, 4090), (2900, 200, 2950), (8192, 136, 1024), (2048, 1032, 2048), (1024, 264, 1040),
+         (300, 8200, 300), (130, 4104, 4096), (3000, 1000, 100), (60, 2001, 3000), (5000, 640, 128)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", LARGE)
+def test_linear_whole_numbers_large(dense, M, K, N, dtype):
+    g = gen_for("large", M, K, N)
+    x, w, b, r = ints(g, (M, K), dtype, 1), ints(g, (N, K), dtype, 1), ints(g, (N,), dtype, 9), ints(g, (M, N), dtype, 9)
+    z = x.double() @ w.double().t() + b.double()
+    y, pre = dense.linear(x, w, bias=b, residual=r, activation="relu", save_preact=True)
+    assert torch.equal(pre, z.float().to(dtype))
+    assert torch.equal(y, (z.clamp(min=0) + r.double()).float().to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(4096, 4096, 4096), (2048, 1032, 1030), (1000, 2001, 1500), (4100, 520, 3000), (64, 4096, 2048)])
+def test_backward_whole_numbers_large(dense, M, K, N, dtype):
+    g = gen_for("blarge", M, K, N)
+    x, w, dy, z = ints(g, (M, K), dtype, 1), ints(g, (N, K), dtype, 1), ints(g, (M, N), dtype, 1), ints(g, (M, N), dtype, 3)
+    dz = dy.double() * (z.double() > 0)
+    dx, dw, db = dense.linear_backward(dy, x, w, preact=z, activation="relu")
+    assert torch.equal(dx, (dz @ w.double()).float().to(dtype))
+    assert torch.equal(dw, (dz.t().contiguous() @ x.double()).float().to(dtype))
+    assert torch.equal(db, dz.sum(0).float().to(dtype))
+    # parts of it give the same bits
+    assert torch.equal(dense.linear_backward(dy, None, w, preact=z, activation="relu", need_weight=False, need_bias=False)[0].float(), dx.float())
+    assert torch.equal(dense.linear_backward(dy, x, None, preact=z, activation="relu", need_x=False)[1].float(), dw.float())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (2, 64, 64), (5, 7, 9), (65, 63, 66), (127, 128, 129), (200, 93, 50), (257, 520, 255),
                                    (513, 1100, 770), (1030, 1032, 1028), (2049, 129, 8), (8, 2000, 700), (1, 513, 514), (3000, 16, 1)])
@@ -204,7 +236,7 @@ def test_gradient_against_differences(dense, act):
 def test_linear_extremes(dense, dtype):
     """infinities, NaN and the type's largest values reach exactly the results that contain them"""
     g = gen_for("extreme")
-    for M, K, N in ((70, 96, 90), (1, 96, 90), (300, 300, 300)):
+    for M, K, N in ((70, 96, 90), (1, 96, 90), (300, 300, 300), (2048, 264, 2048), (3000, 520, 40), (40, 520, 3000), (4096, 1024, 4096)):
         x, w = ints(g, (M, K), dtype, 3), ints(g, (N, K), dtype, 3)
         w[5] = 1
         w[6] = 0
@@ -213,8 +245,7 @@ def test_linear_extremes(dense, dtype):
             x[33, 7] = math.nan
             x[34, 2], x[34, 9] = math.inf, -math.inf
         y = dense.linear(x, w).double()
-        want = x.double().cpu() @ w.double().cpu().t()
-        want = want.to(y.device)
+        want = x.double() @ w.double().t()
         assert torch.equal(torch.isnan(y), torch.isnan(want))
         assert torch.equal(torch.nan_to_num(y, nan=0.0, posinf=1e300, neginf=-1e300), torch.nan_to_num(want.to(dtype).double(), nan=0.0, posinf=1e300, neginf=-1e300))
     # the largest value survives a product with one; twice it overflows
@@ -316,7 +347,7 @@ def orth_bound(x, schedule, dtype):
 
 
 ORTH = [(1, 1, 1), (1, 1, 50), (1, 50, 1), (3, 4, 4), (20, 40, 40), (2, 33, 64), (1, 64, 65), (1, 66, 63), (4, 93, 93), (2, 128, 100), (1, 5, 3000),
-        (1, 3001, 40), (1, 5000, 64), (1, 2000, 100), (1, 130, 700), (1, 700, 130), (2, 256, 512), (1, 515, 300), (1, 1024, 520), (1, 65, 4100)]
+        (1, 3001, 40), (1, 5000, 64), (1, 2000, 100), (1, 130, 700), (1, 700, 130), (2, 256, 512), (1, 515, 300), (1, 1024, 520), (1, 65, 4100), (1, 2048, 1100)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -463,6 +494,21 @@ def test_captured_and_replayed(dense):
         for gr, res in graphs:
             for a, b in zip(res, eager):
                 assert torch.equal(a, b), rep
+
+
+def test_orthogonalize_in_planes(dense):
+    """fp32 of the size that is taken apart into three planes"""
+    g = gen_for("planes")
+    for rows, cols in ((2100, 2304), (2304, 2100)):
+        x = torch.randn(rows, cols, generator=g, device="cuda")
+        off = (dense.orthogonalize(x).double() - orth64(x, UPDATE)).norm().cpu()
+        # the bound of orth_bound without the singular values of 2100 x 2304: x0 has norm 1 and singular values below
+        # (sqrt(rows) + sqrt(cols)) 1.05 / |x|_F; per step L <= 3.4445, at most (2 u + acc) of norms below sqrt(2100) 1.21
+        u, acc = 2.0 ** -23, 2 * (math.sqrt(2304) + 3) * 2.0 ** -24
+        e = u
+        for _ in range(5):
+            e = 3.4445 * e + (2 * u + acc) * (3.4445 + 2 * (4.775 + 2.0315 * 2)) * 1.21 * math.sqrt(2100)
+        assert off <= e, (off, e)
 
 
 def test_two_threads_at_once(dense):
