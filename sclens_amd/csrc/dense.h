@@ -19,7 +19,7 @@ struct Mat {
   int pad = 0;  // rows / columns up to the next multiple of 8 exist and are written as zeros (images of the library)
 };
 
-// C[b] = epilogue(alpha * A[b] B[b]'), A [M][K], B [N][K], K contiguous.
+// C[b] = epilogue(alpha * A[b] B[b]'), A [M][K], B [N][K], the contraction contiguous or (Mat::across) the rows.
 struct Product {
   int type = D_BF16;  // of the operands; D_PL3: fp32 as three bf16 planes each, six products per term
   Mat A, B;
@@ -54,6 +54,9 @@ int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t
 static inline int64_t image_ld(int64_t K) { return round_up(K > 0 ? K : 1, 64); }
 static inline int64_t image_elems(int64_t rows, int64_t K) { return round_up(rows, 8) * image_ld(K); }
 int pack_image(Ctx* ctx, hipStream_t st, int dtype, int image, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img);
+// two of equal K, not transposed, in one launch; an image that is nullptr is left out
+int pack_pair(Ctx* ctx, hipStream_t st, int dtype, int image, const void* a, int64_t lda, int64_t rows_a, Mat* img_a, const void* b, int64_t ldb,
+              int64_t rows_b, Mat* img_b, int64_t K);
 
 struct LinearArgs {
   int dtype = D_F32, act = ACT_NONE;

@@ -105,8 +105,7 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
   *need = c.used;
   if (c.used > ws_bytes) return no_room(ctx, c.used);
   if (a.M == 0 || a.N == 0) return SCLENS_OK;
-  if (!dx) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, false, a.M, a.K, &p.A));
-  if (!dw) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, false, a.N, a.K, &p.B));
+  SCL_TRY(pack_pair(ctx, st, a.dtype, image, a.x, a.ldx, a.M, dx ? nullptr : &p.A, a.w, a.ldw, a.N, dw ? nullptr : &p.B, a.K));
   p.bias = a.bias;
   p.act = a.act;
   if (a.res) { p.res = user_mat(a.res, a.ldr); p.beta = 1.f; }
@@ -227,6 +226,7 @@ __global__ __launch_bounds__(256) void k_colsum_join(const float* __restrict__ p
   const int64_t col = (int64_t)blockIdx.x * 64 + c;
   double s = 0.0;
   if (col < N)
+#pragma unroll 8
     for (int64_t b = g; b < nmb; b += 4) s += (double)part[b * N + col];
   S[g][c] = s;
   __syncthreads();
@@ -279,6 +279,10 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
     else hipLaunchKernelGGL(k_colsum_join<D_F16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
     SCL_HIP(ctx, hipGetLastError());
   }
+  if (!planes && a.K > 0) {
+    const bool copy_w = a.dx && a.M > 0 && !w_as_is, copy_x = a.dw && a.N > 0 && !x_as_is;
+    SCL_TRY(pack_pair(ctx, st, a.dtype, image, a.w, a.ldw, a.N, copy_w ? &wT : nullptr, a.x, a.ldx, a.M, copy_x ? &xT : nullptr, a.K));
+  }
   Product p;
   p.type = type;
   p.out_type = p.res_type = a.dtype;
@@ -286,7 +290,6 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   p.slab_bytes = slab;
   if (a.dx && a.M > 0 && a.K > 0) {
     if (planes) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, true, a.K, a.N, &wT));
-    else if (!w_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, false, a.N, a.K, &wT));
     wT.across = !planes;
     p.M = a.M; p.N = a.K; p.K = a.N;
     p.A = dz; p.B = wT;
@@ -295,7 +298,6 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   }
   if (a.dw && a.N > 0 && a.K > 0) {
     if (planes) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, true, a.K, a.M, &xT));
-    else if (!x_as_is) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.x, a.ldx, false, a.M, a.K, &xT));
     xT.across = !planes;
     p.M = a.N; p.N = a.K; p.K = a.M;
     p.A = planes ? dzT : dz;
@@ -308,20 +310,28 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
 }
 
 // ------------------------------------------------------------------ orthogonalize
-// |g|_F^2 of each matrix: partial sums in fp64 (fp32 squares of large entries overflow), added in a fixed order by whoever needs them
+// |g|_F^2 of each matrix: partial sums in fp64 (fp32 squares of large entries overflow), added in a fixed order by whoever needs them.
+// Bound by reading g: 8 columns per lane, tpr lanes to a row, four rows' loads on their way together.
 template <int T>
-__global__ __launch_bounds__(256) void k_sumsq(const typename Elem<T>::type* __restrict__ x, int64_t batch, int64_t ld, int64_t rows, int64_t cols,
-                                               int tpr, double* __restrict__ part) {
+__global__ __launch_bounds__(256) void k_sumsq(Mat src, int64_t rows, int64_t cols, int tpr, double* __restrict__ part) {
   __shared__ double S[256];
-  const int tid = threadIdx.x, tr = tid / tpr, tc = tid % tpr, rpb = 256 / tpr;
-  const auto* p = x + (int64_t)blockIdx.y * batch;
+  const int tid = threadIdx.x, tr = tid / tpr, tc = (tid % tpr) * 8, rpb = 256 / tpr;
+  const int64_t base = (int64_t)blockIdx.y * src.batch, step = (int64_t)gridDim.x * rpb;
   double s = 0.0;
-  for (int64_t r = (int64_t)blockIdx.x * rpb + tr; r < rows; r += (int64_t)gridDim.x * rpb)
+  for (int64_t r = (int64_t)blockIdx.x * rpb + tr; r < rows; r += 4 * step)
     for (int64_t c = tc; c < cols; c += 8 * tpr) {
+      const int n = (int)min((int64_t)8, cols - c);
+      Raw8<T> q[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double v = c + e * tpr < cols ? (double)Elem<T>::ld(p + r * ld + c + e * tpr) : 0.0;
-        s += v * v;
+      for (int i = 0; i < 4; ++i)
+        if (r + i * step < rows) q[i].load(src, base + (r + i * step) * src.ld + c, n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r + i * step >= rows) continue;
+        float v[8];
+        q[i].get(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
       }
     }
   S[tid] = s;
@@ -338,20 +348,24 @@ template <int T, int IT>
 __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64_t cols, const double* __restrict__ part, int nparts, double eps,
                                                     double scale, Mat img, Mat imgT) {
   __shared__ float L[64][65];
-  __shared__ double factor;
+  __shared__ double S[4];
   const int64_t nb = (cols + 63) / 64, b = blockIdx.y;
   const int64_t m0 = (blockIdx.x / nb) * 64, n0 = (blockIdx.x % nb) * 64;
   const int tid = threadIdx.x, cc = (tid & 7) * 8;
-  if (tid < 64) {
-    double s = 0.0;
-    for (int i = tid; i < nparts; i += 64) s += part[b * nparts + i];
-    for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w);
-    if (tid == 0) factor = scale / (sqrt(s) + eps);
-  }
-  __syncthreads();
-  const double f = factor;
   const int64_t col = n0 + cc;
   const int nin = (int)max((int64_t)0, min((int64_t)8, cols - col));
+  Raw8<T> q[2];  // on their way while the norm is added up
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t row = m0 + i * 32 + (tid >> 3);
+    if (row < rows && nin > 0) q[i].load(src, b * src.batch + row * src.ld + col, nin);
+  }
+  double s = 0.0;
+  for (int i = tid; i < nparts; i += 256) s += part[b * nparts + i];
+  for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w);
+  if ((tid & 63) == 0) S[tid >> 6] = s;
+  __syncthreads();
+  const double f = scale / (sqrt((S[0] + S[1]) + (S[2] + S[3])) + eps);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int lr = i * 32 + (tid >> 3);
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     if (row < rows && nin > 0) {
-      load8<T>(src, b * src.batch + row * src.ld + col, nin, v);
+      q[i].get(v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = e < nin ? (float)((double)v[e] * f) : 0.f;
     }
@@ -434,7 +448,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
 
   const Mat src = user_mat(a.x, a.ldx, a.sx), dst = user_mat(a.y, a.ldy, a.sy);
   int tpr = 1;
-  while (tpr < 256 && tpr < a.cols) tpr *= 2;
+  while (tpr < 256 && 8 * tpr < a.cols) tpr *= 2;
   const int64_t tiles = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
   if (tiles > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: too many elements");
   double bound = 1.0;
@@ -444,7 +458,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     const Mat i0 = tall && f32 ? XT[0] : X[0], i1 = tall && f32 ? X[0] : XT[0];
 #define SCL_START(T, I)                                                                                                             \
   do {                                                                                                                              \
-    hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, static_cast<const Elem<T>::type*>(a.x), a.sx, a.ldx, a.rows, a.cols, tpr, part); \
+    hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, src, a.rows, a.cols, tpr, part);                                                 \
     hipLaunchKernelGGL((k_orth_start<T, I>), g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
   } while (0)
     if (f32) SCL_START(D_F32, D_PL3);
