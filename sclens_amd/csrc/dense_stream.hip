@@ -172,8 +172,9 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto stage = [&](Chunk<T>(&n)[2][2], int t) {
     const int cur = (t - t0) & 1;
-    // this stage has landed on all sides; only the fetch of the stage after it may still be on its way
-    if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    // this stage has landed on all sides; only the fetch of the stage after it may still be on its way (a stage that ends inside its 64
+    // columns is fetched with fewer loads, so they cannot be counted off)
+    if (t + 1 < t1 && (int64_t)(t + 2) * 64 <= a.K) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     u16x8 A[2][2][NP];
 #pragma unroll

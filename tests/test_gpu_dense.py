@@ -553,3 +553,17 @@ def test_device_refusals_leave_no_error_behind(dense):
     with pytest.raises(Exception):
         dense.orthogonalize(x, coefficients=[(50.0, 0.0, 0.0)] * 20)
     assert torch.equal(dense.linear(x, x), torch.full((4, 4), 4.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("S", [24, 40, 120])
+@pytest.mark.parametrize("K", [257, 321, 415, 449, 1025, 2047])
+def test_stream_whose_last_stage_is_short(dense, K, S, dtype):
+    """one short side, rows off 16 bytes: the last stage of the contraction holds 1, 31, 63 or 2 x 32 - 1 columns"""
+    g = gen_for("stream tail", K, S)
+    R = 1 + 2 ** 27 // (K * S)
+    x, w = ints(g, (R, K), dtype, 1), ints(g, (S, K), dtype, 1)
+    ref = x.double() @ w.double().t()
+    for _ in range(2):
+        assert torch.equal(dense.linear(x, w), ref.float().to(dtype))
+        assert torch.equal(dense.linear(w, x), ref.t().float().to(dtype))
