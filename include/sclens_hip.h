@@ -215,13 +215,15 @@ int sclens_hip_get_denoised_f32(sclens_hip_ctx* ctx, const float* pca_n1, int64_
  * (a hipStream_t of the context's device; NULL = that device's default stream, sclens_hip_stream(ctx) = the context's own), nothing
  * synchronises or allocates, and a call can be captured into a graph. Matrices are ROW-MAJOR with the given leading dimension (elements
  * between rows, at least the row's length), any alignment of whole elements; outputs must not overlap inputs. Inputs are read, outputs
- * written, in the element type `dtype` (SCLENS_DTYPE_*); sums are held in fp32 and rounded once. fp32 products are formed from three
- * bf16 pieces per operand (24 bits, exact) on the matrix cores, whatever the option "precision" says.
+ * written, in the element type `dtype` (SCLENS_DTYPE_*); sums are held in fp32 and rounded once. fp32 products run on
+ * the fp32 matrix cores or, where that is faster, from three bf16 pieces per operand (24 bits, exact; what is left out of a term is below
+ * its fp32 rounding), whatever the option "precision" says.
  * Workspace: device memory of the caller, 256-byte aligned, *ws_bytes its size. A call that needs more launches nothing, stores what it
  * needs in *ws_bytes and returns SCLENS_ERR_WORKSPACE; it may be reused or freed (in stream order) when the call's work is done, so two
  * calls that may overlap -- other streams, graphs replayed side by side -- need one each. NULL with *ws_bytes = 0 is a size query, or
  * the call itself when it needs none.
- * Any size may be 0: an empty sum is 0.
+ * Any size may be 0: an empty sum is 0. Rows of more than 2^25 elements (an fp32 dx: N of more than 2^24) are refused with SCLENS_ERR_ARG
+ * where the product runs in tiles (more than 16 rows of x, no short side to stream past); there may be any number of rows.
  *
  * linear: y = act(x w' + bias) + residual. x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]; preact [M][N] or
  * NULL receives the argument of the activation, which linear_backward reads. */

@@ -632,8 +632,9 @@ namespace {
 
 struct Plan { int tile, ksplit, kchunk, tm, tn; int64_t tiles; double us; };
 
-// a lane's place below its tile's base has 32 bits: 64 rows of 2^25 elements, 256 of 2^23
-constexpr int64_t MAX_LD = (int64_t)1 << 25, MAX_LD_BIG = (int64_t)1 << 22;
+// a lane's place below its tile's base has 32 bits: the small tile's 64 rows (across: a stage's 64 or 32
+// columns) have at most MAX_CONTRACTION elements, in fp32 MAX_CONTRACTION_F32, a large tile's 256 at most MAX_LD_BIG
+constexpr int64_t MAX_LD_BIG = (int64_t)1 << 22;
 
 struct TileKind {
   int bm;            // the tile is bm x bm
@@ -732,7 +733,9 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return SCLENS_OK;
   const int64_t slab = p.slabs ? product_slab_bytes(p.M, p.N, p.K, p.batch, p.type, p.symmetric) : 0;
   const Plan pl = plan_product(p.M, p.N, p.K, p.batch, p.type, p.symmetric, p.slabs && slab <= p.slab_bytes);
-  if (std::max(p.A.ld, p.B.ld) > MAX_LD) return ctx->fail(SCLENS_ERR_ARG, "product: a contraction of more than 2^25 columns");
+  for (const Mat* m : {&p.A, &p.B})
+    if (m->ld > (p.type == D_F32 && !m->across ? MAX_CONTRACTION_F32 : MAX_CONTRACTION))
+      return ctx->fail(SCLENS_ERR_ARG, "product: an operand's rows are too long");
   if (pl.tiles > 0x7fffffff || p.batch > 65535) return ctx->fail(SCLENS_ERR_ARG, "product: too many tiles");
   ProdArgs g{};
   g.p = p;

@@ -91,7 +91,8 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
     if (streams(a.dtype, a.x, a.ldx, a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
   Carve c(ws);
-  const bool planes = a.dtype == D_F32 && planes_pay(a.M, a.N, a.K, (a.M + a.N) * a.K);
+  if (a.K > MAX_CONTRACTION && a.M > 0 && a.N > 0) return ctx->fail(SCLENS_ERR_ARG, "linear: more than 2^25 columns");
+  const bool planes = a.dtype == D_F32 && (a.K > MAX_CONTRACTION_F32 || planes_pay(a.M, a.N, a.K, (a.M + a.N) * a.K));
   const int image = planes ? D_PL3 : a.dtype;
   const bool dx = !planes && direct(a.dtype, a.x, a.ldx, a.K), dw = !planes && direct(a.dtype, a.w, a.ldw, a.K);
   Product p;
@@ -235,9 +236,11 @@ __global__ __launch_bounds__(256) void k_colsum_join(const float* __restrict__ p
 
 int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, int64_t ws_bytes, int64_t* need) {
   if (a.M > 0 && a.N > 0 && backward_is_small(a)) return backward_small(ctx, st, a);
+  if (a.N > (a.dtype == D_F32 && a.dx ? MAX_CONTRACTION_F32 : MAX_CONTRACTION) || a.K > MAX_CONTRACTION)
+    return ctx->fail(SCLENS_ERR_ARG, "linear_backward: more than 2^25 columns (2^24 in an fp32 dx)");
   Carve c(ws);
   // fp32 in planes if both products together gain by it (dz both ways, w and x are taken apart)
-  const bool planes = a.dtype == D_F32 && a.dx && a.dw && planes_pay(a.M, a.K, a.N, 2 * a.M * a.N / 2 + a.N * a.K) &&
+  const bool planes = a.dtype == D_F32 && a.dx && a.dw && a.M <= MAX_CONTRACTION && planes_pay(a.M, a.K, a.N, 2 * a.M * a.N / 2 + a.N * a.K) &&
                       planes_pay(a.N, a.K, a.M, 2 * a.M * a.N / 2 + a.M * a.K);
   const int image = planes ? D_PL3 : a.dtype;
   const bool as_is = !planes && a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
@@ -427,7 +430,9 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   // (11 bits: eight times finer than bf16, so that what five steps amplify stays below the rounding of a bf16 result). fp32 inputs:
   // fp32, as it is or as three bf16 planes, exact.
   const bool wide = a.dtype == D_F32;
-  const bool f32 = wide && planes_pay(m, n, m, 0, (int)a.batch) && planes_pay(m, m, n, 0, (int)a.batch, 1);  // planes
+  const bool f32 = wide && n <= MAX_CONTRACTION &&  // planes
+                   ((!tall && n > MAX_CONTRACTION_F32) || (planes_pay(m, n, m, 0, (int)a.batch) && planes_pay(m, m, n, 0, (int)a.batch, 1)));
+  if (m > MAX_CONTRACTION_F32 || (!tall && n > MAX_CONTRACTION)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: more than 2^25 columns");
   const int IT = f32 ? D_PL3 : (wide ? D_F32 : D_F16), img_dtype = IT;
   Carve c(ws);
   const int64_t elems = m * n;

@@ -567,3 +567,39 @@ def test_stream_whose_last_stage_is_short(dense, K, S, dtype):
     for _ in range(2):
         assert torch.equal(dense.linear(x, w), ref.float().to(dtype))
         assert torch.equal(dense.linear(w, x), ref.t().float().to(dtype))
+
+
+def test_long_contractions(dense):
+    """rows of more than 2^24 elements, fp32 and 16 bits: the last columns of the last rows are read"""
+    K = 2 ** 24 + 72
+    for dtype, M in ((F32, 70), (BF16, 80)):
+        x = torch.zeros(M, K, dtype=dtype, device="cuda")
+        x[:, 5], x[:, -1] = 1, 2
+        x[-1, -2] = 3
+        w = torch.zeros(M - 2, K, dtype=dtype, device="cuda")
+        w[:, 5], w[:, -1] = torch.arange(M - 2).to("cuda", dtype), 4
+        w[-1, -2] = 7
+        ref = (torch.arange(M - 2, dtype=torch.float64) + 8).repeat(M, 1)
+        ref[-1, -1] += 21
+        assert torch.equal(dense.linear(x, w).cpu(), ref.to(dtype))
+        del x, w
+
+
+def test_rows_too_long_are_refused_before_anything_runs(dense):
+    """size queries of the C entries: no memory is named, nothing is launched"""
+    import ctypes as C
+
+    ctx = dense.Context(0)
+    lib, n, some = ctx.lib, C.c_int64(0), 1 << 20  # (an address that is never read)
+    long = 2 ** 25 + 64
+    assert lib.sclens_hip_linear(ctx.h, None, 1, 200, 200, long, some, long, some, long, None, None, 200, 0, some, 200, None, 200, None, n) == 1
+    assert lib.sclens_hip_linear(ctx.h, None, 1, 200, 200, long - 64, some, long, some, long, None, None, 200, 0, some, 200, None, 200, None, n) == 8
+    assert n.value > 0
+    for dtype, N, rc in ((1, long, 1), (1, 2 ** 25, 8), (0, 2 ** 24 + 64, 1), (0, 2 ** 24, 8)):
+        n.value = 0
+        assert lib.sclens_hip_linear_backward(ctx.h, None, dtype, 400, N, 500, some, N, some, 500, some, 500, None, N, 0, some, 500, some, 500,
+                                              some, None, n) == rc
+    coef = (C.c_double * 3)(1.5, -0.5, 0.0)
+    n.value = 0
+    assert lib.sclens_hip_orthogonalize(ctx.h, None, 1, 1, 200, long, some, 0, long, some, 0, long, 1, coef, 1e-7, None, n) == 1
+    assert "more than" in lib.sclens_hip_last_error(ctx.h).decode()
