@@ -540,20 +540,25 @@ int orthogonalize(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t
   double bound = 1.0;
   for (int t = 0; t < a.steps; ++t) {
     bound = step_bound(a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2], bound);
-    if (!(bound < 1e15)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: these coefficients let the singular values grow without bound");
+    // (fp32 holds its fourth power, the entries of A A)
+    if (!(bound < 1e9)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: these coefficients let the singular values grow without bound");
   }
-  const int64_t chunk = 32768;  // matrices per launch (a grid holds 65535 in y)
-  OrthArgs b = a;
-  b.batch = std::min(a.batch, chunk);
-  for (int64_t b0 = 0; b0 < a.batch; b0 += chunk) {
-    b.batch = std::min(chunk, a.batch - b0);
-    const int size = a.dtype == D_F32 ? 4 : 2;
-    b.x = static_cast<const char*>(a.x) + b0 * a.sx * size;
-    b.y = static_cast<char*>(a.y) + b0 * a.sy * size;
-    int64_t n1 = 0;
-    const int rc = orth_is_small(b) ? orth_small(ctx, st, b, ws, ws_bytes, &n1) : orth_chunk(ctx, st, b, ws, ws_bytes, &n1);
-    *need = std::max(*need, n1);
-    if (rc != SCLENS_OK) return rc;
+  // 32768 matrices per launch (a grid holds 65535 in y). The last, shorter run may take another path than the others: what all of them
+  // need is settled before the first one is launched.
+  const int64_t chunk = 32768, size = a.dtype == D_F32 ? 4 : 2;
+  for (int pass = a.batch > chunk ? 0 : 1; pass < 2; ++pass) {
+    for (int64_t b0 = 0; b0 < a.batch; b0 += chunk) {
+      OrthArgs b = a;
+      b.batch = std::min(chunk, a.batch - b0);
+      b.x = static_cast<const char*>(a.x) + b0 * a.sx * size;
+      b.y = static_cast<char*>(a.y) + b0 * a.sy * size;
+      const int64_t room = pass == 0 ? -1 : ws_bytes;  // -1: the size only
+      int64_t n1 = 0;
+      const int rc = orth_is_small(b) ? orth_small(ctx, st, b, ws, room, &n1) : orth_chunk(ctx, st, b, ws, room, &n1);
+      *need = std::max(*need, n1);
+      if (rc != SCLENS_OK && (pass == 1 || rc != SCLENS_ERR_WORKSPACE)) return rc;
+    }
+    if (*need > ws_bytes) return no_room(ctx, *need);
   }
   return SCLENS_OK;
 }

@@ -603,3 +603,57 @@ def test_rows_too_long_are_refused_before_anything_runs(dense):
     n.value = 0
     assert lib.sclens_hip_orthogonalize(ctx.h, None, 1, 1, 200, long, some, 0, long, some, 0, long, 1, coef, 1e-7, None, n) == 1
     assert "more than" in lib.sclens_hip_last_error(ctx.h).decode()
+
+
+def test_workspace_of_many_matrices_is_asked_for_before_the_first_is_written(dense):
+    """32 769 matrices: the last one alone takes another path than the runs of 32 768, and needs scratch that they do not"""
+    import ctypes as C
+
+    g = gen_for("many")
+    B, rows, cols = 32769, 3, 1100
+    x = torch.randn(B, rows, cols, generator=g, device="cuda").to(F16)
+    y = torch.full_like(x, 7.0)
+    ctx = dense.Context(0)
+    coef, n = (C.c_double * 15)(*[v for t in UPDATE for v in t]), C.c_int64(0)
+
+    def call(ws):
+        return ctx.lib.sclens_hip_orthogonalize(ctx.h, torch.cuda.current_stream().cuda_stream, 2, B, rows, cols, x.data_ptr(), rows * cols, cols,
+                                                y.data_ptr(), rows * cols, cols, 5, coef, 1e-7, ws, n)
+
+    assert call(None) == 8 and n.value > 0
+    torch.cuda.synchronize()
+    assert (y == 7).all()
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    assert call(ws.data_ptr()) == 0
+    got = dense.orthogonalize(x)
+    assert torch.equal(got, y)
+    assert torch.equal(y[32768], dense.orthogonalize(x[32768]))
+    for i in (0, 1, 32766, 32767):  # alone they take the last one's path: sums in another order in fp64, one step of fp16 below 2
+        assert (y[i] - dense.orthogonalize(x[i])).abs().max() <= 2.0 ** -10
+
+
+def test_many_steps(dense):
+    """more steps than the single-launch kernels carry along: the tiled products take them"""
+    g = gen_for("many steps")
+    q = torch.linalg.qr(torch.randn(90, 40, generator=g, device="cuda").double().cpu())[0]
+    for dtype in TYPES:
+        x = (q * torch.linspace(1, 2, 40)).to("cuda", dtype).contiguous()
+        y = dense.orthogonalize(x, coefficients=UPDATE[:3] + [(1.875, -1.25, 0.375)] * 40)
+        off = (y.double().t() @ y.double() - torch.eye(40, device="cuda", dtype=torch.float64)).norm().item()
+        # Converged: the last step's x = a x + P x has the roundings of its 40 x 40 products (fp16 for 16-bit types) and of the result on
+        # it, each at most half a step of entries whose norm is sqrt(40): x' x is off by twice their sum, a = 1.875 and |P| <= 1.875
+        u = U[F32] if dtype is F32 else U[F16]
+        acc = 0 if dtype is not F32 else 2 * 40 * U[F32]
+        assert off <= 2 * math.sqrt(40) * (U[dtype] + 1.875 * 4 * (u + acc)), (dtype, off)
+
+
+def test_coefficients_that_grow(dense):
+    g = gen_for("growth")
+    x = torch.randn(2, 200, 150, generator=g, device="cuda")
+    for dtype in TYPES:
+        y = dense.orthogonalize(x.to(dtype), coefficients=[(1.0, 0.0, 1e4), (1e-4, 0.0, 0.0)] if dtype is F32 else [(1.0, 0.0, 0.0)])
+        assert torch.isfinite(y).all()
+    with pytest.raises(Exception, match="grow"):
+        dense.orthogonalize(x, coefficients=[(1e10, 0.0, 0.0)])
+    with pytest.raises(Exception, match="grow"):
+        dense.orthogonalize(x, coefficients=[(float("nan"), 0.0, 0.0)])
