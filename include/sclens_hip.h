@@ -7,13 +7,15 @@
  *   (A) the same five operations with the same host-array semantics (drop-in per call site), and
  *   (B) a session that keeps the count matrix, the scaled matrices, the Gram matrix and the
  *       eigenvectors resident in HBM for the whole sclens() call (what a `device_="hip"` branch of
- *       sclens() would call; see INTEGRATION.md for the Julia ccall shim).
+ *       sclens() would call; see INTEGRATION.md for the Julia ccall shim), and
+ *   (C) dense operators on device tensors beside it: a product with bias, activation and residual, its gradient, and the orthogonal
+ *       factor of a matrix (queued on the caller's stream, workspace of the caller, row-major; the rules stand with them).
  *
  * Conventions: plain pointers and sizes, no C++/torch types. Host matrices are COLUMN-MAJOR (Julia
  * layout) unless stated. Sparse input is CSC with 0-BASED int64 column pointers and int32 row indices
  * (Julia's SparseMatrixCSC{Float32,UInt32} minus one, scLENS.jl:103-117). All functions return 0 on
  * success or an SCLENS_ERR_* code and never throw; sclens_hip_last_error() gives the message.
- * Blocking calls; one host thread per context. The caller owns every host buffer; the library owns
+ * Blocking calls, but for (C); one host thread per context. The caller owns every host buffer; the library owns
  * device memory behind the opaque handles.
  */
 #ifndef SCLENS_HIP_H

@@ -1,15 +1,24 @@
-// Products of the dense operators: C[b] = epilogue(alpha * A[b] B[b]') from 16-bit operand images with the contraction contiguous, on
-// v_mfma_f32_32x32x16_{bf16,f16} with fp32 accumulation.
-//   * fp32 operands come as three bf16 planes (24 bits, exact): six products per term, smallest first -- p2 p0, p0 p2, p1 p1, p1 p0,
-//     p0 p1, p0 p0; what is left out (2 p1 p2) is at most 2^-23 of the term and 2^-26 in the mean square, the size of fp32's own rounding.
-//   * a workgroup owns one BM x BN tile; both operands go to LDS 64 columns at a time straight from memory (16 bytes per lane),
-//     S stages in turn: two where two workgroups share a CU or one fills it with 128 x 128 per wave, four where a single workgroup of a
-//     small tile would wait for each stage (0.57 us per stage of a 64 x 64 tile with two, whatever the work in it). Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): 16 rows at one chunk fall into 16 different
-//     16-byte bank groups, so a 16-byte read runs without conflicts.
-//   * the stage loop is a software pipeline of units of 16 columns: the reads of the next unit, and in the stage's last unit the copies
-//     of the stage after the next, are issued one at a time in the shadow of the matrix instructions.
+// Products of the dense operators: C[b] = epilogue(alpha * A[b] B[b]') on the matrix cores with fp32 accumulation.
+//   * 16-bit operands: v_mfma_f32_16x16x32_{bf16,f16}. fp32: v_mfma_f32_32x32x2_f32, or three bf16 planes (24 bits, exact) and six
+//     products per term, smallest first -- p2 p0, p0 p2, p1 p1, p1 p0, p0 p1, p0 p0; what is left out (2 p1 p2) is at most 2^-23 of the
+//     term and 2^-26 in the mean square, the size of fp32's own rounding. dense_ops.hip has the rule; 4096^3 takes 650 us in planes, their
+//     writing included, and about 900 on the fp32 instructions.
+//   * an operand lies in memory with the contraction contiguous, or across it (Mat::across: a gradient's transposed operands), and is
+//     read as it lies: no transposed copy is written. Rows that do not start on 16 bytes come as a padded copy (k_pack).
+//   * a workgroup of four waves owns one BM x BN tile; both operands go to LDS 64 columns at a time (fp32: 32) straight from memory (16
+//     bytes per lane), SA and SB stages in turn: three and two (all of LDS) with 128 x 128 per wave or with two workgroups per CU, four
+//     where a single workgroup of a small tile would wait for each stage (0.57 us per stage of a 64 x 64 tile with two, whatever the work
+//     in it). Chunk q (8 columns) of row r sits in slot q ^ ((r >> 1) & 7): 16 rows at one chunk fall into 16 different 16-byte bank
+//     groups, so a 16-byte read runs without conflicts. Rows across the contraction are read with the transposing LDS reads (pair_swz).
+//   * the stage loop is a software pipeline of units of 32 columns (fp32: 8): the reads of the next unit and the copies of the stages to
+//     come are issued one at a time in the shadow of the matrix instructions, with one barrier a stage.
 //   * the epilogue turns the accumulators through LDS so that bias, residual, pre-activation and result move 16 bytes per lane along
 //     the rows; it can also store the transpose and the mirrored half of a symmetric result.
+// What bounds it: power. 8192^3 in bf16 with SiLU and residual takes 835 us back to back (1.32 PFLOP/s; a plain library product without
+// them 670 to 750): the clock is brought down to 1.8 to 2.0 GHz. 16 x 16 x 32 matrix instructions take less of it than 32 x 32 x 16 (below);
+// fewer instructions beside them and a barrier that nobody waits at came to another 7 % (900 us before all three). One round of 256 tiles
+// (2048 x 2048 -> 8192 with GELU, 66 us) spends 15 us in the launch, the first stages and the epilogue, which nothing overlaps: the
+// accumulators leave room for one wave per SIMD. No LDS bank conflicts (counted).
 #include <algorithm>
 #include <type_traits>
 
@@ -120,17 +129,18 @@ __device__ __forceinline__ u16x8 read_words(const unsigned char* p) {
   return __builtin_bit_cast(u16x8, v);
 }
 
-template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
+template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int SA, int SB>
 __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(ProdArgs g) {
   constexpr int NW = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, NP = PA + PB;  // 1 KB copies (8 rows x 64 columns) per wave and stage
-  constexpr int OPA = BM * 128, STAGE = (BM + BN) * 128;
+  static_assert(SA >= SB && SB >= 2, "the first copies go stage by stage");
+  constexpr int STA = BM * 128, STB = BN * 128, OPB = SA * STA;  // bytes of a stage's operands; B's stages lie behind A's
   constexpr bool PL = (MT == D_PL3), F32 = (MT == D_F32);
   constexpr int ES = F32 ? 4 : 2, CE = 16 / ES, SC = 128 / ES;  // bytes of an element, elements of a chunk, columns of a stage
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const Product& p = g.p;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wid / WN, wn = wid % WN, l31 = lane & 31, h = lane >> 5;
+  const int wm = wid / WN, wn = wid % WN;
 
   // ---- the tile
   int ti, tj;
@@ -183,50 +193,43 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
 #pragma unroll
   for (int i = 0; i < NP; ++i) voff[i] = place(i, 0);
 
-  // ---- stages of this slice: stage t = (plane pair t / nkt, columns 64 (t % nkt) ..)
+  // ---- stages of this slice: stage t = (plane pair t / nkt, stage t % nkt of the contraction)
   const int ntot = (PL ? 6 : 1) * g.nkt;
   const int t0 = (int)blockIdx.z * g.kchunk, t1 = min(ntot, t0 + g.kchunk);
-  int ld_t = t0;                             // the stage the copies load
-  int ld_seg = PL ? t0 / max(1, g.nkt) : 0;  // its plane pair and column block
-  int ld_k = t0 - ld_seg * g.nkt;
-  const char *curA = baseA, *curB = baseB;
-  auto set_cur = [&]() {
-    curA = baseA + ld_k * stepA;
-    curB = baseB + ld_k * stepB;
-    if (PL) {
-      // (A plane, B plane), smallest products first: 20 02 11 10 01 00
-      const int pa = (0x001102 >> (4 * ld_seg)) & 15, pb = (0x010120 >> (4 * ld_seg)) & 15;
-      curA += 2 * pa * p.A.plane;
-      curB += 2 * pb * p.B.plane;
-    }
-  };
   const int ktail = (int)(p.K % SC);
-  bool ld_tail = false;
-  auto set_tail = [&]() {
-    const bool tail = ktail != 0 && ld_k + 1 == g.nkt;
-    if (tail != ld_tail) {
-      ld_tail = tail;
+  // What the copies of an operand load next: `left` more stages follow one step apart, the last of them stage t; behind it the tail, the
+  // next plane, or nothing: then the last stage is copied again and nobody reads the copy.
+  struct Ahead {
+    int t, left;
+    const char* cur;
+    int tail;
+  };
+  auto place_at = [&](Ahead& n, int t, auto is_a) {
+    constexpr bool isA = decltype(is_a)::value;
+    const int seg = PL ? t / g.nkt : 0, k = t - seg * g.nkt;
+    n.cur = (isA ? baseA : baseB) + k * (isA ? stepA : stepB);
+    if (PL)  // (A plane, B plane), smallest products first: 20 02 11 10 01 00
+      n.cur += 2 * ((isA ? 0x001102 : 0x010120) >> (4 * seg) & 15) * (isA ? p.A.plane : p.B.plane);
+    n.left = max(0, min(g.nkt - (ktail != 0 ? 2 : 1) - k, t1 - 1 - t));
+    n.t = t + n.left;
+    const int tail = ktail != 0 && k + 1 == g.nkt ? ktail : 0;
+    if (tail != n.tail) {
+      n.tail = tail;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) voff[i] = place(i, tail ? ktail : 0);
+      for (int i = isA ? 0 : PA; i < (isA ? PA : NP); ++i) voff[i] = place(i, tail);
     }
   };
-  auto advance = [&]() {  // past the last stage the copies repeat it; nobody reads the repetition
-    if (ld_t + 1 < t1) {
-      ++ld_t;
-      if (++ld_k == g.nkt) {
-        ld_k = 0;
-        ++ld_seg;
-      }
-      set_cur();
-      set_tail();
-    }
+  auto advance = [&](Ahead& n, auto is_a) {
+    n.cur += decltype(is_a)::value ? stepA : stepB;
+    if (--n.left < 0) place_at(n, min(n.t + 1, t1 - 1), is_a);
   };
-  auto copy = [&](int buf, int i) {
+  Ahead nA = {}, nB = {};
+  auto copy = [&](int at, int i) {  // copy i of the stage that lies at `at`
     const bool isA = i < PA;
-    unsigned char* dst = lds + buf * STAGE + (isA ? wid * PA + i : OPA / 1024 + wid * PB + i - PA) * 1024;
-    __builtin_amdgcn_global_load_lds((glb_cv*)((isA ? curA : curB) + voff[i]), (lds_v*)dst, 16, 0, 0);
+    unsigned char* dst = lds + at + (isA ? wid * PA + i : wid * PB + i - PA) * 1024;
+    __builtin_amdgcn_global_load_lds((glb_cv*)((isA ? nA.cur : nB.cur) + voff[i]), (lds_v*)dst, 16, 0, 0);
   };
-  auto zero_tail = [&](int buf) {
+  auto zero_tail = [&](int atA, int atB) {
     auto zero = [&](unsigned char* o, auto across, auto w) {
       constexpr int W = decltype(w)::value;
       if constexpr (decltype(across)::value) {  // whole columns of the contraction
@@ -239,140 +242,185 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
         }
       }
     };
-    zero(lds + buf * STAGE, std::integral_constant<bool, AC>(), std::integral_constant<int, BM>());
-    zero(lds + buf * STAGE + OPA, std::integral_constant<bool, BC>(), std::integral_constant<int, BN>());
+    zero(lds + atA, std::integral_constant<bool, AC>(), std::integral_constant<int, BM>());
+    zero(lds + atB, std::integral_constant<bool, BC>(), std::integral_constant<int, BN>());
     wait_lds_barrier();
   };
 
-  f32x16 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  // 16 bits: 16 x 16 x 32 tiles, AM x AN of them per wave. Their rate is that of 32 x 32 x 16, with half the traffic of the accumulators and
+  // the power that it takes, and power is what holds the clock down: both operands from registers on the whole chip 1.81 PFLOP/s with
+  // 32 x 32 x 16, 2.06 with 16 x 16 x 32 if the second operand stays from one instruction to the next, 1.72 if the first one does (random
+  // bf16; 2.46 each on zeros). fp32 (156 TFLOP/s either way): 32 x 32 x 2, which has fewer of them.
+  constexpr int TS = F32 ? 32 : 16, AM = TM * 32 / TS, AN = TN * 32 / TS, KU = F32 ? 8 : 32, NU = SC / KU;  // KU columns a unit, NU units a stage
+  typedef std::conditional_t<F32, f32x16, f32x4> Acc;
+  Acc acc[AM][AN] = {};
 
-  // A fragment of 32 rows x 16 columns: lane (row l31, columns 8 h .. 8 h + 7). Rows along the contraction: 16 bytes, and rows 32 apart
-  // have the same swizzle. Rows across it: two transposing reads of 4 columns each -- 16 lanes name 4 columns x 16 rows (lane i: column
-  // i >> 2, rows 4 (i & 3) ..) and lane i receives row i of all four; lanes 16 .. 31 take the other 16 rows, 32 .. 63 columns 8 .. 15.
-  const int ra = (wm * TM * 32 + l31) * 128, rb = OPA + (wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
+  // A fragment of TS rows x KU columns: lane (row lr, 16 bytes of columns from chunk NU-th .. on: 2 kk + h, 4 kk + kq). Rows along the
+  // contraction: 16 bytes, and rows 16 apart have the same swizzle. Rows across it: two transposing reads of 4 columns each -- 16 lanes name
+  // 4 columns x 16 rows (lane i: column i >> 2, rows 4 (i & 3) ..) and lane i receives row i of all four; the four sixteens take columns
+  // 8 kq ...
+  const int lr = lane & (TS - 1), kq = lane / TS, sw = (lr >> 1) & 7;
+  const int ra = (wm * TM * 32 + lr) * 128, rb = (wn * TN * 32 + lr) * 128;
   // fp32: the chunk of 4 columns 8 kk + 4 h .. of the row, its e-th column in the e-th of four matrix instructions; across, four words.
-  const int tr = (lane & 15) >> 2, tk = 8 * h + tr, th = (lane >> 4) & 1;
-  int ca[AC ? TM : 1], cb[BC ? TN : 1];
-  if constexpr (AC && F32) {
+  const int tk = 8 * kq + ((lane & 15) >> 2);
+  // (16 rows further the pair's number differs in bits that the swizzle changes: one exclusive or, and one address instead of AM, unless the
+  // wave's first pair is not a multiple of 4)
+  constexpr bool XOR = AC && BC && !F32 && TM != 3;
+  int ca[AC && !XOR ? AM : 1], cb[BC && !XOR ? AN : 1];
+  if constexpr (AC) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) ca[i] = 4 * h * 4 * BM + (wm * TM * 32 + i * 32 + l31) * 4;
+    for (int i = 0; i < (XOR ? 1 : AM); ++i)
+      ca[i] = F32 ? 4 * kq * 4 * BM + (wm * TM * 32 + i * 32 + lr) * 4 : tk * 2 * BM + ((wm * TM * 2 + i) ^ pair_swz<BM>(tk)) * 32 + (lane & 3) * 8;
   }
-  if constexpr (BC && F32) {
+  if constexpr (BC) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) cb[j] = OPA + 4 * h * 4 * BN + (wn * TN * 32 + j * 32 + l31) * 4;
+    for (int j = 0; j < (XOR ? 1 : AN); ++j)
+      cb[j] = F32 ? 4 * kq * 4 * BN + (wn * TN * 32 + j * 32 + lr) * 4 : tk * 2 * BN + ((wn * TN * 2 + j) ^ pair_swz<BN>(tk)) * 32 + (lane & 3) * 8;
   }
-  if constexpr (AC && !F32) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) ca[i] = tk * 2 * BM + ((wm * TM * 2 + 2 * i + th) ^ pair_swz<BM>(tk)) * 32 + (lane & 3) * 8;
-  }
-  if constexpr (BC && !F32) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) cb[j] = OPA + tk * 2 * BN + ((wn * TN * 2 + 2 * j + th) ^ pair_swz<BN>(tk)) * 32 + (lane & 3) * 8;
-  }
-  u16x8 av[2][TM], bv[2][TN];
-  auto fragA = [&](const unsigned char* B, int kk, int i) {
-    if constexpr (AC && F32) return read_words<4 * BM>(B + ca[i] + kk * 8 * 4 * BM);
-    else if constexpr (AC) return read_across<2 * BM>(B + ca[i] + kk * 16 * 2 * BM);
-    else return *reinterpret_cast<const u16x8*>(B + ra + i * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
+  u16x8 av[2][AM], bv[2][AN];
+  struct Stage {  // where a stage's operands lie in LDS
+    const unsigned char *A, *B;
+    int atA, atB;
   };
-  auto fragB = [&](const unsigned char* B, int kk, int j) {
-    if constexpr (BC && F32) return read_words<4 * BN>(B + cb[j] + kk * 8 * 4 * BN);
-    else if constexpr (BC) return read_across<2 * BN>(B + cb[j] + kk * 16 * 2 * BN);
-    else return *reinterpret_cast<const u16x8*>(B + rb + j * 32 * 128 + (((2 * kk + h) ^ sw) << 4));
+  auto fragA = [&](const Stage& s, int kk, int i) {
+    if constexpr (XOR) return read_across<2 * BM>(lds + ((s.atA + ca[0]) ^ (i << 5)) + kk * KU * 2 * BM);
+    else if constexpr (AC && F32) return read_words<4 * BM>(s.A + ca[i] + kk * KU * 4 * BM);
+    else if constexpr (AC) return read_across<2 * BM>(s.A + ca[i] + kk * KU * 2 * BM);
+    else return *reinterpret_cast<const u16x8*>(s.A + ra + i * TS * 128 + ((((8 / NU) * kk + kq) ^ sw) << 4));
   };
-  // read n of a unit's TM + TN: the operands in the order in which the matrix instructions want them
-  auto read = [&](int set, const unsigned char* B, int kk, int n) {
-    if (n == 0) av[set][0] = fragA(B, kk, 0);
-    else if (n <= TN) bv[set][n - 1] = fragB(B, kk, n - 1);
-    else av[set][n - TN] = fragA(B, kk, n - TN);
+  auto fragB = [&](const Stage& s, int kk, int j) {
+    if constexpr (XOR) return read_across<2 * BN>(lds + ((s.atB + cb[0]) ^ (j << 5)) + kk * KU * 2 * BN);
+    else if constexpr (BC && F32) return read_words<4 * BN>(s.B + cb[j] + kk * KU * 4 * BN);
+    else if constexpr (BC) return read_across<2 * BN>(s.B + cb[j] + kk * KU * 2 * BN);
+    else return *reinterpret_cast<const u16x8*>(s.B + rb + j * TS * 128 + ((((8 / NU) * kk + kq) ^ sw) << 4));
   };
-  // one matrix instruction at a time, and in its shadow what `beside` issues
+  // A unit's AM + AN reads, while the unit before it works on the other set. In the largest tile the first half of A's fragments has one set
+  // only (64 registers fewer than two of everything would be 32 too many): they are read last, each when its row of matrix instructions is done.
+  constexpr int ONCE = TM == 4 ? AM / 2 : 0;
+  auto read = [&](int set, const Stage& s, int kk, int n) {
+    if (n < AN) bv[set][n] = fragB(s, kk, n);
+    else if (n < AN + AM - ONCE) av[set][n - AN + ONCE] = fragA(s, kk, n - AN + ONCE);
+    else av[0][n - AN - AM + ONCE] = fragA(s, kk, n - AN - AM + ONCE);
+  };
+  // One matrix instruction at a time, and in its shadow what `beside` issues. (HOLD: the large tiles' accumulators stay in the accumulation
+  // registers, and each instruction in its place; left to itself, the compiler moves some of either to and fro. No instruction is emitted.)
+  constexpr bool HOLD = TM * TN >= 9;
   auto unit = [&](int set, auto beside) {
 #pragma unroll
     for (int e = 0; e < (F32 ? 4 : 1); ++e)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < AM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
+        for (int j = 0; j < AN; ++j) {
           if constexpr (F32)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, bv[set][j])[e], __builtin_bit_cast(f32x4, av[set][i])[e],
                                                              acc[i][j], 0, 0, 0);
           else if constexpr (MT == D_F16)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, bv[set][j]), __builtin_bit_cast(f16x8, av[set][i]),
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, bv[set][j]), __builtin_bit_cast(f16x8, av[i < ONCE ? 0 : set][i]),
                                                                acc[i][j], 0, 0, 0);
           else
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bv[set][j]),
-                                                                __builtin_bit_cast(bf16x8, av[set][i]), acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, bv[set][j]),
+                                                                __builtin_bit_cast(bf16x8, av[i < ONCE ? 0 : set][i]), acc[i][j], 0, 0, 0);
+          if constexpr (HOLD) asm volatile("" : "+a"(acc[i][j]));
           __builtin_amdgcn_sched_barrier(0);
-          if (e == 0) beside(i * TN + j);
+          beside((e * AM + i) * AN + j);
           __builtin_amdgcn_sched_barrier(0);
         }
   };
-  constexpr int NM = TM * TN, NR = TM + TN, QR = (NR + NM - 1) / NM;
-  auto reads = [&](int set, const unsigned char* B, int kk, int m) {
+  // one read beside every second matrix instruction where there are enough of those
+  constexpr int NM = AM * AN * (F32 ? 4 : 1), NR = AM + AN, SP = NM >= 2 * NR ? 2 : 1;
+  auto reads = [&](int set, const Stage& s, int kk, int m) {
 #pragma unroll
-    for (int q = 0; q < QR; ++q)
-      if (m * QR + q < NR) read(set, B, kk, m * QR + q);
-  };
-  // copies first .. first + n - 1 of a stage, spread evenly over the NM matrix instructions of a unit
-  auto copies = [&](int buf, int first, int n, int m) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-      if (i >= first && i < first + n && (i - first) * NM / n == m) copy(buf, i);
-  };
-  // Units 0, 1, 2 of stage t work on its columns while the next unit's are read. Behind the barrier every wave has the stage's last
-  // columns in registers -- its buffer is free for stage t + S -- and stage t + 1 has landed (of the wave's copies only those of the
-  // stages t + 2 .. t + S - 1 may still be on their way): unit 3 reads the first columns of t + 1 and issues the first half of the copies
-  // of t + S, unit 0 of t + 1 the other half. (A CU takes one copy per 16 cycles: all of them in one unit stall the waves that issue
-  // them; 8192^3 bf16: 62 % of the matrix cores' cycles, 71 % with the halves.)
-  constexpr int H = NP / 2;
-  if (t1 > t0) {
-    int rd_k = ld_k;  // column block of the stage that is read
-    set_cur();
-    set_tail();
-#pragma unroll
-    for (int b = 0; b < S; ++b) {
-      if (b > 0) advance();
-#pragma unroll
-      for (int i = 0; i < (b + 1 < S ? NP : H); ++i) copy(b, i);
+    for (int n = 0; n < NR; ++n) {
+      const int once = n - AN - AM + ONCE;  // >= 0: a fragment of one set
+      if (m == (once < 0 ? n * SP : std::max(n * SP, AN * (once + 1)))) read(set, s, kk, n);
     }
-    wait_barrier<(S - 2) * NP + H>();
-    if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(0);
+  };
+  // The barrier of stage t stands in its last unit but one, behind the matrix instruction BAR by which the reads of its last columns are
+  // back: every wave has them in registers then, so the stage's buffers are free, and stage t + 1 has landed: of the wave's copies only A's of
+  // t + 2 .. t + SA - 1 and B's of t + 2 .. t + SB - 1 are younger. Behind it go the copies of B's t + SB, then those of A's t + SA, `p` matrix
+  // instructions behind the barrier; a CU takes one per 16 cycles, and the wave whose copy has to wait issues nothing else. B's come first
+  // and closer together: with one stage of B less than of A they are the ones that are waited for.
+  static_assert(NM >= NR, "a read beside each matrix instruction");
+  constexpr int BAR = std::min(NM - 1, std::max((NR - 1) * SP, ONCE * AN) + 8), TOT = NU * NM;
+  constexpr int RB = std::max(1, TOT * 3 / 8 / PB), A0 = PB * RB, RA = std::max(1, (TOT - A0 - 1) / PA);
+  static_assert(A0 + (PA - 1) * RA + 1 < TOT, "all copies of a stage before the next barrier");
+  auto copies = [&](int atA, int atB, int p) {
 #pragma unroll
-    for (int n = 0; n < NR; ++n) read(0, lds, 0, n);
-    int cur = 0, prev = S - 1;  // buffers of the stage worked on and of the one before it, whose copies are half issued
+    for (int i = 0; i < PB; ++i)
+      if (p == i * RB + 1 - (RB == 1)) copy(atB, PA + i);
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (p == A0 + i * RA + 1 - (RA == 1)) copy(atA, i);
+  };
+  // A wave is alone on its SIMD, and every instruction of the loop's own costs the matrix cores 4 cycles that nothing fills: the bookkeeping
+  // of a stage is a few scalar additions.
+  if (t1 > t0) {
+    constexpr std::integral_constant<bool, true> opA{};
+    constexpr std::integral_constant<bool, false> opB{};
+    place_at(nA, t0, opA);
+    place_at(nB, t0, opB);
+#pragma unroll
+    for (int b = 0; b < SA; ++b) {
+      if (b < SB) {
+        if (b > 0) advance(nB, opB);
+#pragma unroll
+        for (int i = PA; i < NP; ++i) copy(OPB + b * STB, i);
+      }
+      if (b > 0) advance(nA, opA);
+#pragma unroll
+      for (int i = 0; i < PA; ++i) copy(b * STA, i);
+    }
+    wait_barrier<(SA - 1) * PA + (SB - 1) * PB>();
+    int to_tail = ktail != 0 ? g.nkt - 1 - t0 % g.nkt : 0x7fffffff;  // stages until the next one that ends inside its columns
+    if (to_tail == 0) {
+      zero_tail(0, OPB);
+      to_tail = g.nkt;
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) read(0, Stage{lds, lds + OPB, 0, OPB}, 0, n);
+    // where A's and B's stages t, t + 1 .. lie in LDS
+    int oa[SA], ob[SB];
+#pragma unroll
+    for (int i = 0; i < SA; ++i) oa[i] = i * STA;
+#pragma unroll
+    for (int i = 0; i < SB; ++i) ob[i] = OPB + i * STB;
     for (int t = t0; t < t1; ++t) {
-      const int nxt = cur + 1 == S ? 0 : cur + 1;
-      const unsigned char* B = lds + cur * STAGE;
-      const unsigned char* Bn = lds + nxt * STAGE;
-      unit(0, [&](int m) {
-        reads(1, B, 1, m);
-        copies(prev, H, NP - H, m);
-      });
-      unit(1, [&](int m) { reads(0, B, 2, m); });
-      unit(0, [&](int m) { reads(1, B, 3, m); });
-      wait_barrier<(S - 2) * NP>();
-      rd_k = rd_k + 1 == g.nkt ? 0 : rd_k + 1;
-      if (ktail != 0 && rd_k + 1 == g.nkt) zero_tail(nxt);
-      advance();
-      unit(1, [&](int m) {
-        reads(0, Bn, 0, m);
-        copies(cur, 0, H, m);
-      });
-      prev = cur;
-      cur = nxt;
+      const Stage now{lds + oa[0], lds + ob[0], oa[0], ob[0]}, next{lds + oa[1], lds + ob[1], oa[1], ob[1]};
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        unit(u & 1, [&](int m) {
+          if (u + 1 < NU) reads((u & 1) ^ 1, now, u + 1, m);
+          else reads(0, next, 0, m);
+          // (before this stage's barrier: what is left of the copies behind the last one, whose buffers have moved to the end)
+          const int p = (u - (NU - 2)) * NM + m - BAR - 1;
+          if (p < 0) copies(oa[SA - 1], ob[SB - 1], p + TOT);
+          if (p >= 0) copies(oa[0], ob[0], p);
+          if (p == -1) {
+            wait_barrier<(SA - 2) * PA + (SB - 2) * PB>();
+            if (--to_tail == 0) {
+              zero_tail(oa[1], ob[1]);
+              to_tail = g.nkt;
+            }
+            advance(nB, opB);
+            advance(nA, opA);
+          }
+        });
+      const int a0 = oa[0], b0 = ob[0];
+#pragma unroll
+      for (int i = 0; i + 1 < SA; ++i) oa[i] = oa[i + 1];
+#pragma unroll
+      for (int i = 0; i + 1 < SB; ++i) ob[i] = ob[i + 1];
+      oa[SA - 1] = a0;
+      ob[SB - 1] = b0;
     }
     wait_barrier<0>();  // no copy may land in the epilogue's LDS
   }
+  if constexpr (HOLD) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");  // (the last results have been written)
 
-  // ---- epilogue: 32 rows x 32 TN columns of the wave at a time, turned through LDS. D (B's rows are the matrix instruction's rows): row
-  // of C = lane & 31, column = (e & 3) + 8 (e >> 2) + 4 (lane >> 5). The loops stay rolled: unrolled, their 250 KB of instructions (every activation, every edge) cost a workgroup 25 us.
+  // ---- epilogue: 32 rows x 32 TN columns of the wave at a time, turned through LDS. D (B's rows are the matrix instruction's rows):
+  // row of C = lane % TS, column = 4 (lane / TS) + (e & 3), in fp32 + 8 (e >> 2). The loops stay rolled: unrolled, their 250 KB of instructions (every
+  // activation, every edge) cost a workgroup 25 us.
   constexpr int C = 32 * TN, LP = C + 4, CH = TN == 3 ? 16 : C / 8, RP = 64 / CH, NS = 32 / RP;  // RP rows per pass, 8 columns per lane
   float* T = reinterpret_cast<float*>(lds) + wid * 32 * LP;
   // (96 columns are twelve lanes of sixteen: the last four repeat the twelfth and store nothing)
@@ -387,11 +435,16 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
         // (the two markers keep the branches from being merged into one that picks its accumulators by index, from scratch memory)
         asm volatile("; rows %0" ::"n"(n) : "memory");
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+        for (int j = 0; j < AN; ++j)
+          if constexpr (F32) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<f32x4*>(&T[l31 * LP + j * 32 + 8 * e + 4 * h]) =
-                f32x4{acc[n][j][4 * e], acc[n][j][4 * e + 1], acc[n][j][4 * e + 2], acc[n][j][4 * e + 3]};
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<f32x4*>(&T[lr * LP + j * 32 + 8 * e + 4 * kq]) =
+                  f32x4{acc[n][j][4 * e], acc[n][j][4 * e + 1], acc[n][j][4 * e + 2], acc[n][j][4 * e + 3]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) *reinterpret_cast<f32x4*>(&T[(16 * e + lr) * LP + j * 16 + 4 * kq]) = acc[2 * n + e][j];
+          }
         asm volatile("; rows %0" ::"n"(n) : "memory");
       }
     });
@@ -683,28 +736,28 @@ Plan plan_product(int64_t M, int64_t N, int64_t K, int batch, int type, int symm
   return best;
 }
 
-template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int S>
+template <int MT, int OT, int RT, bool PART, bool AC, bool BC, int WM, int WN, int TM, int TN, int SA, int SB>
 int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
   // the stages; the epilogue's block of fp32 and two blocks of the residual per wave
-  constexpr int LDS = std::max(S * (WM * TM + WN * TN) * 32 * 128,
+  constexpr int LDS = std::max((SA * WM * TM + SB * WN * TN) * 32 * 128,
                                WM * WN * (32 * (32 * TN + 4) * 4 + 2 * 32 * (TN == 3 ? 128 : 32 * TN) * (MT == D_F32 ? 4 : 2)));
   static_assert(LDS <= 163840, "LDS of a CU");
-  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>);
+  const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, SA, SB>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
-  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, S>), grid, dim3(WM * WN * 64), LDS, st, g);
+  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, SA, SB>), grid, dim3(WM * WN * 64), LDS, st, g);
   SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
 template <int MT, int OT, int RT, bool PART, bool AC, bool BC>
 int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile) {
   if constexpr (MT != D_F32) {
-    if (tile == 0) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 4, 4, 2>(ctx, st, g, grid);
-    if (tile == 1) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 3, 3, 3>(ctx, st, g, grid);
-    if (tile == 2) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 2>(ctx, st, g, grid);
+    if (tile == 0) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 4, 4, 3, 2>(ctx, st, g, grid);
+    if (tile == 1) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 3, 3, 3, 3>(ctx, st, g, grid);
+    if (tile == 2) return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 3, 2>(ctx, st, g, grid);
   }
   switch (tile) {
-    case 3: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 4>(ctx, st, g, grid);
-    default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, 4>(ctx, st, g, grid);
+    case 3: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 4, 4>(ctx, st, g, grid);
+    default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, 4, 4>(ctx, st, g, grid);
   }
 }
 template <int MT, int OT, int RT, bool AC = false, bool BC = false>

@@ -118,7 +118,8 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
 // ------------------------------------------------------------------ linear, backward
 // dz: 64 x 128 per workgroup, 8 columns per lane, its image (the same layout, padded with zeros to whole chunks) and the block's column
 // sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
-// pre-activation and the gradient that comes in already are. Bound by HBM: two reads and a write per element.
+// pre-activation and the gradient that comes in already are. Bound by HBM, two reads and a write per element: 8192 x 8192 bf16 77 us,
+// 5.2 TB/s.
 constexpr int DZ_ROWS = 64;
 template <int T>
 __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
@@ -313,8 +314,12 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
 }
 
 // ------------------------------------------------------------------ orthogonalize
+// Both sides above 64 and one above 128: three products per step of the caller's layout, the two symmetric ones on the tiles on and below
+// the diagonal. One 4096 x 4096 bf16 matrix, five steps: 8 + 18 us to scale it, 84 us per symmetric product (0.82 PFLOP/s of the lower
+// half: 253 tiles of 192, one round), 131 us per full one (1.05 PFLOP/s). Four 1024 x 4096: A 37 us (144 tiles of 128 for 256 CUs), A A
+// 13, the full one 46.
 // |g|_F^2 of each matrix: partial sums in fp64 (fp32 squares of large entries overflow), added in a fixed order by whoever needs them.
-// Bound by reading g: 8 columns per lane, tpr lanes to a row, four rows' loads on their way together.
+// Bound by reading g: 8 columns per lane, tpr lanes to a row, four rows' loads on their way together (4096 x 4096 bf16: 8.2 us, 24 with 2-byte loads).
 template <int T>
 __global__ __launch_bounds__(256) void k_sumsq(Mat src, int64_t rows, int64_t cols, int tpr, double* __restrict__ part) {
   __shared__ double S[256];
@@ -347,6 +352,7 @@ __global__ __launch_bounds__(256) void k_sumsq(Mat src, int64_t rows, int64_t co
 }
 
 // x0 = scale g / (|g|_F + eps), a 64 x 64 block: its image and the image of its transpose. `img` has the orientation of the source.
+// Bound by one read and one write (4096 x 4096 bf16: 18 us, 3.7 TB/s).
 template <int T, int IT>
 __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64_t cols, const double* __restrict__ part, int nparts, double eps,
                                                     double scale, Mat img, Mat imgT) {

@@ -1,7 +1,8 @@
 // Orthogonalisation of small matrices and of matrices with one short side.
 //
 // Both sides at most 128 (k_orth_direct): x and A stay in LDS in fp32, a workgroup per matrix does all steps as they are defined on
-// v_mfma_f32_16x16x4, one launch. Bound by the matrix instructions (40 x 40: 21 tiles of 10 per step, 0.9 us).
+// v_mfma_f32_16x16x4, one launch. Bound by the chain of products, reads from LDS and barriers of a step (40 x 40: 21 tiles of 10 matrix
+// instructions, 2 us; 190 matrices, eight steps: 21 us).
 //
 // A short side m of at most 64, the other longer: all steps of x <- (a + b A + c A A) x, A = x x', act on x from the short side, so
 //   x_T = Q x_0,   P = a I + b A + c A A,   Q <- P Q,   A <- P A P
@@ -11,7 +12,9 @@
 // on v_mfma_f64_16x16x4 (below 64 rows they cost less than reading x does; the entries of x convert exactly).
 // A, P, Q commute and are symmetric: tiles on and below the diagonal are computed and mirrored.
 //   n up to 1024, or many matrices: everything in one workgroup per matrix, one launch (k_orth_small).
-//   longer: partial sums of g g' over slices (k_orth_gram, k_orth_gram_sum), the steps in one workgroup (k_orth_steps), the product.
+//   longer: partial sums of g g' over slices (k_orth_gram, k_orth_gram_sum), the steps in one workgroup (k_orth_steps), the product
+//   (k_orth_apply). 100 000 x 40 in fp32, eight steps: 14 + 4 + 35 + 22 us. The steps are a chain of fp64 products on one CU (4 us each),
+//   the passes over x are bound by HBM (1.1 and 1.4 TB/s: fp64 matrix instructions and 16 MB, too little to fill it).
 #include <algorithm>
 
 #include "dense_dev.h"

@@ -144,8 +144,8 @@ __global__ __launch_bounds__(256) void k_small_backward(LinearBwdArgs a, int ndx
 }
 
 // Forward: at most 2^28 flops and 1024 columns of the contraction, where the tiles would need packed copies (fp32 300 x 300 -> 300: 7.7 us
-// against 20; operands on 16 bytes feed the tiles as they lie). Backward, against seven launches of 25 to 30 us: at most 2^26 flops a
-// product and 384 rows of either contraction (fp32 200 x 93 -> 50: 12.5 us against 36; 512 x 256 -> 512 would take 27).
+// against 20; operands on 16 bytes feed the tiles as they lie). Backward, against up to six launches of 25 to 30 us: at most 2^26 flops a
+// product and 384 rows of either contraction (fp32 200 x 93 -> 50: 11 us against 36; 512 x 256 -> 512 would take 27).
 bool linear_is_small(const LinearArgs& a) { return a.K <= 1024 && (double)a.M * a.N * a.K <= (double)(1 << 27); }
 bool backward_is_small(const LinearBwdArgs& a) { return std::max(a.M, a.N) <= 384 && (double)a.M * a.N * a.K <= (double)(1 << 25); }
 
