@@ -263,9 +263,9 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
   const int ra = (wm * TM * 32 + lr) * 128, rb = (wn * TN * 32 + lr) * 128;
   // fp32: the chunk of 4 columns 8 kk + 4 h .. of the row, its e-th column in the e-th of four matrix instructions; across, four words.
   const int tk = 8 * kq + ((lane & 15) >> 2);
-  // (16 rows further the pair's number differs in bits that the swizzle changes: one exclusive or, and one address instead of AM, unless the
-  // wave's first pair is not a multiple of 4)
-  constexpr bool XOR = AC && BC && !F32 && TM != 3;
+  // (16 rows further the pair number differs in bits that the swizzle changes: with an exclusive or one address does instead of AM, which the
+  // largest tile, its first pair a multiple of 8, has no registers for)
+  constexpr bool XOR = AC && BC && !F32 && TM == 4;
   int ca[AC && !XOR ? AM : 1], cb[BC && !XOR ? AN : 1];
   if constexpr (AC) {
 #pragma unroll
@@ -698,7 +698,11 @@ struct TileKind {
 };
 // measured at 16 and 64 stages on 64 to 1024 tiles
 constexpr int NTILES = 5;
-const TileKind TILES[NTILES] = {{256, 1, 1.0, 1.48, 15.0}, {192, 1, 0.80, 0.90, 11.0}, {128, 2, 0.73, 1.05, 4.0}, {128, 1, 0.53, 0.55, 6.0}, {64, 2, 0.29, 0.41, 3.5}};
+const TileKind TILES[NTILES] = {{256, 1, 1.1, 1.30, 15.0},
+                                  {192, 1, 0.80, 0.90, 11.0},
+                                  {128, 2, 0.73, 1.02, 4.0},
+                                  {128, 1, 0.53, 0.55, 6.0},
+                                  {64, 2, 0.29, 0.41, 3.5}};
 // fp32 on the fp32 matrix cores, stages of 32 columns: bound by the matrix instructions in every tile (two workgroups on a CU take twice as
 // long), so the two smallest do; the larger ones' residual would not fit LDS beside the accumulators
 const TileKind TILES_F32[NTILES] = {{0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {128, 1, 2.0, 2.1, 6.0}, {64, 2, 0.55, 1.05, 4.0}};
