@@ -315,11 +315,12 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
 
 // ------------------------------------------------------------------ orthogonalize
 // Both sides above 64 and one above 128: three products per step of the caller's layout, the two symmetric ones on the tiles on and below
-// the diagonal. One 4096 x 4096 bf16 matrix, five steps: 8 + 18 us to scale it, 84 us per symmetric product (0.82 PFLOP/s of the lower
-// half: 253 tiles of 192, one round), 131 us per full one (1.05 PFLOP/s). Four 1024 x 4096: A 37 us (144 tiles of 128 for 256 CUs), A A
-// 13, the full one 46.
+// the diagonal. One 4096 x 4096 bf16 matrix, five steps: 8 + 18 us to scale it, 88 us per symmetric product (0.78 PFLOP/s of the lower
+// half: 253 tiles of 192, one round), 136 us per full one (1.01 PFLOP/s). Four 1024 x 4096: A 36 us (144 tiles of 128 for 256 CUs), A A
+// 14, the full one 45.
 // |g|_F^2 of each matrix: partial sums in fp64 (fp32 squares of large entries overflow), added in a fixed order by whoever needs them.
-// Bound by reading g: 8 columns per lane, tpr lanes to a row, four rows' loads on their way together (4096 x 4096 bf16: 8.2 us, 24 with 2-byte loads).
+// Bound by reading g: 8 columns per lane, tpr lanes to a row, four rows' loads on their way together (4096 x 4096 bf16: 8.2
+// us, 24 with 2-byte loads).
 template <int T>
 __global__ __launch_bounds__(256) void k_sumsq(Mat src, int64_t rows, int64_t cols, int tpr, double* __restrict__ part) {
   __shared__ double S[256];
