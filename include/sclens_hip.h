@@ -7,7 +7,7 @@
  *   (A) the same five operations with the same host-array semantics (drop-in per call site), and
  *   (B) a session that keeps the count matrix, the scaled matrices, the Gram matrix and the
  *       eigenvectors resident in HBM for the whole sclens() call (what a `device_="hip"` branch of
- *       sclens() would call; see INTEGRATION.md for the Julia ccall shim), and
+ *       sclens() would call through a Julia ccall shim), and
  *   (C) dense operators on device tensors beside it: a product with bias, activation and residual, its gradient, and the orthogonal
  *       factor of a matrix (queued on the caller's stream, workspace of the caller, row-major; the rules stand with them).
  *
