@@ -1,7 +1,7 @@
 // Products with one short side: the long operand is streamed once past at most 16 rows (k_rows, any type) or, in fp32 or from rows
 // that do not start on 16 bytes, at most 128 rows (k_stream). Both are bound by reading the long operand; the matrix cores (16 x 16 x 32
 // tiles, the long operand as the rows of the tile) have room to spare: 26 % of their cycles at 40 short rows in fp32 (six products per
-// term). Measured: 4096 x 4096 bf16 weights past one row 7.6 us (4.4 TB/s), fp32 20 000 x 10 000 past 40 rows 194 us (4.1 TB/s; a large
+// term). Measured: 4096 x 4096 bf16 weights past one row 7.6 us (4.4 TB/s), fp32 20 000 x 10 000 past 40 rows 185 us (4.3 TB/s; a large
 // copy moves 4.9).
 #include <algorithm>
 
@@ -123,10 +123,9 @@ int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
 }
 
 // ---- at most 128 short rows (an image: three bf16 planes for fp32): 256 long rows per workgroup, 32 per wave, the contraction cut into
-// grid.y slices of whole 64-column stages. The short operand's stage sits in LDS (two stages in turn, chunk q of row r in slot
-// q ^ ((r >> 1) & 7)); the long one goes from memory to registers two stages ahead and, in fp32, is taken apart
-// there. A packed copy of it, which the tiled product would read, costs three times the traffic: fp32 20 000 x 10 000 onto 40 took 949 us
-// that way (196 us this way), bf16 20 001 x 10 001 (rows on 2 bytes) 281 us.
+// grid.y slices of whole 64-column stages. The short operand's stages sit in LDS (D in turn, chunk q of row r in slot
+// q ^ ((r >> 1) & 7)); the long one goes from memory to registers D stages ahead and, in fp32, is taken apart there. A packed copy of it, which the tiled product would read, costs three times the traffic: fp32 20 000 x 10 000 onto 40 took 949 us
+// that way (196 us this way, 205 with the long operand two stages ahead instead of three), bf16 20 001 x 10 001 (rows on 2 bytes) 281 us.
 struct StreamArgs {
   const void* big;
   int64_t ldb, R, K;
@@ -137,12 +136,15 @@ struct StreamArgs {
   int64_t sr, ss;     // strides of the long and the short index in a slab
   int kchunk;         // stages per slice
 };
+// stages that the long operand is fetched ahead: three where the registers hold them
+constexpr int stream_depth(int NT) { return NT <= 4 ? 3 : 2; }
 template <int T, int NT>
 __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
   typedef typename Elem<T>::type E;
   constexpr int NP = T == D_F32 ? 3 : 1, ROWS = NT * 16;
   constexpr int PLANE = ROWS * 128, STAGE = NP * PLANE, PIECES = STAGE / 1024;
-  constexpr int LOADS = T == D_F32 ? 8 : 4;  // 16-byte loads of a stage's fetch, at least
+  constexpr int LOADS = T == D_F32 ? 8 : 4, COPIES = PIECES / 8;  // 16-byte loads of a stage's fetch and its copies per wave, at least
+  constexpr int D = stream_depth(NT);
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.x * 256 + wid * 32;
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
       __builtin_amdgcn_global_load_lds((glb_cv*)s, (lds_v*)(lds + buf * STAGE + p * 1024), 16, 0, 0);
     }
   };
-  Chunk<T> n1[2][2], n2[2][2];
+  Chunk<T> ahead[D][2][2];
   auto fetch = [&](Chunk<T>(&n)[2][2], int t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -172,11 +174,14 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto stage = [&](Chunk<T>(&n)[2][2], int t) {
-    const int cur = (t - t0) & 1;
-    // this stage has landed on all sides; only the fetch of the stage after it may still be on its way (a stage that ends inside its 64
-    // columns is fetched with fewer loads, so they cannot be counted off)
-    if (t + 1 < t1 && (int64_t)(t + 2) * 64 <= a.K) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+  auto stage = [&](Chunk<T>(&n)[2][2], int t, int cur) {
+    // This stage's copy has landed on all sides; younger ones may still be on their way: with D = 2 the fetch of t + 1, with D = 3 the fetches
+    // of t + 1 and t + 2 and the copy between them. (A stage that ends inside its 64 columns is fetched with fewer loads, so they cannot be
+    // counted off.)
+    if (t + D - 1 < t1 && (int64_t)(t + D) * 64 <= a.K)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 1) * LOADS + (D - 2) * COPIES) : "memory");
+    else if (D == 3 && t + 1 < t1 && (int64_t)(t + 2) * 64 <= a.K)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS + COPIES) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     u16x8 A[2][2][NP];
 #pragma unroll
@@ -186,8 +191,8 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
         if constexpr (T == D_F32) split8(n[i][kk].v, A[i][kk]);
         else A[i][kk][0] = n[i][kk].v;
       }
-    if (t + 1 < t1) copy(cur ^ 1, t + 1);
-    if (t + 2 < t1) fetch(n, t + 2);
+    if (t + D - 1 < t1) copy((cur + D - 1) % D, t + D - 1);
+    if (t + D < t1) fetch(n, t + D);
     const unsigned char* B = lds + cur * STAGE;
     // up to four column tiles together, so that six products of one accumulator are not issued one after the other
     constexpr int G = NT <= 4 ? NT : NT / 2;
@@ -218,14 +223,16 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
         term(0, 0);
       }
   };
-  if (t0 < t1) {
-    copy(0, t0);
-    fetch(n1, t0);
-    if (t0 + 1 < t1) fetch(n2, t0 + 1);
-  }
-  for (int t = t0; t < t1; t += 2) {
-    stage(n1, t);
-    if (t + 1 < t1) stage(n2, t + 1);
+#pragma unroll
+  for (int i = 0; i < D; ++i)
+    if (t0 + i < t1) {
+      if (i < D - 1) copy(i, t0 + i);
+      fetch(ahead[i], t0 + i);
+    }
+  for (int t = t0; t < t1; t += D) {
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+      if (t + i < t1) stage(ahead[i], t + i, i);
   }
   float* out = a.slabs + (int64_t)blockIdx.y * a.slab;
 #pragma unroll
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(512, 2) void k_stream(StreamArgs a) {
 namespace {
 template <int T, int NT>
 int launch_stream(Ctx* ctx, hipStream_t st, const StreamArgs& a, int slices) {
-  constexpr int LDS = 2 * (T == D_F32 ? 3 : 1) * NT * 16 * 128;
+  constexpr int LDS = stream_depth(NT) * (T == D_F32 ? 3 : 1) * NT * 16 * 128;
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_stream<T, NT>), LDS));
   hipLaunchKernelGGL((k_stream<T, NT>), dim3((unsigned)((a.R + 255) / 256), (unsigned)slices), dim3(512), LDS, st, a);
   SCL_HIP(ctx, hipGetLastError());
