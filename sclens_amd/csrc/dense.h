@@ -48,6 +48,7 @@ int product_join(Ctx* ctx, hipStream_t st, const Product& p, int slices);
 // dense_stream.hip: products with one short side (linear_forward has the rule)
 constexpr int64_t STREAM_SHORT = 128;
 int stream_slices(int64_t R, int64_t S, int64_t K, int* kchunk);
+double stream_us(int64_t R, int64_t S, int64_t K, int dtype);
 int stream_product(Ctx* ctx, hipStream_t st, int dtype, const void* big, int64_t ldb, int64_t R, const Mat& small, int64_t S, int64_t K,
                    float* slabs, int64_t slab, int64_t sr, int64_t ss);
 

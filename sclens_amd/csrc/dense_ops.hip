@@ -49,10 +49,14 @@ bool planes_pay(int64_t M, int64_t N, int64_t K, int64_t packed_elems, int batch
 
 // ------------------------------------------------------------------ linear
 // One short side: at most 16 rows of x go past w in one launch. Where the tiles would need a packed copy of the longer operand (fp32, or
-// rows that do not start on 16 bytes) up to 128 rows of the other stream it as it lies and join the slices of the contraction. Short
-// contractions or few long rows are left to the tiles, which then have as little to read.
-static bool streams(int dtype, const void* big, int64_t ldb, int64_t S, int64_t R, int64_t K) {
-  return (dtype == D_F32 || !direct(dtype, big, ldb, K)) && S <= STREAM_SHORT && R >= 4 * S && R >= 256 && K >= 256;
+// rows that do not start on 16 bytes) up to 128 rows of the other stream it as it lies and join the slices of the contraction, unless the
+// tiles, copies included, are estimated to be faster.
+static bool streams(const LinearArgs& a, bool big_x) {
+  const int64_t R = big_x ? a.M : a.N, S = big_x ? a.N : a.M;
+  const bool dx = direct(a.dtype, a.x, a.ldx, a.K), dw = direct(a.dtype, a.w, a.ldw, a.K);
+  if ((a.dtype != D_F32 && (big_x ? dx : dw)) || S > STREAM_SHORT || R < 4 * S || R < 256 || a.K < 256) return false;
+  const double copied = (double)((dx ? 0 : a.M) + (dw ? 0 : a.N)) * a.K * (a.dtype == D_F32 ? 8 : 4);
+  return stream_us(R, S, a.K, a.dtype) < product_us(a.M, a.N, a.K, 1, a.dtype, 0) + (copied > 0 ? 5.0 + copied / 4e6 : 0.0);
 }
 
 static int linear_stream(Ctx* ctx, hipStream_t st, const LinearArgs& a, bool big_x, void* ws, int64_t ws_bytes, int64_t* need) {
@@ -87,8 +91,8 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
     if (a.M <= 16) return linear_rows(ctx, st, a);
     const bool tiles_as_is = direct(a.dtype, a.x, a.ldx, a.K) && direct(a.dtype, a.w, a.ldw, a.K);
     if (!tiles_as_is && linear_is_small(a)) return linear_small(ctx, st, a);
-    if (streams(a.dtype, a.w, a.ldw, a.M, a.N, a.K)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
-    if (streams(a.dtype, a.x, a.ldx, a.N, a.M, a.K)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
+    if (streams(a, false)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
+    if (streams(a, true)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
   Carve c(ws);
   if (a.K > MAX_CONTRACTION && a.M > 0 && a.N > 0) return ctx->fail(SCLENS_ERR_ARG, "linear: more than 2^25 columns");

@@ -657,3 +657,14 @@ def test_coefficients_that_grow(dense):
         dense.orthogonalize(x, coefficients=[(1e10, 0.0, 0.0)])
     with pytest.raises(Exception, match="grow"):
         dense.orthogonalize(x, coefficients=[(float("nan"), 0.0, 0.0)])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,S,K", [(20000, 40, 1001), (20000, 16, 3001), (20000, 93, 2111), (20000, 128, 1983), (30000, 60, 1023)])
+def test_long_streams(dense, R, S, K, dtype):
+    """long enough that a short side is streamed past, in contractions that end inside a stage and inside a chunk"""
+    g = gen_for("long stream", R, S, K)
+    x, w = ints(g, (R, K), dtype, 1), ints(g, (S, K), dtype, 1)
+    ref = x.double() @ w.double().t()
+    assert torch.equal(dense.linear(x, w), ref.float().to(dtype))
+    assert torch.equal(dense.linear(w, x), ref.t().float().to(dtype))
