@@ -703,9 +703,10 @@ const TileKind TILES[NTILES] = {{256, 1, 1.1, 1.30, 15.0},
                                   {128, 2, 0.73, 1.02, 4.0},
                                   {128, 1, 0.53, 0.55, 6.0},
                                   {64, 2, 0.29, 0.41, 3.5}};
-// fp32 on the fp32 matrix cores, stages of 32 columns: bound by the matrix instructions in every tile (two workgroups on a CU take twice as
-// long), so the two smallest do; the larger ones' residual would not fit LDS beside the accumulators
-const TileKind TILES_F32[NTILES] = {{0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {128, 1, 2.0, 2.1, 6.0}, {64, 2, 0.55, 1.05, 4.0}};
+// fp32 on the fp32 matrix cores, stages of 32 columns: bound by the matrix instructions in every tile (workgroups that share a CU take turns),
+// so the two smallest do; the larger ones' residual would not fit LDS beside the accumulators. Three stages instead of four let a third
+// workgroup of the smallest onto a CU (gradients of 7373 x 480 -> 4838: 733 -> 595 us)
+const TileKind TILES_F32[NTILES] = {{0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {0, 1, 0, 0, 0}, {128, 1, 2.0, 2.1, 6.0}, {64, 3, 0.55, 1.6, 4.5}};
 
 // The tile and the slices of the contraction with the least time by the figures above: rounds of the chip's 256 CUs, the stages of a
 // workgroup, and for slices the slabs written, read and joined by a second launch.
@@ -761,7 +762,7 @@ int launch_tile(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid, int tile
   }
   switch (tile) {
     case 3: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 2, 2, 4, 4>(ctx, st, g, grid);
-    default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, 4, 4>(ctx, st, g, grid);
+    default: return launch<MT, OT, RT, PART, AC, BC, 2, 2, 1, 1, MT == D_F32 ? 3 : 4, MT == D_F32 ? 3 : 4>(ctx, st, g, grid);
   }
 }
 template <int MT, int OT, int RT, bool AC = false, bool BC = false>
