@@ -14,10 +14,10 @@
 //     come are issued one at a time in the shadow of the matrix instructions, with one barrier a stage.
 //   * the epilogue turns the accumulators through LDS so that bias, residual, pre-activation and result move 16 bytes per lane along
 //     the rows; it can also store the transpose and the mirrored half of a symmetric result.
-// What bounds it: power. 8192^3 in bf16 with SiLU and residual takes 770 us (1.43 PFLOP/s; a plain library product without them 670 to
+// What bounds it: power. 8192^3 in bf16 with SiLU and residual takes 764 us (1.44 PFLOP/s; a plain library product without them 670 to
 // 750): the clock is brought down to 1.8 to 2.0 GHz, the matrix cores work in 73 % of the cycles. 16 x 16 x 32 matrix instructions take less of it than 32 x 32 x 16 (below);
 // fewer instructions beside them and a barrier with little to wait for came to more than that (860 us before all three). One round of 256 tiles
-// (2048 x 2048 -> 8192 with GELU, 67 us) spends 15 us in the launch, the first stages and the epilogue, which nothing overlaps: the
+// (2048 x 2048 -> 8192 with GELU, 66 us) spends 15 us in the launch, the first stages and the epilogue, which nothing overlaps: the
 // accumulators leave room for one wave per SIMD. No LDS bank conflicts (counted).
 #include <algorithm>
 #include <type_traits>

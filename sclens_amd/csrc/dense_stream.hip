@@ -1,7 +1,7 @@
 // Products with one short side: the long operand is streamed once past at most 16 rows (k_rows, any type) or, in fp32 or from rows
 // that do not start on 16 bytes, at most 128 rows (k_stream). Both are bound by reading the long operand; the matrix cores (16 x 16 x 32
 // tiles, the long operand as the rows of the tile) have room to spare: 26 % of their cycles at 40 short rows in fp32 (six products per
-// term). Measured: 4096 x 4096 bf16 weights past one row 7.6 us (4.4 TB/s), fp32 20 000 x 10 000 past 40 rows 185 us (4.3 TB/s; a large
+// term). Measured: 4096 x 4096 bf16 weights past one row 7.6 us (4.4 TB/s), fp32 20 000 x 10 000 past 40 rows 182 us (4.4 TB/s; a large
 // copy moves 4.9).
 #include <algorithm>
 
