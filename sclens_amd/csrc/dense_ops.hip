@@ -410,9 +410,8 @@ __global__ __launch_bounds__(256) void k_orth_start(Mat src, int64_t rows, int64
   }
 }
 
-namespace {
 // largest |a s + b s^3 + c s^5| over 0 <= s <= B: the singular values' bound after a step
-double step_bound(double a, double b, double c, double B) {
+double orth_step_bound(double a, double b, double c, double B) {
   auto f = [&](double s) { return std::fabs(((c * s * s + b) * s * s + a) * s); };
   double best = f(B);
   // a + 3 b q + 5 c q^2 = 0, q = s^2
@@ -429,6 +428,8 @@ double step_bound(double a, double b, double c, double B) {
     at(-a / (3 * b));
   return best;
 }
+
+namespace {
 // the power of two that brings a bound just under 2^14 (fp16 holds 65504: a factor of four is left for rounding)
 double pow2_scale(double bound) { return std::ldexp(1.0, 13 - std::ilogb(std::max(bound, 1e-30))); }
 }  // namespace
@@ -488,7 +489,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     const double ca = a.coef[3 * t], cb = a.coef[3 * t + 1], cc = a.coef[3 * t + 2];
     const bool last = t + 1 == a.steps;
     const Mat &x = X[t & 1], &xt = XT[t & 1];
-    const double next = step_bound(ca, cb, cc, bound);
+    const double next = orth_step_bound(ca, cb, cc, bound);
     const double s_a = wide ? 1.0 : pow2_scale(bound * bound);
     const double s_p = wide ? 1.0 : pow2_scale(std::fabs(cb) * bound * bound + std::fabs(cc) * bound * bound * bound * bound);
     const double s_n = wide || last ? 1.0 : pow2_scale(next);
@@ -550,7 +551,7 @@ int orthogonalize(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t
   if (a.batch == 0 || a.rows == 0 || a.cols == 0) return SCLENS_OK;
   double bound = 1.0;
   for (int t = 0; t < a.steps; ++t) {
-    bound = step_bound(a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2], bound);
+    bound = orth_step_bound(a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2], bound);
     // (fp32 holds its fourth power, the entries of A A)
     if (!(bound < 1e9)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: these coefficients let the singular values grow without bound");
   }

@@ -9,13 +9,17 @@
 // needs the m x n matrix twice (for A_0 = x_0 x_0' and for the last product) whatever the number of steps; |g|_F^2 is the trace of g g'.
 // In exact arithmetic that is the definition. In floating point an error of A_0 grows with the square of a small singular value's growth
 // (five steps of a = 3.4445: a^8 = 2e4 relative to the largest), which fp32 cannot pay and fp64 can: the m x m side and both products run
-// on v_mfma_f64_16x16x4 (below 64 rows they cost less than reading x does; the entries of x convert exactly).
+// on v_mfma_f64_16x16x4 (below 64 rows they cost less than reading x does; the entries of x convert exactly). Not for any number of steps:
+// a singular value of zero leaves an eigenvalue of about -1e-17, and one that has grown to -0.1 runs off to infinity (nothing pulls a negative one
+// back; A = x x', formed anew in each step, has none). orth_is_small bounds that growth, eleven of the steps above pass, and what it
+// turns away is worked on by its definition.
 // A, P, Q commute and are symmetric: tiles on and below the diagonal are computed and mirrored.
 //   n up to 1024, or many matrices: everything in one workgroup per matrix, one launch (k_orth_small).
 //   longer: partial sums of g g' over slices (k_orth_gram, k_orth_gram_sum), the steps in one workgroup (k_orth_steps), the product
 //   (k_orth_apply). 100 000 x 40 in fp32, eight steps: 14 + 4 + 35 + 22 us. The steps are a chain of fp64 products on one CU (4 us each),
 //   the passes over x are bound by HBM (1.1 and 1.4 TB/s: fp64 matrix instructions and 16 MB, too little to fill it).
 #include <algorithm>
+#include <cmath>
 
 #include "dense_dev.h"
 
@@ -538,9 +542,34 @@ int run_small_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
 }
 }  // namespace
 
+// largest |a + b l + c l^2| over 0 <= l <= L
+static double largest_quadratic(double a, double b, double c, double L) {
+  double v = std::max(std::fabs(a), std::fabs(a + (b + c * L) * L));
+  if (c != 0.0) {
+    const double l = -b / (2 * c);
+    if (l > 0 && l < L) v = std::max(v, std::fabs(a + (b + c * l) * l));
+  }
+  return v;
+}
+// The largest that the rounding of A_0, m half steps of fp64, can have become in the A of the last step. A step takes an eigenvalue l to
+// l q(l)^2, q(l) = a + b l + c l^2, and an error there to q(l) (a + 3 b l + 5 c l^2) times itself (outside the eigenvalues' range, next to
+// zero, to q(l)^2). Low-rank matrices on which this was tried in fp64: where the bound is 1e-3 (eleven steps of 3.4445, -4.7750, 2.0315)
+// the result is off by 3e-9, at 8e4 (18 steps) by 5e3, then infinite.
+static double orth_error_growth(const OrthArgs& o) {
+  double err = (double)std::min(o.rows, o.cols) * 0x1p-53, bound = 1.0;
+  for (int t = 0; t + 1 < o.steps; ++t) {
+    const double a = o.coef[3 * t], b = o.coef[3 * t + 1], c = o.coef[3 * t + 2], L = bound * bound;
+    const double q = largest_quadratic(a, b, c, L), dp = largest_quadratic(a, 3 * b, 5 * c, L);
+    err *= std::max(1.0, q * std::max(q, dp));
+    bound = orth_step_bound(a, b, c, bound);
+  }
+  return err;
+}
+
 bool orth_is_small(const OrthArgs& o) {
   const int64_t m = std::min(o.rows, o.cols), n = std::max(o.rows, o.cols), ld = std::max(o.ldx, o.ldy);
-  return o.steps <= MAX_RIDE && (n <= 128 || m <= 64) && ld < ((int64_t)1 << 25);
+  if (o.steps > MAX_RIDE || ld >= ((int64_t)1 << 25)) return false;
+  return n <= 128 || (m <= 64 && orth_error_growth(o) < 0x1p-8);
 }
 
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws_bytes, int64_t* need) {

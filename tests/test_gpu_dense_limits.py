@@ -1,0 +1,71 @@
+"""MI355X: the dense operators on device tensors where their ranges end -- long schedules on low-rank matrices, magnitudes near the types'
+limits, addresses off 16 bytes in the tiled kernels, parts of a gradient -- against their definitions in 64 bits."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_dense import BF16, F16, F32, POLAR, TYPES, U, UPDATE, gen_for, ints, orth64, orth_bound, padded  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dense():
+    from sclens_amd import dense as d
+
+    return d
+
+
+# ---------------------------------------------------------------------------------------------------------- orthogonalize
+LOW_RANK = [(40, 2000, 20), (2000, 40, 20), (64, 1500, 8), (30, 1200, 29), (64, 4096, 32)]
+
+
+def low_rank(g, rows, cols, rank, dtype):
+    """whole numbers that every type holds: the singular values behind `rank` are exactly zero"""
+    x = ints(g, (rows, rank), F32, 1).double() @ ints(g, (rank, cols), F32, 1).double()
+    assert x.abs().max() <= 256 if dtype is BF16 else 2048
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,rank", LOW_RANK)
+@pytest.mark.parametrize("steps", [8, 11, 12, 17, 18, 20, 24])
+def test_orthogonalize_low_rank_many_steps(dense, steps, rows, cols, rank, dtype):
+    """A step takes every singular value of 0 .. 1.2024 into 0 .. 1.2024 (the largest value of p there). Roundings fill the empty directions and
+    grow like any small singular value, so the bound holds for them too, but for those of the last steps: a step rounds x, A and P by u
+    and its sums by 2 (sqrt(n) + 3) 2^-24, three times, each a matrix of norm below u |x|_F <= u 1.21 sqrt(m) times |P| <= 3.4445, and the
+    result by u of its type. |p'| <= 3.4445 lifts what one step leaves over the bound by that much in the next, where p itself
+    (p' < 0 at 1.2024 down to 0.7, p(1.2024) < 1) brings it back: twice the rounding of a step is allowed."""
+    g = gen_for("low rank", rows, cols, rank)
+    x = low_rank(g, rows, cols, rank, dtype)
+    y = dense.orthogonalize(x, coefficients=[UPDATE[0]] * steps)
+    assert torch.isfinite(y).all()
+    u = 2.0 ** -11 if dtype is not F32 else 2.0 ** -23
+    m, n = min(rows, cols), max(rows, cols)
+    per_step = 3 * (u + 2 * (math.sqrt(n) + 3) * 2.0 ** -24) * 3.4445 * 1.21 * math.sqrt(m)
+    top = torch.linalg.svdvals(y.double().cpu()).max().item()
+    assert top <= 1.2024 + 2 * 3.4445 * per_step + U[dtype] * 1.21 * math.sqrt(m), top
+    if steps <= 11:  # few enough that the roundings in the empty directions have not grown to one
+        off = (y.double() - orth64(x, [UPDATE[0]] * steps)).norm().cpu()
+        assert off <= orth_bound(x, [UPDATE[0]] * steps, dtype), off
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,rows,cols", [(1, 1, 3000), (2, 3000, 1), (3, 9, 500), (2, 500, 17), (130, 40, 200)])
+def test_orthogonalize_many_steps_of_short_sides(dense, batch, rows, cols, dtype):
+    """full rank, a schedule that converges: whichever path takes it, x' x is the identity up to the last step's roundings"""
+    g = gen_for("many short", batch, rows, cols)
+    k = min(rows, cols)
+    q = torch.linalg.qr(torch.randn(batch, max(rows, cols), k, generator=g, device="cuda").double().cpu())[0]
+    x = q * torch.linspace(1, 2, k, dtype=torch.float64)
+    x = (x.transpose(-1, -2) if rows < cols else x).contiguous().to("cuda", dtype)
+    y = dense.orthogonalize(x, coefficients=UPDATE[:3] + [POLAR[-1]] * 20).double()
+    gram = y @ y.transpose(-1, -2).contiguous() if rows < cols else y.transpose(-1, -2).contiguous() @ y
+    off = (gram - torch.eye(k, device="cuda", dtype=torch.float64)).flatten(1).norm(dim=1).max().item()
+    # x = a x + P x: the roundings of its products (fp16 for 16-bit types, sums of max(rows, cols) terms) and of the result, each at most half a
+    # step of entries whose norm is sqrt(k); a = 1.875, |P| <= 1.875, and x' x is off by twice their sum
+    u = U[F32] if dtype is F32 else U[F16]
+    acc = 2 * (math.sqrt(max(rows, cols)) + 3) * 2.0 ** -24
+    assert off <= 2 * math.sqrt(k) * (U[dtype] + 1.875 * 4 * (u + acc)), off
