@@ -69,3 +69,17 @@ def test_orthogonalize_many_steps_of_short_sides(dense, batch, rows, cols, dtype
     u = U[F32] if dtype is F32 else U[F16]
     acc = 2 * (math.sqrt(max(rows, cols)) + 3) * 2.0 ** -24
     assert off <= 2 * math.sqrt(k) * (U[dtype] + 1.875 * 4 * (u + acc)), off
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,rank", LOW_RANK)
+@pytest.mark.parametrize("steps", [5, 8, 9, 10, 11])
+def test_orthogonalize_low_rank_short_side(dense, steps, rows, cols, rank, dtype):
+    """The m x m side in fp64: A_0 is off by at most m 2^-53, which grows by at most a^2 in a step, 1.1 times that in sum; P is off by (|b| + 2 |c| |A|)
+    times it, |A| <= 1.45 (10.7), on an x of norm at most 1.21. The result is rounded to fp32 and to its type."""
+    x = low_rank(gen_for("low rank", rows, cols, rank), rows, cols, rank, dtype)
+    y, want = dense.orthogonalize(x, coefficients=[UPDATE[0]] * steps).double(), orth64(x, [UPDATE[0]] * steps)
+    tol = 1.01 * (U[dtype] + 2.0 ** -24) * want.norm() + 1.1 * 1.21 * 10.7 * min(rows, cols) * 2.0 ** -53 * 3.4445 ** (2 * (steps - 1))
+    if dtype is F16:  # (entries below its normal numbers)
+        tol = tol + 2.0 ** -25 * math.sqrt(rows * cols)
+    assert (y - want).norm() <= tol, ((y - want).norm().item(), tol.item())
