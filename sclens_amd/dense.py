@@ -6,7 +6,8 @@ each other (`orthogonalize` of `corr_mat(V1, V2)`).
 
 Element types are torch.bfloat16, torch.float16 and torch.float32; sums are held in 32 bits and rounded once. Calls are queued on the
 tensors' device on torch's current stream of that device; they neither block nor synchronise, and can be captured into a graph after one
-eager call of the same thread (which creates the thread's context). They record no autograd graph: gradients are the explicit call.
+eager call of the same thread (which creates the thread's context). They record no autograd graph and propagate no tangents (tensors that ask
+for either are refused): gradients are the explicit call.
 
 torch has to be imported before the library is first used (importing this module does it): both then run on one HIP runtime and torch's
 streams are valid for the library.
@@ -18,6 +19,7 @@ import threading
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Context
@@ -51,14 +53,22 @@ def _context(index: int, ctx: Optional[Context]) -> Context:
     return ctx
 
 
+def _no_graph(name: str, t: torch.Tensor) -> None:
+    """neither of autograd's modes: a result of these calls would lack its graph or its tangent in silence"""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
+    # (inside a dual level only: unpacking costs as much as all other checks of a tensor)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent: these operators propagate none")
+
+
 def _first(name: str, t) -> int:
     """checks of the tensor that sets the element type and the device; its device's index"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} has to be a torch tensor")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name}: element type {t.dtype} (bfloat16, float16 or float32 expected)")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
+    _no_graph(name, t)
     if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}, expected a GPU")
     return t.get_device()
@@ -71,8 +81,7 @@ def _other(name: str, t, like: torch.Tensor, index: int, shape) -> None:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: these operators record no graph (torch.no_grad() and the explicit gradient)")
+    _no_graph(name, t)
 
 
 def _ld(name: str, t: torch.Tensor) -> int:

@@ -98,3 +98,31 @@ def test_library_loaded_before_torch_is_refused(monkeypatch):
         dense._context(0, Ctx())
     with pytest.raises(ValueError, match="context on device"):
         dense._context(1, Ctx())
+
+
+def test_forward_mode_tangents_are_refused():
+    """a dual tensor does not require a gradient: its tangent would be dropped in silence"""
+    from torch.autograd import forward_ad
+
+    calls = [
+        (lambda d: dense.linear(d(2, 3), g(4, 3)), "x carries"),
+        (lambda d: dense.linear(g(2, 3), d(4, 3)), "weight carries"),
+        (lambda d: dense.linear(g(2, 3), g(4, 3), bias=d(4)), "bias carries"),
+        (lambda d: dense.linear(g(2, 3), g(4, 3), residual=d(2, 4)), "residual carries"),
+        (lambda d: dense.linear_backward(d(2, 4), g(2, 3), g(4, 3)), "grad carries"),
+        (lambda d: dense.linear_backward(g(2, 4), d(2, 3), g(4, 3)), "x carries"),
+        (lambda d: dense.linear_backward(g(2, 4), g(2, 3), d(4, 3)), "weight carries"),
+        (lambda d: dense.linear_backward(g(2, 4), g(2, 3), g(4, 3), preact=d(2, 4), activation="silu"), "preact carries"),
+        (lambda d: dense.orthogonalize(d(5, 6)), "x carries"),
+    ]
+    with forward_ad.dual_level():
+        def dual(*shape):
+            v = forward_ad.make_dual(g(*shape), torch.ones(shape))
+            assert v.is_cuda and not v.requires_grad
+            return v
+
+        for call, text in calls:
+            with pytest.raises(ValueError, match=text):
+                call(dual)
+            with torch.no_grad(), pytest.raises(ValueError, match=text):  # no_grad does not switch tangents off
+                call(dual)
