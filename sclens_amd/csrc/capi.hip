@@ -317,7 +317,6 @@ struct DeviceScope {
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
     if (prev != device) (void)hipSetDevice(device);
     else prev = -1;
-    (void)hipGetLastError();  // an error another library left behind is not this call's
   }
   ~DeviceScope() {
     if (prev >= 0) (void)hipSetDevice(prev);

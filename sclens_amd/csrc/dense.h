@@ -5,6 +5,19 @@
 
 namespace scl {
 
+// A launch with its own status. (The runtime keeps one last error per thread: reading it after a launch would take, and report as this call's, one
+// that the host framework has left there and not read yet.)
+template <class T> struct Given { typedef T type; };
+template <class... P>
+int run_kernel(Ctx* ctx, void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t st, typename Given<P>::type... args) {
+  void* at[] = {static_cast<void*>(&args)...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, at, lds, st);
+  if (e != hipSuccess) (void)hipGetLastError();  // reported by this call's code
+  SCL_HIP(ctx, e);
+  return SCLENS_OK;
+}
+#define SCL_RUN(ctx, ...) SCL_TRY((run_kernel(ctx, __VA_ARGS__)))
+
 // element types of the C ABI (SCLENS_DTYPE_*); D_PL3 is internal: an fp32 value held as three bf16 pieces in three planes
 enum { D_F32 = 0, D_BF16 = 1, D_F16 = 2, D_PL3 = 3 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };

@@ -749,8 +749,7 @@ int launch(Ctx* ctx, hipStream_t st, const ProdArgs& g, dim3 grid) {
   static_assert(LDS <= 163840, "LDS of a CU");
   const void* fn = reinterpret_cast<const void*>(k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, SA, SB>);
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, fn, LDS));
-  hipLaunchKernelGGL((k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, SA, SB>), grid, dim3(WM * WN * 64), LDS, st, g);
-  SCL_HIP(ctx, hipGetLastError());
+  SCL_RUN(ctx, k_product<MT, OT, RT, PART, AC, BC, WM, WN, TM, TN, SA, SB>, grid, dim3(WM * WN * 64), LDS, st, g);
   return SCLENS_OK;
 }
 template <int MT, int OT, int RT, bool PART, bool AC, bool BC>
@@ -771,8 +770,7 @@ int launch_types(Ctx* ctx, hipStream_t st, const ProdArgs& g, const Plan& pl) {
   if (pl.ksplit == 1) return launch_tile<MT, OT, RT, false, AC, BC>(ctx, st, g, grid, pl.tile);
   SCL_TRY((launch_tile<MT, D_F32, D_F32, true, AC, BC>(ctx, st, g, grid, pl.tile)));
   const int64_t blocks = ((g.p.M + 31) / 32) * ((g.p.N + 63) / 64);
-  hipLaunchKernelGGL((k_product_join<OT, RT, MT == D_PL3>), dim3((unsigned)blocks, (unsigned)g.p.batch), dim3(256), 0, st, g);
-  SCL_HIP(ctx, hipGetLastError());
+  SCL_RUN(ctx, k_product_join<OT, RT, MT == D_PL3>, dim3((unsigned)blocks, (unsigned)g.p.batch), dim3(256), 0, st, g);
   return SCLENS_OK;
 }
 
@@ -832,10 +830,9 @@ int product_join(Ctx* ctx, hipStream_t st, const Product& p, int slices) {
   g.p = p;
   g.ksplit = slices;
   const dim3 grid((unsigned)(((p.M + 31) / 32) * ((p.N + 63) / 64)), (unsigned)p.batch), blk(256);
-  if (p.out_type == D_F32) hipLaunchKernelGGL((k_product_join<D_F32, D_F32, false>), grid, blk, 0, st, g);
-  else if (p.out_type == D_BF16) hipLaunchKernelGGL((k_product_join<D_BF16, D_BF16, false>), grid, blk, 0, st, g);
-  else hipLaunchKernelGGL((k_product_join<D_F16, D_F16, false>), grid, blk, 0, st, g);
-  SCL_HIP(ctx, hipGetLastError());
+  if (p.out_type == D_F32) SCL_RUN(ctx, k_product_join<D_F32, D_F32, false>, grid, blk, 0, st, g);
+  else if (p.out_type == D_BF16) SCL_RUN(ctx, k_product_join<D_BF16, D_BF16, false>, grid, blk, 0, st, g);
+  else SCL_RUN(ctx, k_product_join<D_F16, D_F16, false>, grid, blk, 0, st, g);
   return SCLENS_OK;
 }
 
@@ -909,7 +906,7 @@ namespace {
 int launch_pack(Ctx* ctx, hipStream_t st, int dtype, int image, bool transposed, const PackSource& first, const PackSource& second, int64_t K) {
   const int64_t n1 = (first.rows + 63) / 64, n2 = (second.rows + 63) / 64;
   const dim3 grid((unsigned)(image_ld(K) / 64), (unsigned)(n1 + n2)), block(256);
-#define SCL_PACK(T, I, TR) hipLaunchKernelGGL((k_pack<T, I, TR>), grid, block, 0, st, first, second, (int)n1, K)
+#define SCL_PACK(T, I, TR) SCL_RUN(ctx, k_pack<T, I, TR>, grid, block, 0, st, first, second, (int)n1, K)
   if (image == D_PL3 && transposed) SCL_PACK(D_F32, D_PL3, true);
   else if (image == D_PL3) SCL_PACK(D_F32, D_PL3, false);
   else if (transposed) return ctx->fail(SCLENS_ERR_ARG, "pack_image: transposed only into planes");
@@ -917,7 +914,6 @@ int launch_pack(Ctx* ctx, hipStream_t st, int dtype, int image, bool transposed,
   else if (dtype == D_BF16) SCL_PACK(D_BF16, D_BF16, false);
   else SCL_PACK(D_F16, D_F16, false);
 #undef SCL_PACK
-  SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
 PackSource pack_source(int dtype, const void* src, int64_t ld, bool transposed, int64_t rows, int64_t K, Mat* img) {

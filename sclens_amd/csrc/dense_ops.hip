@@ -274,18 +274,16 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
     Mat img = as_is ? Mat() : dz;
     const dim3 grid((unsigned)blocks), blk(256);
-    if (planes) hipLaunchKernelGGL(k_dz_planes, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
-    else if (a.dtype == D_F32) hipLaunchKernelGGL(k_dz<D_F32>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_dz<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    else hipLaunchKernelGGL(k_dz<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    SCL_HIP(ctx, hipGetLastError());
+    if (planes) SCL_RUN(ctx, k_dz_planes, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
+    else if (a.dtype == D_F32) SCL_RUN(ctx, k_dz<D_F32>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else if (a.dtype == D_BF16) SCL_RUN(ctx, k_dz<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else SCL_RUN(ctx, k_dz<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
   }
   if (a.db && a.N > 0) {
     const dim3 grid((unsigned)((a.N + 63) / 64));
-    if (a.dtype == D_F32) hipLaunchKernelGGL(k_colsum_join<D_F32>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<float*>(a.db));
-    else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_colsum_join<D_BF16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
-    else hipLaunchKernelGGL(k_colsum_join<D_F16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
-    SCL_HIP(ctx, hipGetLastError());
+    if (a.dtype == D_F32) SCL_RUN(ctx, k_colsum_join<D_F32>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<float*>(a.db));
+    else if (a.dtype == D_BF16) SCL_RUN(ctx, k_colsum_join<D_BF16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
+    else SCL_RUN(ctx, k_colsum_join<D_F16>, grid, dim3(256), 0, st, part, nmb, a.N, static_cast<unsigned short*>(a.db));
   }
   if (!planes && a.K > 0) {
     const bool copy_w = a.dx && a.M > 0 && !w_as_is, copy_x = a.dw && a.N > 0 && !x_as_is;
@@ -475,15 +473,14 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     const Mat i0 = tall && f32 ? XT[0] : X[0], i1 = tall && f32 ? X[0] : XT[0];
 #define SCL_START(T, I)                                                                                                             \
   do {                                                                                                                              \
-    hipLaunchKernelGGL(k_sumsq<T>, g1, blk, 0, st, src, a.rows, a.cols, tpr, part);                                                 \
-    hipLaunchKernelGGL((k_orth_start<T, I>), g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
+    SCL_RUN(ctx, k_sumsq<T>, g1, blk, 0, st, src, a.rows, a.cols, tpr, part);                                                 \
+    SCL_RUN(ctx, k_orth_start<T, I>, g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
   } while (0)
     if (f32) SCL_START(D_F32, D_PL3);
     else if (wide) SCL_START(D_F32, D_F32);
     else if (a.dtype == D_BF16) SCL_START(D_BF16, D_F16);
     else SCL_START(D_F16, D_F16);
 #undef SCL_START
-    SCL_HIP(ctx, hipGetLastError());
   }
   for (int t = 0; t < a.steps; ++t) {
     const double ca = a.coef[3 * t], cb = a.coef[3 * t + 1], cc = a.coef[3 * t + 2];

@@ -506,24 +506,22 @@ int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   const unsigned batch = (unsigned)a.o.batch;
   if (a.slices == 1) {
     if (LDS_ALL > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_small<T, MT>), LDS_ALL));
-    hipLaunchKernelGGL((k_orth_small<T, MT>), dim3(batch), dim3(512), LDS_ALL, st, a, cf);
+    SCL_RUN(ctx, k_orth_small<T, MT>, dim3(batch), dim3(512), LDS_ALL, st, a, cf);
   } else {
     if (LDS_STEPS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_steps<MT>), LDS_STEPS));
-    hipLaunchKernelGGL((k_orth_gram<T, MT>), dim3((unsigned)a.slices, batch), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_orth_gram_sum, dim3(NL * 8, batch), dim3(1024), 0, st, a.part, a.slices, NL * 256, a.gram);
-    hipLaunchKernelGGL((k_orth_steps<MT>), dim3(batch), dim3(512), LDS_STEPS, st, a, cf);
+    SCL_RUN(ctx, k_orth_gram<T, MT>, dim3((unsigned)a.slices, batch), dim3(256), 0, st, a);
+    SCL_RUN(ctx, k_orth_gram_sum, dim3(NL * 8, batch), dim3(1024), 0, st, a.part, a.slices, NL * 256, a.gram);
+    SCL_RUN(ctx, k_orth_steps<MT>, dim3(batch), dim3(512), LDS_STEPS, st, a, cf);
     const int64_t chunks = (a.n + 63) / 64, per = std::max<int64_t>(1, chunks * batch / 768);
-    hipLaunchKernelGGL((k_orth_apply<T, MT>), dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
+    SCL_RUN(ctx, k_orth_apply<T, MT>, dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
   }
-  SCL_HIP(ctx, hipGetLastError());
   return SCLENS_OK;
 }
 template <int T, int MT>
 int run_direct(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   constexpr int LDS = 2 * 16 * MT * (16 * MT + 4) * 4 + 64;
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_direct<T, MT>), LDS));
-  hipLaunchKernelGGL((k_orth_direct<T, MT>), dim3((unsigned)a.o.batch), dim3(512), LDS, st, a, cf);
-  SCL_HIP(ctx, hipGetLastError());
+  SCL_RUN(ctx, k_orth_direct<T, MT>, dim3((unsigned)a.o.batch), dim3(512), LDS, st, a, cf);
   return SCLENS_OK;
 }
 template <int T>

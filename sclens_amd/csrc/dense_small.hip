@@ -151,10 +151,9 @@ bool backward_is_small(const LinearBwdArgs& a) { return std::max(a.M, a.N) <= 38
 
 int linear_small(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
   const dim3 grid((unsigned)(((a.M + 31) / 32) * ((a.N + 31) / 32))), blk(256);
-  if (a.dtype == D_F32) hipLaunchKernelGGL(k_small_linear<D_F32>, grid, blk, 0, st, a);
-  else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_small_linear<D_BF16>, grid, blk, 0, st, a);
-  else hipLaunchKernelGGL(k_small_linear<D_F16>, grid, blk, 0, st, a);
-  SCL_HIP(ctx, hipGetLastError());
+  if (a.dtype == D_F32) SCL_RUN(ctx, k_small_linear<D_F32>, grid, blk, 0, st, a);
+  else if (a.dtype == D_BF16) SCL_RUN(ctx, k_small_linear<D_BF16>, grid, blk, 0, st, a);
+  else SCL_RUN(ctx, k_small_linear<D_F16>, grid, blk, 0, st, a);
   return SCLENS_OK;
 }
 int backward_small(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a) {
@@ -162,10 +161,9 @@ int backward_small(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a) {
   const int64_t ndb = a.db ? (a.N + 31) / 32 : 0, all = ndx + ndw + ndb;
   if (all == 0) return SCLENS_OK;
   const dim3 grid((unsigned)all), blk(256);
-  if (a.dtype == D_F32) hipLaunchKernelGGL(k_small_backward<D_F32>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
-  else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_small_backward<D_BF16>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
-  else hipLaunchKernelGGL(k_small_backward<D_F16>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
-  SCL_HIP(ctx, hipGetLastError());
+  if (a.dtype == D_F32) SCL_RUN(ctx, k_small_backward<D_F32>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
+  else if (a.dtype == D_BF16) SCL_RUN(ctx, k_small_backward<D_BF16>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
+  else SCL_RUN(ctx, k_small_backward<D_F16>, grid, blk, 0, st, a, (int)ndx, (int)ndw);
   return SCLENS_OK;
 }
 

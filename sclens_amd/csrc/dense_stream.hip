@@ -115,10 +115,9 @@ __global__ __launch_bounds__(512) void k_rows(LinearArgs a) {
 
 int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
   const dim3 grid((unsigned)((a.N + 15) / 16)), blk(512);
-  if (a.dtype == D_F32) hipLaunchKernelGGL(k_rows<D_F32>, grid, blk, 0, st, a);
-  else if (a.dtype == D_BF16) hipLaunchKernelGGL(k_rows<D_BF16>, grid, blk, 0, st, a);
-  else hipLaunchKernelGGL(k_rows<D_F16>, grid, blk, 0, st, a);
-  SCL_HIP(ctx, hipGetLastError());
+  if (a.dtype == D_F32) SCL_RUN(ctx, k_rows<D_F32>, grid, blk, 0, st, a);
+  else if (a.dtype == D_BF16) SCL_RUN(ctx, k_rows<D_BF16>, grid, blk, 0, st, a);
+  else SCL_RUN(ctx, k_rows<D_F16>, grid, blk, 0, st, a);
   return SCLENS_OK;
 }
 
@@ -264,8 +263,7 @@ template <int T, int NT>
 int launch_stream(Ctx* ctx, hipStream_t st, const StreamArgs& a, int slices) {
   constexpr int LDS = stream_depth(NT) * (T == D_F32 ? 3 : 1) * NT * 16 * 128;
   if (LDS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_stream<T, NT>), LDS));
-  hipLaunchKernelGGL((k_stream<T, NT>), dim3((unsigned)((a.R + 255) / 256), (unsigned)slices), dim3(512), LDS, st, a);
-  SCL_HIP(ctx, hipGetLastError());
+  SCL_RUN(ctx, k_stream<T, NT>, dim3((unsigned)((a.R + 255) / 256), (unsigned)slices), dim3(512), LDS, st, a);
   return SCLENS_OK;
 }
 template <int T>

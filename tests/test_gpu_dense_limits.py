@@ -83,3 +83,32 @@ def test_orthogonalize_low_rank_short_side(dense, steps, rows, cols, rank, dtype
     if dtype is F16:  # (entries below its normal numbers)
         tol = tol + 2.0 ** -25 * math.sqrt(rows * cols)
     assert (y - want).norm() <= tol, ((y - want).norm().item(), tol.item())
+
+
+# ---------------------------------------------------------------------------------------------------------- beside other libraries
+def test_an_error_that_somebody_else_has_left_stays_theirs(dense):
+    """the runtime keeps one last error per thread: a call of this library neither reports it as its own nor takes it away"""
+    lib = dense.Context(0).lib
+    for name in ("hipSetDevice", "hipPeekAtLastError", "hipGetLastError"):
+        getattr(lib, name).restype = int
+    g = gen_for("pending")
+    small, big = ints(g, (40, 40), F32, 2), ints(g, (600, 1040), BF16, 1)
+    grad = ints(g, (600, 600), BF16, 1)
+
+    def calls():
+        return (dense.linear(small, small), dense.linear(small[:3], small), dense.linear(big, big), *dense.linear_backward(grad, big, big),
+                *dense.linear_backward(small, small, small), dense.orthogonalize(small), dense.orthogonalize(big), dense.orthogonalize(big[:40]))
+
+    want = calls()
+    torch.cuda.synchronize()
+    lib.hipGetLastError()
+    assert lib.hipSetDevice(9999) == 101  # refused by the runtime on the host; nothing has happened on the device
+    got = []
+    try:
+        got = calls()
+        pending = lib.hipPeekAtLastError()
+    finally:
+        lib.hipGetLastError()
+    assert pending == 101
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
