@@ -234,7 +234,8 @@ int sclens_hip_linear(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, i
                       void* preact, int64_t ldz, void* ws, int64_t* ws_bytes);
 /* Its gradients: dz = dy * act'(preact) (preact may be NULL for SCLENS_ACT_NONE; relu'(0) = 0), dx = dz w, dw = dz' x, dbias = column
  * sums of dz; the residual's gradient is dy. dx / dw / dbias may be NULL: not computed (x is then only read for dw, w for dx). For
- * 16-bit types dz is rounded to that type before the two products. Every sum runs in a fixed order: equal inputs give equal bits. */
+ * 16-bit types dz is rounded to that type before the two products. Every sum runs in a fixed order: equal inputs give equal bits, whichever
+ * of the three are asked for. */
 int sclens_hip_linear_backward(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* dy,
                                int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* preact, int64_t ldz,
                                int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias, void* ws, int64_t* ws_bytes);

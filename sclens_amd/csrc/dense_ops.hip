@@ -244,9 +244,10 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   if (a.N > (a.dtype == D_F32 && a.dx ? MAX_CONTRACTION_F32 : MAX_CONTRACTION) || a.K > MAX_CONTRACTION)
     return ctx->fail(SCLENS_ERR_ARG, "linear_backward: more than 2^25 columns (2^24 in an fp32 dx)");
   Carve c(ws);
-  // fp32 in planes if both products together gain by it (dz both ways, w and x are taken apart)
-  const bool planes = a.dtype == D_F32 && a.dx && a.dw && a.M <= MAX_CONTRACTION && planes_pay(a.M, a.K, a.N, 2 * a.M * a.N / 2 + a.N * a.K) &&
-                      planes_pay(a.N, a.K, a.M, 2 * a.M * a.N / 2 + a.M * a.K);
+  // fp32 in planes if each of the two products gains by it (dz, w and x are taken apart), whichever of them is asked for: a part of the gradients has
+  // the bits that it has among all of them
+  const bool planes = a.dtype == D_F32 && a.M <= MAX_CONTRACTION && planes_pay(a.M, a.K, a.N, a.M * a.N + a.N * a.K) &&
+                      planes_pay(a.N, a.K, a.M, a.M * a.N + a.M * a.K);
   const int image = planes ? D_PL3 : a.dtype;
   const bool as_is = !planes && a.act == ACT_NONE && direct(a.dtype, a.dy, a.lddy, a.N);  // dz is dy
   const int rows_per = planes ? 64 : DZ_ROWS, cols_per = planes ? 64 : 128;

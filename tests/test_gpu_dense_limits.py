@@ -112,3 +112,19 @@ def test_an_error_that_somebody_else_has_left_stays_theirs(dense):
     assert pending == 101
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------------------------ gradients
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(300, 40, 64), (700, 93, 510), (2304, 2176, 2048), (4096, 1024, 1000)])
+def test_parts_of_a_gradient_have_the_bits_of_the_whole(dense, M, K, N, dtype):
+    """one launch, tiles as the matrices lie, and (fp32) three planes"""
+    g = gen_for("parts", M, K, N)
+    x, w, dy, z = (torch.randn(*s, generator=g, device="cuda").to(dtype) for s in ((M, K), (N, K), (M, N), (M, N)))
+    dx, dw, db = dense.linear_backward(dy, x, w, preact=z, activation="silu")
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)):
+        got = dense.linear_backward(dy, x if need[1] else None, w if need[0] else None, preact=z, activation="silu", need_x=bool(need[0]),
+                                    need_weight=bool(need[1]), need_bias=bool(need[2])) if need[0] or need[1] else \
+            dense.linear_backward(dy, x, w, preact=z, activation="silu", need_x=False, need_weight=False)
+        for part, whole, wanted in zip(got, (dx, dw, db), need):
+            assert part is None if not wanted else torch.equal(part, whole), need
