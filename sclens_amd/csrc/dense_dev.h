@@ -185,18 +185,21 @@ __device__ __forceinline__ float normal_tail(float az, float* e) {
   p = fmaf(p, t, 0.16918801f);
   return 0.5f * *e * t * p;
 }
+// At infinities the limits: z times a sigmoid that is zero, and z times 1 - sigmoid, are zero there and not NaN. (A saved fp16 argument of 65 520 is
+// infinite already.) Nothing is clamped that is finite, and NaN stays NaN through the other factor.
+constexpr float LARGEST = 3.40282347e38f;
 // beyond 14 the tail is below 1e-43: the clamp keeps infinity times zero away
 __device__ __forceinline__ float tail_arg(float z) { return fminf(fabsf(z), 14.f); }
 template <int ACT>
 __device__ __forceinline__ float act_apply(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (NaN stays)
-  if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == ACT_SILU) return fmaxf(z, -LARGEST) * sigmoid(z);
   if constexpr (ACT == ACT_GELU) {
     float e;
     const float az = tail_arg(z), q = normal_tail(az, &e);
     return (z < 0.f ? 0.f : z) - az * q;
   }
-  if constexpr (ACT == ACT_GELU_TANH) return z * sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
+  if constexpr (ACT == ACT_GELU_TANH) return fmaxf(z, -LARGEST) * sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
   return z;
 }
 template <int ACT>
@@ -204,7 +207,7 @@ __device__ __forceinline__ float act_grad(float z) {
   if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
   if constexpr (ACT == ACT_SILU) {
     const float s = sigmoid(z);
-    return s * (1.f + z * (1.f - s));
+    return s * (1.f + __builtin_amdgcn_fmed3f(z, -LARGEST, LARGEST) * (1.f - s));
   }
   if constexpr (ACT == ACT_GELU) {
     float e;
@@ -212,6 +215,8 @@ __device__ __forceinline__ float act_grad(float z) {
     return (z > 0.f ? 1.f - q : q) + zc * 0.39894228f * e;
   }
   if constexpr (ACT == ACT_GELU_TANH) {
+    // from |z| = 12 the sigmoid is 0 or 1 to the last bit; z z, which overflows at 1.8e19, would meet 1 - s = 0
+    z = z != z ? z : fminf(fmaxf(z, -12.f), 12.f);
     const float s = sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
     return s + z * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * z * z);
   }

@@ -114,6 +114,101 @@ def test_an_error_that_somebody_else_has_left_stays_theirs(dense):
         assert torch.equal(a, b)
 
 
+# ---------------------------------------------------------------------------------------------------------------- activations
+ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def ends_of(dtype):
+    """infinities, NaN, the type's largest and smallest values, the places where exponentials leave fp32 and where clamps begin"""
+    big, tiny = torch.finfo(dtype).max, torch.finfo(dtype).tiny
+    v = [0.0, tiny, 1e-3, 0.5, 1.0, 3.0, 5.5, 9.0, 9.9, 11.5, 12.5, 13.9, 14.1, 15.0, 40.0, 86.0, 88.5, 89.0, 103.0, 105.0, 200.0, 1e4, 6e4, 1e6,
+         1e12, 1.5e13, 1e18, 1.7e19, 2e19, 1e30, 1e38, big, math.inf]
+    z = torch.tensor([s * t for t in v for s in (1, -1)] + [math.nan], dtype=torch.float64).to(dtype)
+    return z.cuda()
+
+
+def normal_cdf(z):
+    """(torch.special.ndtr is 1 + erf, zero from -8.3 on)"""
+    return 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+
+
+def act_limits(z, kind):
+    """in 64 bits, the limits at infinities"""
+    if kind == "none":
+        return z
+    if kind == "relu":
+        return torch.where(z < 0, torch.zeros_like(z), z)
+    c = z.clamp(-1e150, 1e150)  # (infinities too; NaN stays)
+    if kind == "gelu":
+        s = normal_cdf(c)
+    else:
+        s = torch.sigmoid(c if kind == "silu" else 2 * math.sqrt(2 / math.pi) * (c + 0.044715 * c.clamp(-1e3, 1e3) ** 3))
+    return torch.where(z == math.inf, z, c * s)
+
+
+def act_grad_limits(z, kind):
+    c = z.clamp(-1e3, 1e3)  # every derivative is 0 or 1 to the last bit there
+    if kind == "relu":
+        return torch.where(z.isnan(), z, (z > 0).double())
+    if kind == "silu":
+        s = torch.sigmoid(c)
+        return s * (1 + c * (1 - s))
+    if kind == "gelu":
+        return normal_cdf(c) + c * torch.exp(-0.5 * c * c) / math.sqrt(2 * math.pi)
+    k2 = 2 * math.sqrt(2 / math.pi)
+    s = torch.sigmoid(k2 * (c + 0.044715 * c ** 3))
+    return s + c * s * (1 - s) * k2 * (1 + 0.134145 * c * c)
+
+
+def assert_close_or_same(got, want, tol, dtype):
+    """non-finite results are the ones that the rounded exact result has; finite ones are within tol"""
+    rounded = want.to(dtype).double()
+    assert torch.equal(got.isnan(), rounded.isnan()), (got, rounded)
+    inf = rounded.isinf() | got.isinf()
+    assert torch.equal(got[inf], rounded[inf])
+    ok = ((got - want).abs() <= tol) | inf | rounded.isnan()
+    assert ok.all(), (got[~ok], want[~ok])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,K,N", [(8, 8, 64), (40, 8, 64), (520, 1040, 264), (70, 3, 90)])
+def test_activations_at_their_ends(dense, M, K, N, act, dtype):
+    """x w' = z exactly (one column of x times one; the others zero), past few rows, in tiles, in one launch"""
+    z = ends_of(dtype)
+    col = z.repeat(M // z.numel() + 1)[:M] if M >= z.numel() else None
+    for first in range(0, z.numel(), M) if col is None else (0,):
+        c = (z[first: first + M] if col is None else col)
+        x = torch.zeros(c.numel(), K, dtype=dtype, device="cuda")
+        x[:, K // 2] = c
+        w = torch.zeros(N, K, dtype=dtype, device="cuda")
+        w[:, K // 2] = 1
+        got = dense.linear(x, w, activation=act).double()
+        zz = c.double()[:, None].expand(-1, N)
+        want = act_limits(zz, act)
+        # the activation in fp32: sigmoid and tail from exp2 of a rounded product, relative 2^-23 per unit of the exponent (at most 104 before
+        # the result is zero) and 16 roundings; absolute: below the smallest normal numbers of fp32, and what |z| times those is
+        rel = 2.0 ** -24 * (16 + 2 * 104)
+        e = want.abs() * rel + 2.0 ** -126 * (2 + zz.abs().clamp(max=200))
+        assert_close_or_same(got, want, e + U[dtype] * 1.01 * (want.abs() + e) + (2.0 ** -25 if dtype is F16 else 2.0 ** -126), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("N", [67, 400])
+def test_derivatives_at_their_ends(dense, N, act, dtype):
+    """one row of gradients: dbias is dz"""
+    z = ends_of(dtype).repeat(N // 60 + 1)[:N][None].contiguous()
+    dy = torch.full_like(z, 0.75)
+    x, w = torch.ones(1, 8, dtype=dtype, device="cuda"), torch.ones(N, 8, dtype=dtype, device="cuda")
+    _, _, db = dense.linear_backward(dy, x, w, preact=z, activation=act)
+    d = act_grad_limits(z.double(), act)[0]
+    # derivative in fp32: sigmoid to 2^-24 (16 + 2 |exponent|) of itself, times 1 + |z| terms that cancel: absolute, 32 units of (1 + |z|) where it
+    # has not reached 0 or 1 (|z| <= 110 for SiLU)
+    tol = 0.75 * 32 * 2.0 ** -24 * (1 + z.double()[0].abs().clamp(max=110))
+    assert_close_or_same(db.double(), 0.75 * d, tol + U[dtype] * 1.01 * (0.75 * d.abs() + tol) + (2.0 ** -25 if dtype is F16 else 0), dtype)
+
+
 # ------------------------------------------------------------------------------------------------------------------ gradients
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N", [(300, 40, 64), (700, 93, 510), (2304, 2176, 2048), (4096, 1024, 1000)])
