@@ -43,6 +43,7 @@ struct Product {
   int symmetric = 0;  // M == N and C is symmetric: tiles on / below the diagonal, mirrored
   // epilogue: v = alpha acc + bias[col]; pre = v; v = act(v) + beta res; out = v; outT (transposed) = v
   float alpha = 1.f, beta = 0.f;
+  const float* scale = nullptr;  // device: alpha times this
   int act = ACT_NONE;
   const void* bias = nullptr;
   Mat res, pre, out, outT;

@@ -73,10 +73,10 @@ __device__ __forceinline__ void wave_sync() {
 template <int OT, int RT>
 struct Epilogue {
   // 8 columns from col of row `row`, n of them inside (images with `pad`: all 8, those outside as zeros)
-  static __device__ __forceinline__ void apply(const Product& p, int64_t b, int64_t row, int64_t col, int nin, bool row_in, float v[8],
-                                               const float* bias8, const Raw8<RT>& res) {
+  static __device__ __forceinline__ void apply(const Product& p, float alpha, int64_t b, int64_t row, int64_t col, int nin, bool row_in,
+                                               float v[8], const float* bias8, const Raw8<RT>& res) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * p.alpha + bias8[e];
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * alpha + bias8[e];
     if (p.pre.p && row_in) store8<OT>(p.pre, b * p.pre.batch + row * p.pre.ld + col, nin, v);
     if (p.act != ACT_NONE) act8<false>(v, p.act);
     if (p.res.p && row_in && nin > 0) {
@@ -473,6 +473,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
       wave_sync();
     }
   } else {
+    const float alpha = p.scale ? p.alpha * *p.scale : p.alpha;
     float bias8[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bias8[e] = 0.f;
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
             float v[8];
             from_lds(s * RP + cr, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], p.alpha, bias8[e]);
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], alpha, bias8[e]);
             if (has_pre) {
               plain.p = pz;
               if (mine) store8<OT>(plain, 0, 8, v);
@@ -600,7 +601,7 @@ __global__ __launch_bounds__(WM* WN * 64, TM * TN >= 9 ? 1 : 2) void k_product(P
         }
         Raw8<RT> res;
         if (p.res.p && row_in && nin > 0) res.load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
-        Epilogue<OT, RT>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
+        Epilogue<OT, RT>::apply(p, alpha, batch, row, col, nin, row_in, v, bias8, res);
         if (p.out.p) {
           const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
           const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;
@@ -629,6 +630,7 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
   const int64_t row = row0 + lr, col = col0 + cc;
   const int nin = (int)max((int64_t)0, min((int64_t)8, p.N - col));
   const bool row_in = row < p.M;
+  const float alpha = p.scale ? p.alpha * *p.scale : p.alpha;
   float v[8], bias8[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = bias8[e] = 0.f;
@@ -657,7 +659,7 @@ __global__ __launch_bounds__(256) void k_product_join(ProdArgs g) {
   }
   Raw8<RT> res;
   if (p.res.p && row_in && nin > 0) res.load(p.res, batch * p.res.batch + row * p.res.ld + col, nin);
-  Epilogue<OT, RT>::apply(p, batch, row, col, nin, row_in, v, bias8, res);
+  Epilogue<OT, RT>::apply(p, alpha, batch, row, col, nin, row_in, v, bias8, res);
   if (p.out.p) {
     const int n = p.out.pad ? (nin > 0 ? 8 : 0) : nin;
     const bool rin = p.out.pad ? row < round_up8(p.M) : row_in;

@@ -124,10 +124,42 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
 // sums in fp32, before dz is rounded. dz in 16 bits is one rounding of half a step per element, as the saved
 // pre-activation and the gradient that comes in already are. Bound by HBM, two reads and a write per element: 8192 x 8192 bf16 77 us,
 // 5.2 TB/s.
-constexpr int DZ_ROWS = 64;
+// fp16, whose steps are relative between 6e-5 and 65504 only, holds dz under a power of two that brings the largest |dy| to 2^14 .. 2^15 (no
+// derivative exceeds 1.13): gradients of 1e-6 keep their eleven bits and those next to 65504 do not overflow. The products' epilogue takes
+// it out again (`unscale`). k_largest finds it, a read of dy more; ReLU's dz is dy or zero and goes without.
+constexpr int DZ_ROWS = 64, MAXIMA = 256;
+__global__ __launch_bounds__(256) void k_largest(Mat dy, int64_t rows, int64_t cols, int tpr, unsigned* __restrict__ maxima) {
+  __shared__ unsigned S[4];
+  const int tid = threadIdx.x, tr = tid / tpr, tc = (tid % tpr) * 8, rpb = 256 / tpr;
+  const int64_t step = (int64_t)gridDim.x * rpb;
+  unsigned top = 0;  // finite fp16 magnitudes are ordered as their bits
+  for (int64_t r = (int64_t)blockIdx.x * rpb + tr; r < rows; r += 4 * step)
+    for (int64_t c = tc; c < cols; c += 8 * tpr) {
+      const int n = (int)min((int64_t)8, cols - c);
+      Raw8<D_F16> q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r + i * step < rows) q[i].load(dy, (r + i * step) * dy.ld + c, n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r + i * step >= rows) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned h = q[i].r[0][e] & 0x7fffu;
+          if (h < 0x7c00u) top = max(top, h);
+        }
+      }
+    }
+  for (int w = 32; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
+  if ((tid & 63) == 0) S[tid >> 6] = top;
+  __syncthreads();
+  if (tid == 0) maxima[blockIdx.x] = max(max(S[0], S[1]), max(S[2], S[3]));
+}
 template <int T>
-__global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part) {
+__global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, int64_t N, Mat img, float* __restrict__ part,
+                                            const unsigned* __restrict__ maxima, int nmax, float* __restrict__ unscale) {
   __shared__ float L[16][132];
+  __shared__ unsigned S[4];
   const int64_t nb = (N + 127) / 128, mb = blockIdx.x / nb;
   const int64_t m0 = mb * DZ_ROWS, n0 = (blockIdx.x % nb) * 128;
   const int tid = threadIdx.x, cc = (tid & 15) * 8, r0 = tid >> 4;
@@ -136,9 +168,9 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
   float sum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  constexpr int NR = DZ_ROWS / 16;
+  Raw8<T> g[NR], zz[NR];  // all loads first
   if (nin > 0) {
-    constexpr int NR = DZ_ROWS / 16;
-    Raw8<T> g[NR], zz[NR];  // all loads first
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int64_t row = m0 + r0 + 16 * i;
@@ -147,6 +179,21 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
         if (act != ACT_NONE) zz[i].load(z, row * z.ld + col, nin);
       }
     }
+  }
+  float scale = 1.f;
+  if constexpr (T == D_F16) {
+    if (maxima) {
+      unsigned top = tid < nmax ? maxima[tid] : 0;
+      for (int w = 32; w > 0; w >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, w));
+      if ((tid & 63) == 0) S[tid >> 6] = top;
+      __syncthreads();
+      top = max(max(S[0], S[1]), max(S[2], S[3]));
+      const int k = top == 0 ? 0 : 14 - ilogbf(f16_to_f32((unsigned short)top));
+      scale = ldexpf(1.f, k);
+      if (blockIdx.x == 0 && tid == 0) *unscale = ldexpf(1.f, -k);
+    }
+  }
+  if (nin > 0) {
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int64_t row = m0 + r0 + 16 * i;
@@ -160,9 +207,13 @@ __global__ __launch_bounds__(256) void k_dz(Mat dy, Mat z, int act, int64_t M, i
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = e < nin ? v[e] * d[e] : 0.f;
       }
-      if (img.p) store8<T>(img, row * img.ld + col, 8, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += v[e];
+      if constexpr (T == D_F16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= scale;
+      }
+      if (img.p) store8<T>(img, row * img.ld + col, 8, v);
     }
   }
   if (!part) return;
@@ -261,6 +312,9 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   if (a.dw && planes) dzT = image_of(c, image, a.N, a.M);
   if (a.dw) xT = planes ? image_of(c, image, a.K, a.M) : (x_as_is ? user_mat(a.x, a.ldx) : image_of(c, image, a.M, a.K));
   float* part = a.db ? c.take<float>(std::max<int64_t>(1, nmb * a.N)) : nullptr;
+  const bool scaled = a.dtype == D_F16 && a.act > ACT_RELU && (a.dx || a.dw);
+  unsigned* maxima = scaled ? c.take<unsigned>(MAXIMA) : nullptr;
+  float* unscale = scaled ? c.take<float>(1) : nullptr;
   const int type = image;
   const int64_t slab_dx = a.dx ? product_slab_bytes(a.M, a.K, a.N, 1, type, 0) : 0;
   const int64_t slab_dw = a.dw ? product_slab_bytes(a.N, a.K, a.M, 1, type, 0) : 0;
@@ -275,10 +329,16 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
     Mat img = as_is ? Mat() : dz;
     const dim3 grid((unsigned)blocks), blk(256);
+    int tpr = 1, nmax = 0;
+    if (scaled) {
+      while (tpr < 256 && 8 * tpr < a.N) tpr *= 2;
+      nmax = (int)std::min<int64_t>(MAXIMA, std::max<int64_t>(1, a.M * tpr / 1024));
+      SCL_RUN(ctx, k_largest, dim3((unsigned)nmax), blk, 0, st, mdy, a.M, a.N, tpr, maxima);
+    }
     if (planes) SCL_RUN(ctx, k_dz_planes, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, dzT, part);
-    else if (a.dtype == D_F32) SCL_RUN(ctx, k_dz<D_F32>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    else if (a.dtype == D_BF16) SCL_RUN(ctx, k_dz<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
-    else SCL_RUN(ctx, k_dz<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part);
+    else if (a.dtype == D_F32) SCL_RUN(ctx, k_dz<D_F32>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part, nullptr, 0, nullptr);
+    else if (a.dtype == D_BF16) SCL_RUN(ctx, k_dz<D_BF16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part, nullptr, 0, nullptr);
+    else SCL_RUN(ctx, k_dz<D_F16>, grid, blk, 0, st, mdy, mz, a.act, a.M, a.N, img, part, maxima, nmax, unscale);
   }
   if (a.db && a.N > 0) {
     const dim3 grid((unsigned)((a.N + 63) / 64));
@@ -295,6 +355,7 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   p.out_type = p.res_type = a.dtype;
   p.slabs = slabs;
   p.slab_bytes = slab;
+  p.scale = a.M > 0 && a.N > 0 ? unscale : nullptr;  // (an empty sum: nothing was scaled)
   if (a.dx && a.M > 0 && a.K > 0) {
     if (planes) SCL_TRY(pack_image(ctx, st, a.dtype, image, a.w, a.ldw, true, a.K, a.N, &wT));
     wT.across = !planes;

@@ -223,3 +223,39 @@ def test_parts_of_a_gradient_have_the_bits_of_the_whole(dense, M, K, N, dtype):
             dense.linear_backward(dy, x, w, preact=z, activation="silu", need_x=False, need_weight=False)
         for part, whole, wanted in zip(got, (dx, dw, db), need):
             assert part is None if not wanted else torch.equal(part, whole), need
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("M,K,N", [(520, 1040, 648), (1000, 77, 450), (60, 600, 4000)])
+@pytest.mark.parametrize("top", [1e-6, 3e-3, 6e4])
+def test_fp16_gradients_of_any_size_keep_their_bits(dense, top, M, K, N, act):
+    """dz is held in fp16 under a scale that brings the largest |dy| to 2^14 or more: half a step of dz is 2^-11 of it or, below 2^-14 of the scaled
+    numbers, 2^-25 / scale <= 2^-39 of the largest |dy|. Nothing overflows: |dz| <= 1.13 |dy|. Derivatives and sums as in test_gpu_dense."""
+    g = gen_for("fp16 scale", M, K, N, act)
+    z = (torch.randn(M, N, generator=g, device="cuda") * 2).to(F16)
+    dy = (torch.randn(M, N, generator=g, device="cuda") * top / 8).clamp(-top, top).to(F16)
+    dy[M // 2, N // 3] = top
+    z[M // 2, N // 3] = 1.5  # where GELU's derivative is above 1.12: dz = 67 000
+    # results of ordinary size whatever the gradients' is
+    x = (torch.randn(M, K, generator=g, device="cuda") * min(1e3, 1 / top / 100)).to(F16)
+    w = (torch.randn(N, K, generator=g, device="cuda") * min(1e3, 1 / top / 100)).to(F16)
+    d = dy.double().abs().max().item()
+    dz = dy.double() * act_grad_limits(z.double(), act)
+    ddz = dy.double().abs() * 32 * 2.0 ** -24 * (1 + z.double().abs())
+    ddz = ddz + U[F16] * 1.01 * (dz.abs() + ddz) + 2.0 ** -39 * d
+    dx, dw, db = dense.linear_backward(dy, x, w, preact=z, activation=act)
+    for got, want, terms, prop in ((dx, dz @ w.double(), dz.abs() @ w.double().abs() * (2 * (N + 3)), ddz @ w.double().abs()),
+                                   (dw, dz.t().contiguous() @ x.double(), dz.abs().t().contiguous() @ x.double().abs() * (2 * (M + 3)),
+                                    ddz.t().contiguous() @ x.double().abs()),
+                                   (db, dz.sum(0), dz.abs().sum(0) * (M + 3), (dy.double().abs() * 32 * 2.0 ** -24 * (1 + z.double().abs())).sum(0))):
+        tol = (2.0 ** -24 * terms + prop) * 1.02
+        assert_close_or_same(got.double(), want, tol + U[F16] * 1.01 * (want.abs() + tol) + 2.0 ** -25, F16)
+    # rows of zeros, all zeros, and what is not finite beside what is
+    dy2 = dy.clone()
+    dy2[0], dy2[1, 5], dy2[2, 7] = 0, math.inf, math.nan
+    dx2, dw2, db2 = dense.linear_backward(dy2, x, w, preact=z, activation=act)
+    assert torch.equal(dx2[3:], dx[3:]) and (dx2[0] == 0).all() and not torch.isfinite(dx2[1:3]).any()
+    want = (dy2.double() * act_grad_limits(z.double(), act)).sum(0).to(F16)  # (sums of gradients next to 65504 may pass it)
+    assert torch.equal(torch.isfinite(db2), torch.isfinite(want)) and not torch.isfinite(db2[[5, 7]]).any()
+    z0 = dense.linear_backward(torch.zeros_like(dy), x, w, preact=z, activation=act)
+    assert all((t == 0).all() for t in z0)
