@@ -13,9 +13,9 @@
 // a singular value of zero leaves an eigenvalue of about -1e-17, and one that has grown to -0.1 runs off to infinity (nothing pulls a negative one
 // back; A = x x', formed anew in each step, has none). orth_is_small bounds that growth, eleven of the steps above pass, and what it
 // turns away is worked on by its definition.
-// A, P, Q commute and are symmetric: what lies on and below the diagonal is computed and mirrored, inside the tiles on the diagonal too. Left as
-// it comes out of A P and P Q, their upper half differs from the lower one by roundings, and that difference grows by a^3 a step (in
-// eight steps of the above to 6e-6 of a low-rank matrix, in twelve to 20; mirrored 3e-11 and 6e-9).
+// A, P, Q commute and are symmetric: tiles on and below the diagonal are computed and mirrored, those of A in themselves too. Left as it comes
+// out of the product of A P and P, A's upper half would differ from the lower one by roundings there, and that difference grows by a^3 a step
+// (in eight steps of the above to 6e-6 of a low-rank matrix, in twelve to 20; mirrored 4e-11 and 8e-9).
 //   n up to 1024, or many matrices: everything in one workgroup per matrix, one launch (k_orth_small).
 //   longer: partial sums of g g' over slices (k_orth_gram, k_orth_gram_sum), the steps in one workgroup (k_orth_steps), the product
 //   (k_orth_apply). 100 000 x 40 in fp32, eight steps: 14 + 4 + 35 + 22 us. The steps are a chain of fp64 products on one CU (4 us each),
@@ -160,15 +160,15 @@ __device__ __forceinline__ f64x4 tile_product(const double* X, const double* Y, 
     if (s < 4 * (MT - 1) || 4 * s < m) acc[s & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[s], yv[s], acc[s & 1], 0, 0, 0);
   return acc[0] + acc[1];
 }
-template <int MT>
+template <int MT, bool EXACT = false>  // EXACT: a tile on the diagonal is made symmetric
 __device__ __forceinline__ void tile_store(double* C, int i, int j, f64x4 v) {
   constexpr int LQ = Tiles<MT>::LQ;
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int r = i * 16 + q + 4 * g, c = j * 16 + r16;
-    if (r >= c) C[r * LQ + c] = v[g];
-    if (r > c) C[c * LQ + r] = v[g];
+    if (!EXACT || r >= c) C[r * LQ + c] = v[g];
+    if (EXACT ? r > c : i != j) C[c * LQ + r] = v[g];
   }
 }
 
@@ -264,7 +264,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
       if (w < NL) {
         int i, j;
         lower_tile(w, &i, &j);
-        tile_store<MT>(A, i, j, va[u]);
+        tile_store<MT, true>(A, i, j, va[u]);
       }
     }
     __syncthreads();
