@@ -505,6 +505,22 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   const bool f32 = wide && n <= MAX_CONTRACTION &&  // planes
                    ((!tall && n > MAX_CONTRACTION_F32) || (planes_pay(m, n, m, 0, (int)a.batch) && planes_pay(m, m, n, 0, (int)a.batch, 1)));
   if (m > MAX_CONTRACTION_F32 || (!tall && n > MAX_CONTRACTION)) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: more than 2^25 columns");
+  // The scales come from the bound, which may lie far above the singular values that are there. Those of a matrix of norm one reach 1 / sqrt(m);
+  // `there` follows such a one through the steps, while it is small and at most to the bound. Held under the bound's scale, x is off by
+  // (sqrt(m) + sqrt(n)) 2^-38 of the bound and P = b A + c A A by sqrt(m) 2^-36 of its bound (A's share included): up to the limits
+  // here, and 8192 rows, less than 2^-11 of what is there.
+  if (!wide) {
+    double bound = 1.0, there = 1.0;  // (in units of 1 / sqrt(m))
+    for (int t = 0; t < a.steps; ++t) {
+      const double ca = std::fabs(a.coef[3 * t]), cb = std::fabs(a.coef[3 * t + 1]), cc = std::fabs(a.coef[3 * t + 2]);
+      const double b2 = bound * bound, l = there * there / (double)m, grow = ca + (cb + cc * l) * l;
+      if (bound > 0x1p14 * there || (cb + cc * b2) * b2 > 0x1p20 * grow)
+        return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: 16 bits between the products are too few for singular values that may grow this far; "
+                                         "use fp32");
+      bound = orth_step_bound(a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2], bound);
+      there = std::min(there * grow, bound);
+    }
+  }
   const int IT = f32 ? D_PL3 : (wide ? D_F32 : D_F16), img_dtype = IT;
   Carve c(ws);
   const int64_t elems = m * n;

@@ -114,6 +114,57 @@ def test_an_error_that_somebody_else_has_left_stays_theirs(dense):
         assert torch.equal(a, b)
 
 
+GROWING = [[(16.0, 0.0, 0.0), (1.5, -0.5, 0.0)], [(1.0, 0.0, 1e3), (1.0, 0.0, 0.0)], [(4.0, 0.0, 0.0), (1.5, -0.5, 0.0), (1.0, 0.0, 0.0)],
+           [(12.0, -30.0, 19.0)] * 2, [(0.01, 0.0, 0.0), (100.0, 0.0, 0.0)], [(5e3, 0.0, 0.0), (1.0, 0.0, 0.0)], [(1.0, 1e5, 0.0)]]
+
+
+def step_bounds(schedule):
+    """the largest singular value that could be there before each step"""
+    b = [1.0]
+    for a1, a3, a5 in schedule:
+        s = torch.linspace(0, b[-1], 20001, dtype=torch.float64)
+        b.append((a1 * s + a3 * s ** 3 + a5 * s ** 5).abs().max().item() * 1.001)
+    return b
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("schedule", GROWING)
+@pytest.mark.parametrize("rows,cols", [(200, 150), (130, 700), (600, 300)])
+def test_schedules_whose_bound_grows(dense, rows, cols, schedule, dtype):
+    """the scales of 16-bit x, A and P come from the bound: besides orth_bound's relative roundings, entries are rounded to steps of
+    2^-24 / scale, scale >= 2^13 / bound of what is held, half a step each: (sqrt(m) + sqrt(n)) 2^-38 bound in norm for x, and for A and P
+    2 sqrt(m) 2^-38 of theirs times what the step makes of them; what a step leaves grows by the following steps' |p'|"""
+    g = gen_for("growing", rows, cols)
+    x = torch.randn(rows, cols, generator=g, device="cuda").to(dtype)
+    got, want = dense.orthogonalize(x, coefficients=schedule).double(), orth64(x, schedule)
+    tol = orth_bound(x, schedule, dtype)
+    if dtype is not F32:
+        m, n = min(rows, cols), max(rows, cols)
+        s = torch.linalg.svdvals((x.double() / (x.double().norm() + 1e-7)).cpu())
+        e = 0.0
+        for (a, b, c), B in zip(schedule, step_bounds(schedule)):
+            top = s.max().item()
+            q = torch.linspace(0, 1.02 * top, 513, dtype=torch.float64)
+            L = max((a + 3 * b * q ** 2 + 5 * c * q ** 4).abs().max().item(), (a + b * q ** 2 + c * q ** 4).abs().max().item())
+            P = abs(b) * B ** 2 + abs(c) * B ** 4
+            e = L * (e + math.sqrt(m * n) * 2.0 ** -38 * B) + top * m * 2.0 ** -38 * ((abs(b) + 2 * abs(c) * top ** 2) * B ** 2 + P)
+            s = (a * s + b * s ** 3 + c * s ** 5).abs()
+        tol = tol + e
+    assert (got - want).norm().cpu() <= tol, ((got - want).norm().item(), tol)
+
+
+def test_16_bits_that_do_not_suffice_are_refused(dense):
+    x = torch.ones(200, 150, device="cuda")
+    for schedule in ([(1.0, 0.0, 60.0), (0.0, 0.0, 1.0)], [(1.0, 0.0, 900.0), (0.0, 1.0, 0.0)], [(1.0, 0.0, 3e8), (1.0, 0.0, 0.0)]):
+        assert torch.isfinite(dense.orthogonalize(x, coefficients=schedule)).all()
+        small = dense.orthogonalize(x[:100, :100].to(F16).contiguous(), coefficients=schedule)  # one launch, in fp32
+        assert small.shape == (100, 100)
+        for dtype in (BF16, F16):
+            with pytest.raises(Exception, match="16 bits"):
+                dense.orthogonalize(x.to(dtype), coefficients=schedule)
+    assert torch.equal(dense.orthogonalize(x.to(F16)), dense.orthogonalize(x.to(F16)))
+
+
 # ---------------------------------------------------------------------------------------------------------------- activations
 ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
 
