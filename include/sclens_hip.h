@@ -225,7 +225,7 @@ int sclens_hip_get_denoised_f32(sclens_hip_ctx* ctx, const float* pca_n1, int64_
  * calls that may overlap -- other streams, graphs replayed side by side -- need one each. NULL with *ws_bytes = 0 is a size query, or
  * the call itself when it needs none.
  * Any size may be 0: an empty sum is 0. Rows of more than 2^25 elements (an fp32 dx: N of more than 2^24) are refused with SCLENS_ERR_ARG
- * where the product runs in tiles (more than 16 rows of x, no short side to stream past); there may be any number of rows.
+ * where the product runs in tiles (more than 16 rows of x, no short side to stream past), and so are more than 2^30 - 64 rows.
  * Activations and their derivatives take their limits at infinities (SiLU and both GELU: 0 at -infinity); NaN stays NaN.
  *
  * linear: y = act(x w' + bias) + residual. x [M][K], w [N][K], bias [N] or NULL, residual [M][N] or NULL, y [M][N]; preact [M][N] or

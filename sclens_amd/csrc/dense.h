@@ -35,6 +35,7 @@ struct Mat {
 // C[b] = epilogue(alpha * A[b] B[b]'), A [M][K], B [N][K], the contraction contiguous or (Mat::across) the rows.
 constexpr int64_t MAX_CONTRACTION = (int64_t)1 << 25;      // elements of an operand's row in the tiled products,
 constexpr int64_t MAX_CONTRACTION_F32 = (int64_t)1 << 24;  // of an fp32 row along the contraction
+constexpr int64_t MAX_ROWS = ((int64_t)1 << 30) - 64;      // rows: a grid's side holds fewer than 2^32 threads, 256 for 64 rows
 struct Product {
   int type = D_BF16;  // of the operands; D_PL3: fp32 as three bf16 planes each, six products per term
   Mat A, B;

@@ -794,7 +794,7 @@ int product(Ctx* ctx, hipStream_t st, const Product& p) {
   for (const Mat* m : {&p.A, &p.B})
     if (m->ld > (p.type == D_F32 && !m->across ? MAX_CONTRACTION_F32 : MAX_CONTRACTION))
       return ctx->fail(SCLENS_ERR_ARG, "product: an operand's rows are too long");
-  if (pl.tiles > 0x7fffffff || p.batch > 65535) return ctx->fail(SCLENS_ERR_ARG, "product: too many tiles");
+  if (pl.tiles >= 1 << 24 || p.batch > 65535) return ctx->fail(SCLENS_ERR_ARG, "product: too many tiles");
   ProdArgs g{};
   g.p = p;
   g.tiles_m = pl.tm;

@@ -54,7 +54,7 @@ bool planes_pay(int64_t M, int64_t N, int64_t K, int64_t packed_elems, int batch
 static bool streams(const LinearArgs& a, bool big_x) {
   const int64_t R = big_x ? a.M : a.N, S = big_x ? a.N : a.M;
   const bool dx = direct(a.dtype, a.x, a.ldx, a.K), dw = direct(a.dtype, a.w, a.ldw, a.K);
-  if ((a.dtype != D_F32 && (big_x ? dx : dw)) || S > STREAM_SHORT || R < 4 * S || R < 256 || a.K < 256) return false;
+  if ((a.dtype != D_F32 && (big_x ? dx : dw)) || S > STREAM_SHORT || R < 4 * S || R < 256 || R > 1 << 29 || a.K < 256) return false;
   const double copied = (double)((dx ? 0 : a.M) + (dw ? 0 : a.N)) * a.K * (a.dtype == D_F32 ? 8 : 4);
   return stream_us(R, S, a.K, a.dtype) < product_us(a.M, a.N, a.K, 1, a.dtype, 0) + (copied > 0 ? 5.0 + copied / 4e6 : 0.0);
 }
@@ -91,6 +91,7 @@ int linear_forward(Ctx* ctx, hipStream_t st, const LinearArgs& a, void* ws, int6
     if (a.M <= 16) return linear_rows(ctx, st, a);
     const bool tiles_as_is = direct(a.dtype, a.x, a.ldx, a.K) && direct(a.dtype, a.w, a.ldw, a.K);
     if (!tiles_as_is && linear_is_small(a)) return linear_small(ctx, st, a);
+    if (std::max(a.M, a.N) > MAX_ROWS) return ctx->fail(SCLENS_ERR_ARG, "linear: more than 2^30 - 64 rows");
     if (streams(a, false)) return linear_stream(ctx, st, a, false, ws, ws_bytes, need);
     if (streams(a, true)) return linear_stream(ctx, st, a, true, ws, ws_bytes, need);
   }
@@ -294,6 +295,7 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
   if (a.M > 0 && a.N > 0 && backward_is_small(a)) return backward_small(ctx, st, a);
   if (a.N > (a.dtype == D_F32 && a.dx ? MAX_CONTRACTION_F32 : MAX_CONTRACTION) || a.K > MAX_CONTRACTION)
     return ctx->fail(SCLENS_ERR_ARG, "linear_backward: more than 2^25 columns (2^24 in an fp32 dx)");
+  if (a.M > MAX_ROWS) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: more than 2^30 - 64 rows");
   Carve c(ws);
   // fp32 in planes if each of the two products gains by it (dz, w and x are taken apart), whichever of them is asked for: a part of the gradients has
   // the bits that it has among all of them
@@ -325,7 +327,7 @@ int linear_backward(Ctx* ctx, hipStream_t st, const LinearBwdArgs& a, void* ws, 
 
   if (a.M > 0 && a.N > 0 && (a.db || (a.dw && planes) || ((a.dx || a.dw) && !as_is))) {
     const int64_t blocks = nmb * ((a.N + cols_per - 1) / cols_per);
-    if (blocks > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
+    if (blocks >= 1 << 24) return ctx->fail(SCLENS_ERR_ARG, "linear_backward: too many elements");
     const Mat mdy = user_mat(a.dy, a.lddy), mz = user_mat(a.pre, a.ldz);
     Mat img = as_is ? Mat() : dz;
     const dim3 grid((unsigned)blocks), blk(256);
@@ -543,7 +545,7 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
   int tpr = 1;
   while (tpr < 256 && 8 * tpr < a.cols) tpr *= 2;
   const int64_t tiles = ((a.rows + 63) / 64) * ((a.cols + 63) / 64);
-  if (tiles > 0x7fffffff) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: too many elements");
+  if (tiles >= 1 << 24) return ctx->fail(SCLENS_ERR_ARG, "orthogonalize: too many elements");
   double bound = 1.0;
   double s_x = wide ? 1.0 : pow2_scale(bound);
   {

@@ -77,7 +77,8 @@ __global__ __launch_bounds__(512) void k_rows(LinearArgs a) {
   typedef typename Elem<T>::type E;
   __shared__ float S[8][256];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, q = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16;
+  if (n0 >= a.N) return;
   const E* wr = static_cast<const E*>(a.w) + min(n0 + r16, a.N - 1) * a.ldw;  // (rows behind the end: not stored)
   const E* xr = static_cast<const E*>(a.x) + min((int64_t)r16, a.M - 1) * a.ldx;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -114,7 +115,8 @@ __global__ __launch_bounds__(512) void k_rows(LinearArgs a) {
 }
 
 int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a) {
-  const dim3 grid((unsigned)((a.N + 15) / 16)), blk(512);
+  const int64_t groups = (a.N + 15) / 16, x = std::min<int64_t>(groups, 1 << 22);  // (a grid's side holds fewer than 2^32 threads)
+  const dim3 grid((unsigned)x, (unsigned)((groups + x - 1) / x)), blk(512);
   if (a.dtype == D_F32) SCL_RUN(ctx, k_rows<D_F32>, grid, blk, 0, st, a);
   else if (a.dtype == D_BF16) SCL_RUN(ctx, k_rows<D_BF16>, grid, blk, 0, st, a);
   else SCL_RUN(ctx, k_rows<D_F16>, grid, blk, 0, st, a);

@@ -310,3 +310,33 @@ def test_fp16_gradients_of_any_size_keep_their_bits(dense, top, M, K, N, act):
     assert torch.equal(torch.isfinite(db2), torch.isfinite(want)) and not torch.isfinite(db2[[5, 7]]).any()
     z0 = dense.linear_backward(torch.zeros_like(dy), x, w, preact=z, activation=act)
     assert all((t == 0).all() for t in z0)
+
+
+# -------------------------------------------------------------------------------------------------------------------- sizes
+def test_few_rows_past_very_many_weights(dense):
+    """more groups of 16 weights than one side of a grid holds"""
+    N, K = 2 ** 27 + 21, 8
+    w = torch.ones(N, K, dtype=BF16, device="cuda")
+    w[-1, 3] = 5
+    w[2 ** 26 + 3, 0] = -1
+    x = torch.ones(2, K, dtype=BF16, device="cuda")
+    x[1] = 2
+    y = dense.linear(x, w)
+    want = torch.full((N,), 8.0, dtype=BF16, device="cuda")
+    want[-1], want[2 ** 26 + 3] = 12, 6
+    assert torch.equal(y[0], want) and torch.equal(y[1], 2 * want)
+
+
+def test_more_rows_than_a_grid_holds_are_refused(dense):
+    """size queries: no memory is named, nothing is launched"""
+    import ctypes as C
+
+    ctx = dense.Context(0)
+    lib, n, some = ctx.lib, C.c_int64(0), 1 << 20  # (an address that is never read)
+    for M, N, rc in ((2 ** 30, 24, 1), (24, 2 ** 30, 1), (2 ** 30 - 64, 24, 8)):
+        n.value = 0
+        assert lib.sclens_hip_linear(ctx.h, None, 1, M, N, 2049, some, 2049, some, 2049, None, None, N, 0, some, N, None, N, None, n) == rc
+        assert rc == 8 or "rows" in lib.sclens_hip_last_error(ctx.h).decode()
+    for M, rc in ((2 ** 30, 1), (2 ** 30 - 64, 8)):
+        n.value = 0
+        assert lib.sclens_hip_linear_backward(ctx.h, None, 1, M, 24, 24, some, 24, some, 24, some, 24, None, 24, 0, some, 24, some, 24, some, None, n) == rc
