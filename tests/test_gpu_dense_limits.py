@@ -340,3 +340,98 @@ def test_more_rows_than_a_grid_holds_are_refused(dense):
     for M, rc in ((2 ** 30, 1), (2 ** 30 - 64, 8)):
         n.value = 0
         assert lib.sclens_hip_linear_backward(ctx.h, None, 1, M, 24, 24, some, 24, some, 24, some, 24, None, 24, 0, some, 24, some, 24, some, None, n) == rc
+
+
+# --------------------------------------------------------------------------------------------- addresses in the larger kernels
+ADDRESSES = [(0, 0), (8, 0), (8, 8), (8, 4), (16, 5), (3, 0), (1, 1), (0, 3)]
+
+
+def spread(t, extra, offset):
+    """rows `extra` apart in a buffer of NaN, which no result may see, `offset` elements into the storage"""
+    buf = torch.full((t.size(0) * (t.size(1) + extra) + offset + 8,), math.nan, dtype=t.dtype, device=t.device)
+    v = buf[offset: offset + t.size(0) * (t.size(1) + extra)].view(t.size(0), t.size(1) + extra)[:, : t.size(1)]
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("extra,offset", ADDRESSES)
+@pytest.mark.parametrize("M,K,N", [(520, 1032, 648), (515, 1030, 641), (20000, 1001, 40), (30, 2056, 3000), (2304, 1024, 1100)])
+def test_strides_and_addresses_in_tiles_and_streams(dense, M, K, N, extra, offset, dtype):
+    """past the sizes of the one-launch kernels: every operand with its own stride and address, what lies between the rows is NaN"""
+    g = gen_for("tile strides", M, K, N)
+    x, w = ints(g, (M, K), dtype, 1), ints(g, (N, K), dtype, 1)
+    b, r, dy, z = ints(g, (N,), dtype, 9), ints(g, (M, N), dtype, 9), ints(g, (M, N), dtype, 1), ints(g, (M, N), dtype, 3)
+    xs, ws, rs = spread(x, extra, offset), spread(w, 2 * extra, 0), spread(r, extra // 2, offset)
+    bs = torch.cat([b.new_full((offset + 1,), math.nan), b])[offset + 1:]
+    zz = x.double() @ w.double().t() + b.double()
+    y, pre = dense.linear(xs, ws, bias=bs, residual=rs, activation="relu", save_preact=True)
+    assert torch.equal(pre, zz.float().to(dtype))
+    assert torch.equal(y, (zz.clamp(min=0) + r.double()).float().to(dtype))
+    assert torch.equal(dense.linear(x, spread(w, extra, offset)), (zz - b.double()).float().to(dtype))
+    dys, zs = spread(dy, extra, 0), spread(z, 3 * extra, offset)
+    for act, pre_in, dz in (("relu", zs, dy.double() * (z.double() > 0)), ("none", None, dy.double())):
+        dx, dw, db = dense.linear_backward(dys, xs, ws, preact=pre_in, activation=act)
+        assert torch.equal(dx, (dz @ w.double()).float().to(dtype))
+        assert torch.equal(dw, (dz.t().contiguous() @ x.double()).float().to(dtype))
+        assert torch.equal(db, dz.sum(0).float().to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("extra,offset", ADDRESSES)
+@pytest.mark.parametrize("rows,cols", [(200, 304), (201, 303), (304, 200), (3000, 40), (40, 3000), (41, 700)])
+def test_strides_and_addresses_of_larger_orthogonalizations(dense, rows, cols, extra, offset, dtype):
+    g = gen_for("orth strides", rows, cols)
+    x = torch.randn(3, rows, cols, generator=g, device="cuda").to(dtype)
+    want = dense.orthogonalize(x[1].contiguous())
+    assert torch.equal(dense.orthogonalize(spread(x[1], extra, offset)), want)
+    # a batch whose matrices lie apart, each with longer rows
+    buf = torch.full((3, rows + 2, cols + extra), math.nan, dtype=dtype, device="cuda")
+    v = buf[:, 1: 1 + rows, :cols]
+    v.copy_(x)
+    assert torch.equal(dense.orthogonalize(v), dense.orthogonalize(x))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(5, 7, 9), (130, 200, 136), (520, 1032, 648), (515, 1030, 641), (2304, 1024, 1100)])
+def test_results_with_longer_rows(dense, M, K, N, dtype):
+    """the C entries write results whose rows lie apart, on any element: nothing between the rows, before or behind them"""
+    import ctypes as C
+
+    ctx = dense.Context(0)
+    lib, code = ctx.lib, dense.DTYPES[dtype]
+    g = gen_for("long results", M, K, N)
+    x, w, b = ints(g, (M, K), dtype, 1), ints(g, (N, K), dtype, 1), ints(g, (N,), dtype, 9)
+    r, dy, z = ints(g, (M, N), dtype, 9), ints(g, (M, N), dtype, 1), ints(g, (M, N), dtype, 3)
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def result(rows, cols, extra, offset):
+        buf = torch.full((rows * (cols + extra) + offset + 64,), -7.0, dtype=dtype, device="cuda")
+        return buf, buf[offset: offset + rows * (cols + extra)].view(rows, cols + extra)
+
+    def untouched(buf, v, cols, offset):
+        assert (v[:, cols:] == -7).all() and (buf[:offset] == -7).all() and (buf[offset + v.numel():] == -7).all()
+
+    for extra, offset in ((8, 0), (8, 8), (3, 0), (5, 1), (16, 4)):
+        (yb, y), (pb, p) = result(M, N, extra, offset), result(M, N, 2 * extra, 0)
+        n = C.c_int64(ws.numel())
+        ctx.check(lib.sclens_hip_linear(ctx.h, stream, code, M, N, K, x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), r.data_ptr(), N, 1,
+                                        y.data_ptr(), N + extra, p.data_ptr(), N + 2 * extra, ws.data_ptr(), C.byref(n)))
+        zz = x.double() @ w.double().t() + b.double()
+        assert torch.equal(p[:, :N], zz.float().to(dtype)) and torch.equal(y[:, :N], (zz.clamp(min=0) + r.double()).float().to(dtype))
+        untouched(yb, y, N, offset)
+        untouched(pb, p, N, 0)
+        (xb, dx), (wb, dw), (bb, db) = result(M, K, extra, offset), result(N, K, 2 * extra, 0), result(1, N, 0, offset)
+        n = C.c_int64(ws.numel())
+        ctx.check(lib.sclens_hip_linear_backward(ctx.h, stream, code, M, N, K, dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, z.data_ptr(), N, 1,
+                                                 dx.data_ptr(), K + extra, dw.data_ptr(), K + 2 * extra, db.data_ptr(), ws.data_ptr(), C.byref(n)))
+        dz = dy.double() * (z.double() > 0)
+        assert torch.equal(dx[:, :K], (dz @ w.double()).float().to(dtype))
+        assert torch.equal(dw[:, :K], (dz.t().contiguous() @ x.double()).float().to(dtype))
+        assert torch.equal(db[0], dz.sum(0).float().to(dtype))
+        untouched(xb, dx, K, offset)
+        untouched(wb, dw, K, 0)
+        untouched(bb, db, N, offset)
+    torch.cuda.synchronize()
+    ctx.close()
