@@ -218,8 +218,8 @@ int sclens_hip_get_denoised_f32(sclens_hip_ctx* ctx, const float* pca_n1, int64_
  * synchronises or allocates, and a call can be captured into a graph. Matrices are ROW-MAJOR with the given leading dimension (elements
  * between rows, at least the row's length), any alignment of whole elements; outputs must not overlap inputs. Inputs are read, outputs
  * written, in the element type `dtype` (SCLENS_DTYPE_*); sums are held in fp32 and rounded once. fp32 products run on
- * the fp32 matrix cores or, where that is faster, from three bf16 pieces per operand (24 bits, exact; what is left out of a term is below
- * its fp32 rounding), whatever the option "precision" says.
+ * the fp32 matrix cores or, where that is faster, from three bf16 pieces per operand (24 bits, exact from 1e-33 on; what is left out of a
+ * term is below its fp32 rounding), whatever the option "precision" says.
  * Workspace: device memory of the caller, 256-byte aligned, *ws_bytes its size. A call that needs more launches nothing, stores what it
  * needs in *ws_bytes and returns SCLENS_ERR_WORKSPACE; it may be reused or freed (in stream order) when the call's work is done, so two
  * calls that may overlap -- other streams, graphs replayed side by side -- need one each. NULL with *ws_bytes = 0 is a size query, or
@@ -235,8 +235,9 @@ int sclens_hip_linear(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, i
                       void* preact, int64_t ldz, void* ws, int64_t* ws_bytes);
 /* Its gradients: dz = dy * act'(preact) (preact may be NULL for SCLENS_ACT_NONE; relu'(0) = 0), dx = dz w, dw = dz' x, dbias = column
  * sums of dz; the residual's gradient is dy. dx / dw / dbias may be NULL: not computed (x is then only read for dw, w for dx). For
- * 16-bit types dz is rounded to that type before the two products. Every sum runs in a fixed order: equal inputs give equal bits, whichever
- * of the three are asked for. */
+ * 16-bit types dz is rounded to that type before the two products (fp16: under a power of two from the largest |dy|, so that gradients keep
+ * their bits whatever their size), unless the sizes are small enough for one launch, which keeps fp32. Every sum runs in a fixed order:
+ * equal inputs give equal bits, whichever of the three are asked for. */
 int sclens_hip_linear_backward(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t M, int64_t N, int64_t K, const void* dy,
                                int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* preact, int64_t ldz,
                                int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* dbias, void* ws, int64_t* ws_bytes);

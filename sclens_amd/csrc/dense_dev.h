@@ -22,7 +22,9 @@ __device__ __forceinline__ float f16_to_f32(unsigned short h) { return (float)__
 __device__ __forceinline__ unsigned short f32_to_f16(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
 
 // v = p0 + p1 + p2 exactly, each piece a bf16: p0 is v rounded to 8 bits, the remainder (exact in fp32, at most 2^-8 |v|) gives p1,
-// the next one (at most 8 bits left) is p2. Infinities and NaN sit in p0 alone. A v that would round up to infinity is cut instead.
+// the next one (at most 8 bits left) is p2. Infinities and NaN sit in p0 alone. A v that would round up to infinity is cut instead. Below 2^-110
+// (1e-33) the last bits fall under bf16's smallest step, 2^-133: fp32 products of such values lose them where they run in planes (relative
+// error 4e-5 at 2^-120).
 __device__ __forceinline__ void split3(float v, unsigned short& p0, unsigned short& p1, unsigned short& p2) {
   const unsigned u = __float_as_uint(v);
   if ((u & 0x7f800000u) == 0x7f800000u) {
@@ -170,7 +172,8 @@ __device__ __forceinline__ void store8(const Mat& m, int64_t off, int n, const f
 // much as eight of its stages.
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 // erfc(x) / 2 for x = |z| / sqrt(2): e^(-x^2) t P(t), t = 1 / (1 + 0.3 x). P is the polynomial of degree 8 of least largest relative
-// error on 0 <= x <= 10 (2e-8 before rounding; 4e-7 in fp32); *e gets e^(-z^2 / 2)
+// error on 0 <= x <= 10 (3e-8 with these coefficients); *e gets e^(-z^2 / 2). In fp32 the relative error is 5e-7 for |z| up to 2 and grows with the
+// exponent, whose rounding it is: 2e-6 at 6, 7e-6 at 13, where the tail itself is 1e-9 and 1e-38.
 __device__ __forceinline__ float normal_tail(float az, float* e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3f * 0.70710678f, az, 1.f));
   *e = __expf(-0.5f * az * az);

@@ -1,8 +1,9 @@
 // Small products and gradients in one launch, for matrices of any address and order: where the tiles would first need packed copies (fp32,
 // rows that do not start on 16 bytes) or a gradient several passes, the launches cost more than the work. 32 x 32 results per workgroup,
 // a quarter per wave, on v_mfma_f32_16x16x4 (16-bit operands convert exactly); 32 columns of the contraction at a time go through
-// registers to LDS, the next 32 on their way meanwhile. What bounds it is the latency of those steps (about 0.5 us each), not the
-// rate: 200 x 93 -> 50 in fp32 takes 4 to 7 of them.
+// registers to LDS, the next 32 on their way meanwhile. What bounds it is the latency of those steps, not the rate: gradients of 200 x 93
+// -> 50 in fp32 with ReLU take 9.9 us one after another in a graph, 2.4 and 1.07 for each of dw's seven steps (0.8 without an activation, whose kind
+// is decided per element); dx (two steps, 4.6 us alone) and the column sums (5.2 us alone) run beside it.
 #include <algorithm>
 
 #include "dense_dev.h"

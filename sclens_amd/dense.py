@@ -4,10 +4,13 @@ scores of cells outside a decomposition (`linear` with the centring as the bias)
 and encoders trained on the signals (`linear`, `linear_backward`, an `orthogonalize`d update), bases of two runs or members turned onto
 each other (`orthogonalize` of `corr_mat(V1, V2)`).
 
-Element types are torch.bfloat16, torch.float16 and torch.float32; sums are held in 32 bits and rounded once. Calls are queued on the
-tensors' device on torch's current stream of that device; they neither block nor synchronise, and can be captured into a graph after one
-eager call of the same thread (which creates the thread's context). They record no autograd graph and propagate no tangents (tensors that ask
-for either are refused): gradients are the explicit call.
+Element types are torch.bfloat16, torch.float16 and torch.float32; sums are held in 32 bits and rounded once. What 16-bit types hold in 16 bits
+between two products: `linear_backward` the gradient of the activation's argument (fp16 under a scale), `orthogonalize` its iterates (fp16
+under scales); the single-launch forms of small sizes keep 32 bits.
+
+Calls are queued on the tensors' device on torch's current stream of that device; they neither block nor synchronise, and can be captured
+into a graph after one eager call of the same thread (which creates the thread's context). They record no autograd graph and propagate
+no tangents (tensors that ask for either are refused): gradients are the explicit call.
 
 torch has to be imported before the library is first used (importing this module does it): both then run on one HIP runtime and torch's
 streams are valid for the library.
