@@ -7,6 +7,8 @@ Poisson-lognormal counts with `C` planted clusters, tuned to a target sparsity, 
 """
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import scipy.sparse as sp
 
@@ -23,6 +25,22 @@ def _rates(M, C, rng, marker_frac=0.05, marker_sd=1.0):
 def _sparsity_for_offset(beta0, off, lib_sigma=0.3):
     # E[P(x = 0)] ignoring the marker shifts and library-size spread (good enough for tuning)
     return float(np.mean(np.exp(-np.exp(beta0 + off))))
+
+
+def _entries(x):
+    """stored entries of a dense block of rows in CSR order: per row their number, their columns, their values"""
+    M = x.shape[1]
+    flat = np.flatnonzero(x)
+    ends = np.searchsorted(flat, np.arange(1, x.shape[0] + 1, dtype=np.int64) * M)
+    return np.diff(ends, prepend=0), (flat % M).astype(np.int32), x.ravel()[flat].astype(np.float32)
+
+
+def _join_blocks(blocks, M):
+    """consecutive blocks of rows as one CSC matrix with sorted indices"""
+    counts, cols, vals = (np.concatenate(v) for v in zip(*blocks))
+    indptr = np.concatenate([[0], np.cumsum(counts)])
+    blocks.clear()
+    return sp.csr_matrix((vals, cols, indptr), shape=(len(counts), M)).tocsc()
 
 
 def synth_counts(N: int, M: int, seed: int, C: int = 8, sparsity: float = 0.90,
@@ -42,17 +60,28 @@ def synth_counts(N: int, M: int, seed: int, C: int = 8, sparsity: float = 0.90,
     labels = np.arange(N) % C
     rng.shuffle(labels)
     lib = rng.lognormal(0.0, 0.3, size=N)
-    rows, cols, vals = [], [], []
-    for r0 in range(0, N, chunk_rows):
+    starts = list(range(0, N, chunk_rows))
+
+    def rates(r0):
         r1 = min(N, r0 + chunk_rows)
-        lam = lib[r0:r1, None] * np.exp(beta0[None, :] + delta[labels[r0:r1]])
-        x = rng.poisson(lam).astype(np.float32)
-        i, j = np.nonzero(x)
-        rows.append((i + r0).astype(np.int64))
-        cols.append(j.astype(np.int64))
-        vals.append(x[i, j])
-    X = sp.csc_matrix((np.concatenate(vals), (np.concatenate(rows), np.concatenate(cols))),
-                      shape=(N, M), dtype=np.float32)
+        return lib[r0:r1, None] * np.exp(beta0[None, :] + delta[labels[r0:r1]])
+
+    # the draws follow one generator, chunk after chunk; two chunks' rates are computed ahead of them and their entries collected behind, by
+    # other threads (numpy releases the interpreter's lock): 12 288 x 10 000 in 5.9 s instead of 10 on eight CPUs
+    blocks = []
+    with ThreadPoolExecutor(4) as pool:
+        ahead = [pool.submit(rates, r0) for r0 in starts[:2]]
+        for k in range(len(starts)):
+            lam = ahead[k].result()
+            ahead[k] = None
+            if k + 2 < len(starts):
+                ahead.append(pool.submit(rates, starts[k + 2]))
+            if k >= 3:
+                blocks[k - 3].result()  # (bounds what is held densely)
+            blocks.append(pool.submit(_entries, rng.poisson(lam)))
+            del lam
+        blocks = [b.result() for b in blocks]
+    X = _join_blocks(blocks, M)
     # enforce the QC invariants by planting single counts where needed (deterministic given seed)
     mg = min(200, max(2, M // 20)) if min_genes_per_cell is None else min_genes_per_cell
     mc = min(15, max(2, N // 20)) if min_cells_per_gene is None else min_cells_per_gene
@@ -110,24 +139,22 @@ def synth_counts_rows(N_total: int, M: int, seed: int, row0: int, row1: int, C: 
     rng.shuffle(labels)
     lib = rng.lognormal(0.0, 0.3, size=N_total)
     mg = min(min_genes_per_cell, max(2, M // 20))
-    rows, cols, vals = [], [], []
-    c0 = row0 // chunk_rows
-    for c in range(c0, (row1 + chunk_rows - 1) // chunk_rows):
+
+    def chunk(c):
         a, b = c * chunk_rows, min(N_total, (c + 1) * chunk_rows)
         crng = np.random.Generator(np.random.PCG64([seed, c]))
         lam = lib[a:b, None] * np.exp(beta0[None, :] + delta[labels[a:b]])
         x = crng.poisson(lam).astype(np.float32)
+        del lam
         short = np.flatnonzero((x > 0).sum(axis=1) < mg)
         for i in short:  # plant single counts (deterministic given seed and chunk)
             zero_cols = np.flatnonzero(x[i] == 0)
             x[i, crng.choice(zero_cols, size=mg - int((x[i] > 0).sum()), replace=False)] = 1.0
-        s0, s1 = max(a, row0) - a, min(b, row1) - a
-        i, j = np.nonzero(x[s0:s1])
-        rows.append((i + (a + s0 - row0)).astype(np.int32))  # (32-bit triplets: a 125 000 x 30 000 slab peaked at 23 GB with 64-bit ones)
-        cols.append(j.astype(np.int32))
-        vals.append(x[s0:s1][i, j])
-    rows, cols, vals = np.concatenate(rows), np.concatenate(cols), np.concatenate(vals)
-    X = sp.csc_matrix((vals, (rows, cols)), shape=(row1 - row0, M), dtype=np.float32)
-    del rows, cols, vals
+        return _entries(x[max(a, row0) - a:min(b, row1) - a])
+
+    # two chunks at a time: every chunk has its own generator (the slabs of an atlas are generated by one process per slab besides)
+    with ThreadPoolExecutor(2) as pool:
+        blocks = list(pool.map(chunk, range(row0 // chunk_rows, (row1 + chunk_rows - 1) // chunk_rows)))
+    X = _join_blocks(blocks, M)
     X.sort_indices()
     return X
