@@ -15,7 +15,7 @@ torch.distributed.run`, before anything here touches the GPU) and relays the chi
 Under torch.distributed.run (WORLD_SIZE set) it is one rank of the job.
 
 A full sclens() at cfg4 takes about a minute, so K timed steps may not fit the time a caller allows: the run is held
-to `--budget-s` seconds of wall-clock (default 1500 s, SCLENS_BENCH_BUDGET_S) and executes as many of the requested
+to `--budget-s` seconds of wall-clock (default 420 s, SCLENS_BENCH_BUDGET_S) and executes as many of the requested
 warm-up / timed steps as fit. The JSON line reports the TRUE counts in `steps` / `warmup` and the requested ones in
 `steps_requested` / `warmup_requested`.
 
@@ -407,7 +407,7 @@ def main():
     ap.add_argument("--steps", type=int, default=1)
     ap.add_argument("--warmup", type=int, default=0)
     ap.add_argument("--config", default="cfg4", choices=list(CONFIGS))
-    ap.add_argument("--budget-s", type=float, default=float(os.environ.get("SCLENS_BENCH_BUDGET_S", "1500")),
+    ap.add_argument("--budget-s", type=float, default=float(os.environ.get("SCLENS_BENCH_BUDGET_S", "420")),
                     help="wall-clock limit of the whole run; warm-up and timed steps are cut to fit (true counts are reported)")
     ap.add_argument("--n-perturb", type=int, default=20)
     ap.add_argument("--no-cpu-baseline", action="store_true")
