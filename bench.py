@@ -472,6 +472,10 @@ def main():
     if rank == 0 and world > 1:
         print(f"[bench] {world} ranks, backend {args.backend}, self-check {check}", file=sys.stderr, flush=True)
 
+    def say(text):  # progress, on stderr: a run takes minutes before its line
+        if rank == 0:
+            print(f"[bench] {text}", file=sys.stderr, flush=True)
+
     def agree(x):  # rank 0's decision on every rank (steps must match or the collectives dead-lock)
         return float(shard.bcast_host(np.array([float(x)]), 0)[0])
 
@@ -520,6 +524,7 @@ def main():
         t0 = time.perf_counter()
         X = api._csc_f32(cached_counts(cfg, N, M, 20240427 + cfg_index))  # PCG64(20240427 + config_index)
         t_synth = time.perf_counter() - t0
+        say(f"{cfg}: {N} x {M} matrix ready after {t_synth:.1f} s")
         row_shard = args.row_shard and N > M
         if row_shard:
             from sclens_amd import atlas
@@ -554,6 +559,7 @@ def main():
             res = one_step(-1 - w)
             t_step = time.perf_counter() - ts
             n_warm += 1
+            say(f"warm-up step {n_warm}: {t_step:.1f} s")
         fence()
         n_steps, decisions, phase_peaks = 0, [], {}  # phase_peaks: largest live device bytes of the library's pool per phase, timed steps
         t0 = time.perf_counter()
@@ -565,6 +571,7 @@ def main():
             res = one_step(this)
             t_step = time.perf_counter() - ts
             n_steps += 1
+            say(f"timed step {n_steps}: {t_step:.1f} s")
             for k_, v_ in (res.get("phase_peak_GB") or {}).items():
                 phase_peaks[k_] = max(phase_peaks.get(k_, 0.0), float(v_))
             if "search_trace" in res:
