@@ -92,14 +92,17 @@ struct Epilogue {
 };
 
 // an fp32 product term by term in fp32: only for results that came out NaN, which the pieces also give where an infinity meets a piece
-// that is zero (inf * 1.0 contains inf * p1(1.0) = inf * 0)
+// that is zero (inf * 1.0 contains inf * p1(1.0) = inf * 0). Eight terms per step, whose loads are on their way together (an image's rows are whole
+// chunks, zeros behind K): term by term each waited for its own, and one such result of a long contraction took seconds.
 __device__ __forceinline__ float recompute_f32(const unsigned short* A, const unsigned short* B, int64_t planeA, int64_t planeB, int64_t K) {
+  auto load = [](const unsigned short* p) { return *reinterpret_cast<const u16x8*>(p); };
   float s = 0.f;
-  for (int64_t k = 0; k < K; ++k) {
-    const float a = (bf16_to_f32(A[k]) + bf16_to_f32(A[k + planeA])) + bf16_to_f32(A[k + 2 * planeA]);
-    const float b = (bf16_to_f32(B[k]) + bf16_to_f32(B[k + planeB])) + bf16_to_f32(B[k + 2 * planeB]);
-    s = fmaf(a, b, s);
-    if (s != s) break;
+  for (int64_t k = 0; k < K && s == s; k += 8) {
+    const u16x8 a0 = load(A + k), a1 = load(A + k + planeA), a2 = load(A + k + 2 * planeA);
+    const u16x8 b0 = load(B + k), b1 = load(B + k + planeB), b2 = load(B + k + 2 * planeB);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      s = fmaf((bf16_to_f32(a0[e]) + bf16_to_f32(a1[e])) + bf16_to_f32(a2[e]), (bf16_to_f32(b0[e]) + bf16_to_f32(b1[e])) + bf16_to_f32(b2[e]), s);
   }
   return s;
 }

@@ -435,3 +435,64 @@ def test_results_with_longer_rows(dense, M, K, N, dtype):
         untouched(bb, db, N, offset)
     torch.cuda.synchronize()
     ctx.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("M,K,N", [(200, 93, 50), (520, 1032, 648), (515, 1030, 641), (2304, 2176, 2048)])
+def test_gradients_of_infinities(dense, M, K, N, act, dtype):
+    """infinities and NaN of every operand reach exactly the results that contain them, whole numbers elsewhere"""
+    g = gen_for("grad extremes", M, K, N)
+    x, w, dy, z = ints(g, (M, K), dtype, 1), ints(g, (N, K), dtype, 1), ints(g, (M, N), dtype, 1), ints(g, (M, N), dtype, 3)
+    dy[3, 5], dy[7, 9], dy[8, 1], dy[8, 2] = math.inf, math.nan, math.inf, -math.inf
+    x[11, 13], x[12, 2] = -math.inf, math.nan
+    w[17, 19], w[18, 7] = math.inf, math.nan
+    dz = dy.double() * ((z.double() > 0) if act == "relu" else 1)
+    dx, dw, db = dense.linear_backward(dy, x, w, preact=z if act == "relu" else None, activation=act)
+    for got, want in ((dx, dz @ w.double()), (dw, dz.t().contiguous() @ x.double()), (db, dz.sum(0))):
+        want = want.float().to(dtype).double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        fix = dict(nan=0.0, posinf=1e300, neginf=-1e300)
+        assert torch.equal(torch.nan_to_num(got.double(), **fix), torch.nan_to_num(want, **fix))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 100000), (100000, 5)])
+def test_orthogonalize_many_steps_of_a_long_side(dense, rows, cols, dtype):
+    g = gen_for("long side")
+    x = torch.randn(rows, cols, generator=g, device="cuda").to(dtype)
+    y = dense.orthogonalize(x, coefficients=UPDATE[:3] + [POLAR[-1]] * 20).double()
+    gram = y @ y.t() if rows < cols else y.t().contiguous() @ y
+    u = U[F32] if dtype is F32 else U[F16]
+    off = (gram - torch.eye(5, device="cuda", dtype=torch.float64)).norm().item()
+    assert off <= 2 * math.sqrt(5) * (U[dtype] + 1.875 * 4 * (u + 2 * (math.sqrt(1e5) + 3) * 2.0 ** -24)), off
+
+
+def test_scaled_gradients_captured_and_replayed(dense):
+    """the scale of fp16 gradients is found on the device: a replay uses that of its own inputs, and two graphs share nothing"""
+    g = gen_for("scaled graph")
+    M, K, N = 520, 200, 648
+    x, w = torch.randn(M, K, generator=g, device="cuda").to(F16), torch.randn(N, K, generator=g, device="cuda").to(F16)
+    z, dy = torch.randn(M, N, generator=g, device="cuda").to(F16), torch.randn(M, N, generator=g, device="cuda").to(F16)
+    o = torch.randn(40, 300, generator=g, device="cuda").to(F16)
+
+    def work():
+        return (*dense.linear_backward(dy, x, w, preact=z, activation="gelu"), dense.orthogonalize(o, coefficients=UPDATE + UPDATE + UPDATE))
+
+    work()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = work()
+        graphs.append((gr, res))
+    for scale in (1.0, 1e-6, 3e3, 0.0, 1e-3):
+        dy.copy_(torch.randn(M, N, generator=g, device="cuda") * scale)
+        eager = [t.clone() for t in work()]
+        for gr, _ in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for _, res in graphs:
+            for a, b in zip(res, eager):
+                assert torch.equal(a, b), scale
