@@ -246,8 +246,8 @@ int sclens_hip_linear_backward(sclens_hip_ctx* ctx, void* stream, int dtype, int
  * many rows as columns; a taller matrix is worked on transposed). Each singular value s goes through a s + b s^3 + c s^5.
  * (3.4445, -4.7750, 2.0315) brings everything above ~1e-2 of the norm near 1 in five steps (an optimiser's update); (15/8, -5/4, 3/8)
  * then converges cubically to the orthogonal factor. A matrix of zeros gives zeros (with eps = 0: NaN); a NaN or an infinity spoils its own
- * matrix only. Coefficients under which a singular value could pass 1e9 are refused. Where 16-bit matrices are worked on in tiles (a side above
- * 128, the other above 64 or many steps) x, A and P are fp16 between the products, scaled by that bound; coefficients whose bound lies so
+ * matrix only. Coefficients under which a singular value could pass 1e9 are refused. Where 16-bit matrices are worked on in tiles (both sides above
+ * 64, one of them above 128 or more than 24 steps) x, A and P are fp16 between the products, scaled by that bound; coefficients whose bound lies so
  * far above singular values of 1 / sqrt(rows) that too few bits are left for those are refused as well. */
 int sclens_hip_orthogonalize(sclens_hip_ctx* ctx, void* stream, int dtype, int64_t batch, int64_t rows, int64_t cols, const void* x,
                              int64_t stride_x, int64_t ldx, void* y, int64_t stride_y, int64_t ldy, int steps, const double* coef,

@@ -101,7 +101,7 @@ struct OrthArgs {
   double eps = 0;
 };
 double orth_step_bound(double a, double b, double c, double B);  // the singular values' bound after a step
-bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: both sides at most 128, or a short side of at most 64 (and not too many steps)
+bool orth_is_small(const OrthArgs& a);  // dense_orth.hip: both sides at most 128 (and few steps), or a short side of at most 64
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int64_t ws_bytes, int64_t* need);
 int linear_rows(Ctx* ctx, hipStream_t st, const LinearArgs& a);  // M <= 16
 

@@ -11,8 +11,8 @@
 // (five steps of a = 3.4445: a^8 = 2e4 relative to the largest), which fp32 cannot pay and fp64 can: the m x m side and both products run
 // on v_mfma_f64_16x16x4 (below 64 rows they cost less than reading x does; the entries of x convert exactly). Not for any number of steps:
 // a singular value of zero leaves an eigenvalue of about -1e-17, and one that has grown to -0.1 runs off to infinity (nothing pulls a negative one
-// back; A = x x', formed anew in each step, has none). orth_is_small bounds that growth, eleven of the steps above pass, and what it
-// turns away is worked on by its definition.
+// back; a newly formed A = x x' has none). orth_run bounds that growth from the coefficients; where it ends (after eleven of the steps above) the
+// product is written in fp32 and the next run starts from it.
 // A, P, Q commute and are symmetric: tiles on and below the diagonal are computed and mirrored, those of A in themselves too. Left as it comes
 // out of the product of A P and P, A's upper half would differ from the lower one by roundings there, and that difference grows by a^3 a step
 // (in eight steps of the above to 6e-6 of a low-rank matrix, in twelve to 20; mirrored 4e-11 and 8e-9).
@@ -32,6 +32,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 struct SmallArgs {
   OrthArgs o;  // coef: device pointer is not needed, the steps' coefficients ride in `coef`
   int tall, m, slices;
+  int start;  // x is the caller's and is divided by its norm first
   int64_t n;
   double* part;  // [batch][slices][tiles * 256]
   double* gram;  // [batch][tiles * 256]
@@ -193,7 +194,7 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
   if (tid == 0) {
     double s = 0.0;
     for (int i = 0; i < a.m; ++i) s += A[i * LQ + i];
-    scal[0] = 1.0 / (sqrt(s) + a.o.eps);
+    scal[0] = a.start ? 1.0 / (sqrt(s) + a.o.eps) : 1.0;
   }
   __syncthreads();
   const double f = scal[0];
@@ -271,13 +272,13 @@ __device__ __forceinline__ void steps(const SmallArgs& a, const Coefs& cf, const
   }
 }
 
-// y = Q x for k0 <= k < kend, 16 NW columns at a time; Q [R][ldq] in LDS
-template <int T, int MT, int NW>
+// y = Q x for k0 <= k < kend, 16 NW columns at a time; Q [R][ldq] in LDS. y may be x: columns are read before they are written.
+template <int T, int U, int MT, int NW>
 __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64_t k0, int64_t kend, float* Xs, const double* Q) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, CK = 16 * NW;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
   constexpr int KS = 4 * MT;
-  auto* y = static_cast<typename Elem<T>::type*>(a.o.y) + b * a.o.sy;
+  auto* y = static_cast<typename Elem<U>::type*>(a.o.y) + b * a.o.sy;
   const Places<MT, NW> pl(a);
   Slab<T, MT, NW> s;
   s.fetch(a, pl, b, k0, kend);
@@ -305,7 +306,7 @@ __device__ __forceinline__ void apply_range(const SmallArgs& a, int64_t b, int64
     const int n = (int)min((int64_t)CK, kend - k);
 #pragma unroll
     for (int e = 0; e < 4 * MT; ++e)
-      if (pl.k[e] < n) Elem<T>::st(yk + pl.out[e], Xs[pl.at[e]]);
+      if (pl.k[e] < n) Elem<U>::st(yk + pl.out[e], Xs[pl.at[e]]);
     __syncthreads();
   }
 }
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(SmallArgs a, Coefs cf) {
   }
 }
 
-template <int T, int MT>
+template <int T, int U, int MT>
 __global__ __launch_bounds__(512) void k_orth_small(SmallArgs a, Coefs cf) {
   constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -449,7 +450,7 @@ __global__ __launch_bounds__(512) void k_orth_small(SmallArgs a, Coefs cf) {
   const int64_t b = blockIdx.x;
   gram_range<T, MT, 8>(a, b, 0, a.n, Xs, A, red);
   steps<MT>(a, cf, red, A, P, Q, scal);
-  apply_range<T, MT, 8>(a, b, 0, a.n, Xs, Q);
+  apply_range<T, U, MT, 8>(a, b, 0, a.n, Xs, Q);
 }
 template <int T, int MT>
 __global__ __launch_bounds__(256) void k_orth_gram(SmallArgs a) {
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(512) void k_orth_steps(SmallArgs a, Coefs cf) {
   steps<MT>(a, cf, a.gram + b * NL * 256, A, P, Q, scal);
   for (int e = threadIdx.x; e < R * R; e += 512) a.Q[b * R * R + e] = Q[(e / R) * LQ + e % R];
 }
-template <int T, int MT>
+template <int T, int U, int MT>
 __global__ __launch_bounds__(256) void k_orth_apply(SmallArgs a) {
   constexpr int LQ = Tiles<MT>::LQ, R = Tiles<MT>::R, LI = Tiles<MT>::LI;
   __shared__ double Q[R * LQ];
@@ -495,25 +496,25 @@ __global__ __launch_bounds__(256) void k_orth_apply(SmallArgs a) {
   const int64_t b = blockIdx.y, chunks = (a.n + 63) / 64, per = (chunks + gridDim.x - 1) / gridDim.x;
   for (int e = threadIdx.x; e < R * R; e += 256) Q[(e / R) * LQ + e % R] = a.Q[b * R * R + e];
   const int64_t k0 = (int64_t)blockIdx.x * per * 64, kend = min(a.n, k0 + per * 64);
-  apply_range<T, MT, 4>(a, b, k0, kend, Xs, Q);  // (its first barrier orders Q too)
+  apply_range<T, U, MT, 4>(a, b, k0, kend, Xs, Q);  // (its first barrier orders Q too)
 }
 
 namespace {
-template <int T, int MT>
+template <int T, int U, int MT>
 int run_small(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
   constexpr int R = Tiles<MT>::R, LQ = Tiles<MT>::LQ, LI = Tiles<MT>::LI, NL = Tiles<MT>::NL;
   constexpr int LDS_STEPS = (3 * R * LQ + 2) * 8, LDS_ALL = (Tiles<MT>::WORK + 2 + NL * 256) * 8 + 128 * LI * 4;
   const unsigned batch = (unsigned)a.o.batch;
   if (a.slices == 1) {
-    if (LDS_ALL > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_small<T, MT>), LDS_ALL));
-    SCL_RUN(ctx, k_orth_small<T, MT>, dim3(batch), dim3(512), LDS_ALL, st, a, cf);
+    if (LDS_ALL > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_small<T, U, MT>), LDS_ALL));
+    SCL_RUN(ctx, k_orth_small<T, U, MT>, dim3(batch), dim3(512), LDS_ALL, st, a, cf);
   } else {
     if (LDS_STEPS > 65536) SCL_TRY(ensure_dyn_lds(ctx, reinterpret_cast<const void*>(k_orth_steps<MT>), LDS_STEPS));
     SCL_RUN(ctx, k_orth_gram<T, MT>, dim3((unsigned)a.slices, batch), dim3(256), 0, st, a);
     SCL_RUN(ctx, k_orth_gram_sum, dim3(NL * 8, batch), dim3(1024), 0, st, a.part, a.slices, NL * 256, a.gram);
     SCL_RUN(ctx, k_orth_steps<MT>, dim3(batch), dim3(512), LDS_STEPS, st, a, cf);
     const int64_t chunks = (a.n + 63) / 64, per = std::max<int64_t>(1, chunks * batch / 768);
-    SCL_RUN(ctx, k_orth_apply<T, MT>, dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
+    SCL_RUN(ctx, k_orth_apply<T, U, MT>, dim3((unsigned)((chunks + per - 1) / per), batch), dim3(256), 0, st, a);
   }
   return SCLENS_OK;
 }
@@ -533,12 +534,19 @@ int run_direct_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) 
   if (a.n <= 96) return run_direct<T, 6>(ctx, st, a, cf);
   return run_direct<T, 8>(ctx, st, a, cf);
 }
-template <int T>
+template <int T, int U>
 int run_small_t(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf) {
-  if (a.m <= 16) return run_small<T, 1>(ctx, st, a, cf);
-  if (a.m <= 32) return run_small<T, 2>(ctx, st, a, cf);
-  if (a.m <= 48) return run_small<T, 3>(ctx, st, a, cf);
-  return run_small<T, 4>(ctx, st, a, cf);
+  if (a.m <= 16) return run_small<T, U, 1>(ctx, st, a, cf);
+  if (a.m <= 32) return run_small<T, U, 2>(ctx, st, a, cf);
+  if (a.m <= 48) return run_small<T, U, 3>(ctx, st, a, cf);
+  return run_small<T, U, 4>(ctx, st, a, cf);
+}
+// from the caller's type or fp32 (between two runs) to either
+int run_small_types(Ctx* ctx, hipStream_t st, const SmallArgs& a, const Coefs& cf, int from, int to) {
+  if (from == D_F32 && to == D_F32) return run_small_t<D_F32, D_F32>(ctx, st, a, cf);
+  if (from == D_F32) return to == D_BF16 ? run_small_t<D_F32, D_BF16>(ctx, st, a, cf) : run_small_t<D_F32, D_F16>(ctx, st, a, cf);
+  if (from == D_BF16) return to == D_F32 ? run_small_t<D_BF16, D_F32>(ctx, st, a, cf) : run_small_t<D_BF16, D_BF16>(ctx, st, a, cf);
+  return to == D_F32 ? run_small_t<D_F16, D_F32>(ctx, st, a, cf) : run_small_t<D_F16, D_F16>(ctx, st, a, cf);
 }
 }  // namespace
 
@@ -551,56 +559,77 @@ static double largest_quadratic(double a, double b, double c, double L) {
   }
   return v;
 }
-// The largest that the rounding of A_0, m half steps of fp64, can have become in the A of the last step. A step takes an eigenvalue l to
-// l q(l)^2, q(l) = a + b l + c l^2, and an error there to q(l) (a + 3 b l + 5 c l^2) times itself (outside the eigenvalues' range, next to
-// zero, to q(l)^2). Low-rank matrices on which this was tried in fp64: where the bound is 1e-3 (eleven steps of 3.4445, -4.7750, 2.0315)
-// the result is off by 3e-9, at 8e4 (18 steps) by 5e3, then infinite.
-static double orth_error_growth(const OrthArgs& o) {
-  double err = (double)std::min(o.rows, o.cols) * 0x1p-53, bound = 1.0;
-  for (int t = 0; t + 1 < o.steps; ++t) {
-    const double a = o.coef[3 * t], b = o.coef[3 * t + 1], c = o.coef[3 * t + 2], L = bound * bound;
-    const double q = largest_quadratic(a, b, c, L), dp = largest_quadratic(a, 3 * b, 5 * c, L);
+// The steps from `first` on that one run may take, singular values of at most *bound before and after. The rounding of A, m half steps of fp64 of
+// bound^2, must not pass 2^-8 before the last of them. A step takes an eigenvalue l to l q(l)^2, q(l) = a + b l + c l^2, and an
+// error there to q(l) (a + 3 b l + 5 c l^2) times itself (outside the eigenvalues' range, next to zero, to q(l)^2). Low-rank matrices on
+// which this was tried in fp64: where the bound is 1e-3 (eleven steps of 3.4445, -4.7750, 2.0315) the result is off by 3e-9, at 8e4
+// (18 steps) by 5e3, then infinite. One step is the definition and always fits.
+static int orth_run(const OrthArgs& o, int first, double* bound) {
+  double err = (double)std::min(o.rows, o.cols) * 0x1p-53 * *bound * *bound;
+  int n = 0;
+  while (first + n < o.steps && n < MAX_RIDE && (n == 0 || err < 0x1p-8)) {
+    const double* c = o.coef + 3 * (first + n);
+    const double L = *bound * *bound, q = largest_quadratic(c[0], c[1], c[2], L), dp = largest_quadratic(c[0], 3 * c[1], 5 * c[2], L);
     err *= std::max(1.0, q * std::max(q, dp));
-    bound = orth_step_bound(a, b, c, bound);
+    *bound = orth_step_bound(c[0], c[1], c[2], *bound);
+    ++n;
   }
-  return err;
+  return n;
 }
 
+static bool orth_is_direct(const OrthArgs& o) { return std::max(o.rows, o.cols) <= 128 && o.steps <= MAX_RIDE; }
 bool orth_is_small(const OrthArgs& o) {
-  const int64_t m = std::min(o.rows, o.cols), n = std::max(o.rows, o.cols), ld = std::max(o.ldx, o.ldy);
-  if (o.steps > MAX_RIDE || ld >= ((int64_t)1 << 25)) return false;
-  return n <= 128 || (m <= 64 && orth_error_growth(o) < 0x1p-8);
+  return std::max(o.ldx, o.ldy) < ((int64_t)1 << 25) && (orth_is_direct(o) || std::min(o.rows, o.cols) <= 64);
 }
 
 int orth_small(Ctx* ctx, hipStream_t st, const OrthArgs& o, void* ws, int64_t ws_bytes, int64_t* need) {
   SmallArgs a{};
   a.o = o;
+  a.o.coef = nullptr;
   a.tall = o.rows > o.cols;
   a.m = (int)std::min(o.rows, o.cols);
   a.n = std::max(o.rows, o.cols);
+  a.start = 1;
   const int MT = (a.m + 15) / 16, elems = MT * (MT + 1) / 2 * 256;
-  const bool direct = a.n <= 128;
+  const bool direct = orth_is_direct(o);
   if (direct || a.n <= 1024 || o.batch >= 128) a.slices = 1;
   else a.slices = (int)std::max<int64_t>(2, std::min<int64_t>((a.n + 255) / 256, 512 / o.batch));
+  double bound = 1.0;
+  int run = direct ? o.steps : orth_run(o, 0, &bound);
   Carve c(ws);
   if (a.slices > 1) {
     a.part = c.take<double>(o.batch * a.slices * elems);
     a.gram = c.take<double>(o.batch * elems);
     a.Q = c.take<double>(o.batch * 256 * MT * MT);
   }
+  float* between = run < o.steps ? c.take<float>(o.batch * o.rows * o.cols) : nullptr;
   *need = c.used;
   if (c.used > ws_bytes) return ctx->fail(SCLENS_ERR_WORKSPACE, "this call needs " + std::to_string(c.used) + " bytes of device workspace");
   Coefs cf{};
-  for (int i = 0; i < 3 * o.steps; ++i) cf.v[i] = o.coef[i];
-  a.o.coef = nullptr;
   if (direct) {
+    for (int i = 0; i < 3 * o.steps; ++i) cf.v[i] = o.coef[i];
     if (o.dtype == D_F32) return run_direct_t<D_F32>(ctx, st, a, cf);
     if (o.dtype == D_BF16) return run_direct_t<D_BF16>(ctx, st, a, cf);
     return run_direct_t<D_F16>(ctx, st, a, cf);
   }
-  if (o.dtype == D_F32) return run_small_t<D_F32>(ctx, st, a, cf);
-  if (o.dtype == D_BF16) return run_small_t<D_BF16>(ctx, st, a, cf);
-  return run_small_t<D_F16>(ctx, st, a, cf);
+  for (int first = 0; first < o.steps;) {
+    const bool last = first + run == o.steps;
+    if (first > 0) {
+      a.start = 0;
+      a.o.x = between;
+      a.o.ldx = o.cols;
+      a.o.sx = o.rows * o.cols;
+    }
+    a.o.y = last ? o.y : between;
+    a.o.ldy = last ? o.ldy : o.cols;
+    a.o.sy = last ? o.sy : o.rows * o.cols;
+    a.o.steps = run;
+    for (int i = 0; i < 3 * run; ++i) cf.v[i] = o.coef[3 * first + i];
+    SCL_TRY(run_small_types(ctx, st, a, cf, first > 0 ? D_F32 : o.dtype, last ? o.dtype : D_F32));
+    first += run;
+    run = orth_run(o, first, &bound);
+  }
+  return SCLENS_OK;
 }
 
 }  // namespace scl

@@ -496,3 +496,26 @@ def test_scaled_gradients_captured_and_replayed(dense):
         for _, res in graphs:
             for a, b in zip(res, eager):
                 assert torch.equal(a, b), scale
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,rank", LOW_RANK + [(60, 90, 10), (3, 128, 2)])
+@pytest.mark.parametrize("steps", [12, 14, 16, 30])
+def test_orthogonalize_low_rank_in_runs(dense, steps, rows, cols, rank, dtype):
+    """Between two runs of the m x m side (eleven steps, at most 24) x is rounded to fp32, 2^-24 of a norm of at most 1.21 sqrt(m) counted once
+    too often, which no step makes more than 4 times as large (|p'| <= 3.97 up to 1.2024); likewise what the fp64 of the definition here rounds.
+    From 22 steps on both have grown to one in the empty directions: what remains is that nothing leaves 0 .. 1.2024."""
+    x = low_rank(gen_for("low rank", rows, cols, rank), rows, cols, rank, dtype)
+    y = dense.orthogonalize(x, coefficients=[UPDATE[0]] * steps).double()
+    assert torch.isfinite(y).all()
+    m, n = min(rows, cols), max(rows, cols)
+    top = torch.linalg.svdvals(y.cpu()).max().item()
+    assert top <= 1.2024 + (U[dtype] + 8 * (math.sqrt(n) + 3) * 2.0 ** -24) * 1.21 * math.sqrt(m), top
+    if steps <= 16:
+        want = orth64(x, [UPDATE[0]] * steps)
+        tol = 1.01 * (U[dtype] + 2.0 ** -24) * want.norm() + 1.21 * math.sqrt(m) * (1.1 * 2.0 ** -24 * 4.0 ** (steps - 11) +
+                                                                                   2 * (math.sqrt(n) + 3) * 2.0 ** -53 * 4.0 ** steps)
+        if dtype is F16:
+            tol = tol + 2.0 ** -25 * math.sqrt(rows * cols)
+        if n > 128 or steps > 24:
+            assert (y - want).norm() <= tol, ((y - want).norm().item(), tol.item())
