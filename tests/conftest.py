@@ -8,6 +8,36 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 
+def _keep_large_matrices():
+    """The full-size cases ask for the same few synthetic matrices again and again, half a minute of host time each: the last three of more than
+    1e9 elements are kept, every caller gets a copy. (Here, before any test module takes the function by its name.)"""
+    import functools
+    import inspect
+
+    from sclens_amd import synth
+
+    generate, kept = synth.synth_counts, {}
+    signature = inspect.signature(generate)
+
+    @functools.wraps(generate)
+    def synth_counts(N, M, *args, **kw):
+        if N * M < 10 ** 9:
+            return generate(N, M, *args, **kw)
+        call = signature.bind(N, M, *args, **kw)
+        call.apply_defaults()
+        key = tuple(call.arguments.items())
+        if key not in kept:
+            while len(kept) > 2:
+                kept.pop(next(iter(kept)))
+            kept[key] = generate(N, M, *args, **kw)
+        return kept[key].copy()
+
+    synth.synth_counts = synth_counts
+
+
+_keep_large_matrices()
+
+
 def _usable_cpus():
     """CPUs this process may really use: affinity and cgroup quota (the GPU box shows 256 CPUs with a quota of 16)."""
     n = len(os.sched_getaffinity(0)) if hasattr(os, "sched_getaffinity") else (os.cpu_count() or 1)
