@@ -553,8 +553,8 @@ static int orth_chunk(Ctx* ctx, hipStream_t st, const OrthArgs& a, void* ws, int
     const Mat i0 = tall && f32 ? XT[0] : X[0], i1 = tall && f32 ? X[0] : XT[0];
 #define SCL_START(T, I)                                                                                                             \
   do {                                                                                                                              \
-    SCL_RUN(ctx, k_sumsq<T>, g1, blk, 0, st, src, a.rows, a.cols, tpr, part);                                                 \
-    SCL_RUN(ctx, k_orth_start<T, I>, g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                \
+    SCL_RUN(ctx, k_sumsq<T>, g1, blk, 0, st, src, a.rows, a.cols, tpr, part);                                                       \
+    SCL_RUN(ctx, k_orth_start<T, I>, g2, blk, 0, st, src, a.rows, a.cols, part, nparts, a.eps, s_x, i0, i1);                        \
   } while (0)
     if (f32) SCL_START(D_F32, D_PL3);
     else if (wide) SCL_START(D_F32, D_F32);

@@ -559,19 +559,20 @@ static double largest_quadratic(double a, double b, double c, double L) {
   }
   return v;
 }
-// The steps from `first` on that one run may take, singular values of at most *bound before and after. The rounding of A, m half steps of fp64 of
-// bound^2, must not pass 2^-8 before the last of them. A step takes an eigenvalue l to l q(l)^2, q(l) = a + b l + c l^2, and an
-// error there to q(l) (a + 3 b l + 5 c l^2) times itself (outside the eigenvalues' range, next to zero, to q(l)^2). Low-rank matrices on
-// which this was tried in fp64: where the bound is 1e-3 (eleven steps of 3.4445, -4.7750, 2.0315) the result is off by 3e-9, at 8e4
-// (18 steps) by 5e3, then infinite. One step is the definition and always fits.
+// The steps from `first` on that one run may take, singular values of at most *bound before and after. What A is off by, m half steps of fp64 of
+// bound^2 from every step's rounding, must not pass 2^-8 before the last of them. A step takes an eigenvalue l to l q(l)^2,
+// q(l) = a + b l + c l^2, and an error there to q(l) (a + 3 b l + 5 c l^2) times itself (outside the eigenvalues' range, next to zero, to q(l)^2).
+// Low-rank matrices on which this was tried in fp64: where the bound is 1e-3 (eleven steps of 3.4445, -4.7750, 2.0315) the result is off by
+// 3e-9, at 8e4 (18 steps) by 5e3, then infinite. One step is the definition and always fits.
 static int orth_run(const OrthArgs& o, int first, double* bound) {
-  double err = (double)std::min(o.rows, o.cols) * 0x1p-53 * *bound * *bound;
+  const double rounding = (double)std::min(o.rows, o.cols) * 0x1p-53;
+  double err = rounding * *bound * *bound;
   int n = 0;
   while (first + n < o.steps && n < MAX_RIDE && (n == 0 || err < 0x1p-8)) {
     const double* c = o.coef + 3 * (first + n);
     const double L = *bound * *bound, q = largest_quadratic(c[0], c[1], c[2], L), dp = largest_quadratic(c[0], 3 * c[1], 5 * c[2], L);
-    err *= std::max(1.0, q * std::max(q, dp));
     *bound = orth_step_bound(c[0], c[1], c[2], *bound);
+    err = err * q * std::max(q, dp) + rounding * *bound * *bound;
     ++n;
   }
   return n;

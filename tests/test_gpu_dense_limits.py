@@ -519,3 +519,13 @@ def test_orthogonalize_low_rank_in_runs(dense, steps, rows, cols, rank, dtype):
             tol = tol + 2.0 ** -25 * math.sqrt(rows * cols)
         if n > 128 or steps > 24:
             assert (y - want).norm() <= tol, ((y - want).norm().item(), tol.item())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(40, 900), (3000, 12)])
+def test_short_side_schedules_that_shrink_and_grow_back(dense, rows, cols, dtype):
+    """one run of the m x m side in fp64, however small x is in between: 24 factors and their product, the norm, the result's rounding"""
+    x = torch.randn(rows, cols, generator=gen_for("shrink", rows, cols), device="cuda").to(dtype)
+    y = dense.orthogonalize(x, coefficients=[(1e-4, 0.0, 0.0)] * 12 + [(1e4, 0.0, 0.0)] * 12).double()
+    want = x.double() / (x.double().norm() + 1e-7)
+    assert ((y - want).abs() <= (U[dtype] + 2.0 ** -24) * 1.01 * want.abs() + (2.0 ** -25 if dtype is F16 else 0)).all()
